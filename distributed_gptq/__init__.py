@@ -9,7 +9,7 @@ isinstance checks and monkeypatching agree under both names):
 
     distributed_gptq                         -> distributed_gptq_amd
     distributed_gptq.core(.gptq|.quantizer|.dequantizer)
-    distributed_gptq.models(.layers)
+    distributed_gptq.models(.layers|.attention)
     distributed_gptq.kernels(.triton_kernels)
 
 The reference's multi-process coordinator (``DistributedGPTQCoordinator``,
@@ -24,10 +24,11 @@ from distributed_gptq_amd import models as _models
 from distributed_gptq_amd.core import dequantizer as _dequantizer
 from distributed_gptq_amd.core import gptq as _gptq
 from distributed_gptq_amd.core import quantizer as _quantizer
+from distributed_gptq_amd.models import attention as _attention
 from distributed_gptq_amd.models import layers as _layers
 
 for _name, _mod in {"core": _core, "core.gptq": _gptq, "core.quantizer": _quantizer,
-                    "core.dequantizer": _dequantizer, "models": _models, "models.layers": _layers,
+                    "core.dequantizer": _dequantizer, "models": _models, "models.layers": _layers, "models.attention": _attention,
                     "kernels": _kernels, "kernels.triton_kernels": _kernels}.items():
     sys.modules[f"{__name__}.{_name}"] = _mod
 

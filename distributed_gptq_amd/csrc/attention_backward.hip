@@ -1,0 +1,481 @@
+// Gradients of the attention of packed sequences on gfx950 MFMA.  With the
+// forward pass' weights p_ij = 2^(c q_i k_j - lse_i) and g = dL/do:
+//   delta_i = g_i o_i (o to about 16 bits),  ds_ij = p_ij (g_i v_j - delta_i),
+//   dv_j = sum_i p_ij g_i,  dk_j = scale sum_i ds_ij q_i,  dq_i = scale sum_j ds_ij k_j,
+// sums over the query heads of a key head included.  The weights are computed
+// again from the scores, in one kernel per key (dk, dv) and one per query (dq):
+// seven products of tiles instead of five, but every sum is made in one place
+// and in one order, so that the gradients are the same from call to call.
+#include "attn_tile.hpp"
+
+namespace gptq {
+namespace {
+
+constexpr int kRows = 64;        // packed query rows, or keys, of a tile
+constexpr int kMaxima = 1024;    // workgroups of the first kernel
+
+struct BackArgs {
+  AttnArgs f;                    // q, k, v, offsets, sizes; lse as input
+  Rows16 g;                      // dL/do
+  const uint16_t *o, *o_rest;    // (T, H, D): the output, and what its rounding left
+  float* delta;                  // (T, H)
+  float* maxima;                 // 2 x kMaxima: largest |g_i|^2 and |v_j|^2 of each workgroup (fp16)
+  float scale;
+  uint16_t *dq, *dk, *dv;        // contiguous
+};
+
+// fp16 ends at 2^-24, far above the ds of a long row (p alone is 1 / length):
+// ds is multiplied by 2^e before it is rounded, and the sum by 2^-e.  With
+// |ds_ij| <= 2 max |g_i| max |v_j|, e is the largest that keeps ds below 2^14.
+// p is multiplied by 2^14.  bf16 has fp32's exponents and needs neither.
+constexpr float kWeightShift = 14.0f;
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m));
+  return v;
+}
+
+// e for all of a kernel's ds, by all threads of a workgroup (one barrier)
+__device__ __forceinline__ float ds_shift(const BackArgs& a, float (*room)[4]) {
+  float g = 0.0f, v = 0.0f;
+#pragma unroll
+  for (int x = 0; x < kMaxima / 256; ++x) {
+    g = fmaxf(g, a.maxima[256 * x + threadIdx.x]);
+    v = fmaxf(v, a.maxima[kMaxima + 256 * x + threadIdx.x]);
+  }
+  g = wave_max(g);
+  v = wave_max(v);
+  if ((threadIdx.x & 63) == 0) room[0][threadIdx.x >> 6] = g, room[1][threadIdx.x >> 6] = v;
+  __syncthreads();
+  g = fmaxf(fmaxf(room[0][0], room[0][1]), fmaxf(room[0][2], room[0][3]));
+  v = fmaxf(fmaxf(room[1][0], room[1][1]), fmaxf(room[1][2], room[1][3]));
+  const float bound = 2.0f * sqrtf(g) * sqrtf(v);
+  if (!(bound > 0.0f && bound < 1e30f)) return 0.0f;
+  const float e = floorf(14.0f - log2f(bound));
+  return e < -100.0f ? -100.0f : e > 100.0f ? 100.0f : e;
+}
+
+// delta, and for fp16 the maxima.  16 lanes a row, 8 values a lane.
+template <bool kBF16>
+__global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
+  const int sub = threadIdx.x & 15, d = 8 * sub;
+  // (rows past the offsets have no gradient, and may hold anything)
+  const int64_t rows = static_cast<int64_t>(first_row(a.f.cu_q, a.f.B, a.f.B, a.f.T)) * a.f.H;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 16;
+  float most[2] = {0.0f, 0.0f};
+  auto values = [&](const uint16_t* p, float (&x)[8]) {
+    const u32x4 w = d < a.f.D ? *reinterpret_cast<const u32x4*>(p + d) : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = value16<kBF16>(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
+  };
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); row < rows; row += step) {
+    const int64_t t = row / a.f.H;
+    const int h = static_cast<int>(row - t * a.f.H);
+    float g[8], o[8], rest[8];
+    values(a.g.p + t * a.g.st + h * a.g.sh, g);
+    values(a.o + row * a.f.D, o);
+    values(a.o_rest + row * a.f.D, rest);
+    float dot = 0.0f, sq = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) dot = fmaf(g[e], o[e] + rest[e], dot), sq = fmaf(g[e], g[e], sq);
+#pragma unroll
+    for (int m = 8; m; m >>= 1) dot += __shfl_xor(dot, m), sq += __shfl_xor(sq, m);
+    if (sub == 0) a.delta[row] = dot;
+    most[0] = fmaxf(most[0], sq);
+  }
+  if constexpr (!kBF16) {
+    const int64_t vrows = static_cast<int64_t>(first_row(a.f.cu_k, a.f.B, a.f.B, a.f.S)) * a.f.Hk;
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); row < vrows; row += step) {
+      const int64_t t = row / a.f.Hk;
+      float v[8], sq = 0.0f;
+      values(a.f.v.p + t * a.f.v.st + (row - t * a.f.Hk) * a.f.v.sh, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq = fmaf(v[e], v[e], sq);
+#pragma unroll
+      for (int m = 8; m; m >>= 1) sq += __shfl_xor(sq, m);
+      most[1] = fmaxf(most[1], sq);
+    }
+    __shared__ float room[2][4];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const float w = wave_max(most[x]);
+      if ((threadIdx.x & 63) == 0) room[x][threadIdx.x >> 6] = w;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2)
+      a.maxima[threadIdx.x * kMaxima + blockIdx.x] =
+          fmaxf(fmaxf(room[threadIdx.x][0], room[threadIdx.x][1]), fmaxf(room[threadIdx.x][2], room[threadIdx.x][3]));
+  }
+}
+
+// 32 columns' channels to memory: y = x * r, rounded
+template <bool kBF16, int DT>
+__device__ __forceinline__ void store_rows(uint16_t* row, const f32x16 (&x)[DT / 32], float r, int D, int half) {
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * db + acc_row(i, half);
+      if (d < D)
+        *reinterpret_cast<u32x2*>(row + d) =
+            u32x2{pack16<kBF16>(x[db][i] * r, x[db][i + 1] * r), pack16<kBF16>(x[db][i + 2] * r, x[db][i + 3] * r)};
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void load_operand(u32x4 (&x)[DT / 16], const uint16_t* row, bool inside, int D, int half) {
+#pragma unroll
+  for (int s = 0; s < DT / 16; ++s) {
+    const int d = 16 * s + 8 * half;
+    x[s] = inside && d < D ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
+  }
+}
+
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_back_a0[kRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_back_a1[kRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_back_b0[kRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_back_b1[kRows * DT * 2];
+
+// dq: as the forward pass, 32 packed rows a wave (a lane's column), tiles of 64
+// keys and values in LDS.
+template <bool kBF16, int DT>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slots) {
+  constexpr int R = 128, W = kRows / 4;
+  __shared__ float room[2][4];
+  const AttnArgs& a = args.f;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int G = static_cast<int>(a.G.d);
+  const int hk = blockIdx.x % a.Hk;
+  int tile;
+  const int b = find_seq(a.cu_q, a.B, a.T, G, R, slots - 1 - static_cast<int>(blockIdx.x / a.Hk), &tile);
+  const Seq s = seq_of<false>(a, b);
+  const int rows = s.Lq * G;
+  if (tile * R >= rows) return;
+  float shift = 0.0f;
+  if constexpr (!kBF16) shift = ds_shift(args, room);
+  const float up = exp2f(shift);
+
+  const int r = tile * R + wave * 32 + (lane & 31);
+  const bool inside = r < rows;
+  const int tok = div_by(inside ? r : rows - 1, a.G);
+  const int head = hk * G + ((inside ? r : rows - 1) - tok * G);
+  const int limit = last_key(a, s, tok);
+  const int first_r = tile * R + wave * 32;
+  const int full = last_key(a, s, div_by(first_r < rows ? first_r : rows - 1, a.G));
+  const int last_r = (tile + 1) * R < rows ? (tile + 1) * R - 1 : rows - 1;
+  const int wave_r = first_r + 31 < rows ? first_r + 31 : rows - 1;
+  const int wave_end = first_r < rows ? last_key(a, s, div_by(wave_r, a.G)) + 1 : 0;
+  const int last = last_key(a, s, div_by(last_r, a.G));
+  const int tiles = last < 0 ? 0 : last / kRows + 1;
+
+  const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
+  u32x4 q[DT / 16], g[DT / 16];
+  load_operand<DT>(q, a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh, inside, a.D, half);
+  load_operand<DT>(g, args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh, inside, a.D, half);
+  const float lse = a.lse[row], delta = args.delta[row];
+
+  f32x16 acc[DT / 32];
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db) acc[db] = zero16();
+
+  KvAt at = kv_at<false>(a, s, wave * W + lane % W);
+  auto fetch = [&](int t, uint8_t* kt, uint8_t* vt) {
+    at.at = s.k0 + t * kRows + wave * W + lane % W;
+    fetch_rows<DT, W, false>(a, hk, at, t * kRows, wave * W, s.Lk, kt, vt, lane);
+  };
+  auto use = [&](int t, const lds_u8* kt, const lds_u8* vt) {
+    const int key0 = t * kRows;
+    if (key0 >= wave_end) return;
+    const bool masked = key0 + kRows - 1 > full;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+      for (int d = 0; d < DT / 16; ++d) {
+        sc = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, lane), q[d], sc);
+        dp = mma32<kBF16>(row_operand<DT>(vt, 32 * n, d, lane), g[d], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, -lse));
+        sc[i] = p * (dp[i] - delta) * up;
+      }
+      if (masked) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (key0 + 32 * n + acc_row(i, half) > limit) sc[i] = 0.0f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        const u32x4 x = operand_of<kBF16>(sc, 8 * ks);
+#pragma unroll
+        for (int db = 0; db < DT / 32; ++db)
+          acc[db] = mma32<kBF16>(column_operand<DT>(kt, 32 * n + 16 * ks, db, lane), x, acc[db]);
+      }
+    }
+  };
+  if (tiles > 0) {
+    fetch(0, g_back_a0<DT>, g_back_b0<DT>);
+    __syncthreads();
+    for (int t = 0; t < tiles; t += 2) {
+      if (t + 1 < tiles) fetch(t + 1, g_back_a1<DT>, g_back_b1<DT>);
+      use(t, (const lds_u8*)&g_back_a0<DT>[0], (const lds_u8*)&g_back_b0<DT>[0]);
+      __syncthreads();
+      if (t + 1 >= tiles) break;
+      if (t + 2 < tiles) fetch(t + 2, g_back_a0<DT>, g_back_b0<DT>);
+      use(t + 1, (const lds_u8*)&g_back_a1<DT>[0], (const lds_u8*)&g_back_b1<DT>[0]);
+      __syncthreads();
+    }
+  }
+  if (inside) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale * exp2f(-shift), a.D, half);
+}
+
+// dk and dv: a workgroup has 64 keys and passes tiles of 64 packed query rows
+// and their gradients through LDS, with each row's lse, delta and last key.
+// Wave w has keys 32 (w % 2) .. (a lane's column) and each tile's rows
+// 32 (w / 2) ..; the two waves of a key are joined at the end.  (With all four
+// waves on keys of their own, 128 to a workgroup, the workgroups of the first
+// keys, which all queries see, ran twice as long as the average.)
+template <bool kBF16, int DT>
+__global__ __launch_bounds__(256, DT == 128 ? 1 : 2) void attn_dkv_kernel(BackArgs args) {
+  constexpr int R = 64, W = kRows / 4, CH = DT / 8, RPI = 64 / CH;
+  __shared__ float room[2][4];
+  __shared__ __attribute__((aligned(16))) float stats[2][2][kRows];
+  __shared__ __attribute__((aligned(16))) int limits[2][kRows];
+  const AttnArgs& a = args.f;
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int G = static_cast<int>(a.G.d);
+  const int hk = blockIdx.x % a.Hk;
+  int tile;
+  const int b = find_seq(a.cu_k, a.B, a.S, 1, R, static_cast<int>(blockIdx.x / a.Hk), &tile);
+  Seq s = seq_of<false>(a, b);
+  if (b == a.B) {  // rows past the offsets
+    s.Lk = a.S - s.k0;
+    s.Lq = 0;
+  }
+  if (tile * R >= s.Lk) return;
+  float shift = 0.0f;
+  if constexpr (!kBF16) shift = ds_shift(args, room);
+  const float up = exp2f(kBF16 ? 0.0f : shift - kWeightShift);
+
+  const int rows = s.Lq * G;
+  const int key0 = tile * R, kw = key0 + 32 * (wave & 1), n = wave >> 1;
+  const int key = kw + (lane & 31);
+  const bool inside = key < s.Lk;
+  const int off = s.Lk - s.Lq;
+  // the first token that sees the workgroup's first key
+  const int i0 = a.causal && key0 > off ? key0 - off : 0;
+  const int t0 = (i0 < s.Lq ? i0 * G : rows) / kRows, t1 = (rows + kRows - 1) / kRows;
+
+  u32x4 kf[DT / 16], vf[DT / 16];
+  {
+    const int64_t kr = s.k0 + (inside ? key : 0);
+    load_operand<DT>(kf, a.k.p + kr * a.k.st + hk * a.k.sh, inside, a.D, half);
+    load_operand<DT>(vf, a.v.p + kr * a.v.st + hk * a.v.sh, inside, a.D, half);
+  }
+  f32x16 dk[DT / 32], dv[DT / 32];
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db) dk[db] = zero16(), dv[db] = zero16();
+
+  float n_lse = 0.0f, n_delta = 0.0f;
+  int n_limit = -1;
+  auto fetch = [&](int t, uint8_t* qt, uint8_t* gt) {
+#pragma unroll
+    for (int x = 0; x < W / RPI; ++x) {
+      const int i = wave * W + x * RPI + lane / CH;
+      const int r = t * kRows + i;
+      const int ch = (lane % CH) ^ row_slot<DT>(i);
+      const bool in = r < rows && ch * 8 < a.D;
+      const int tok = div_by(in ? r : 0, a.G);
+      const int head = hk * G + ((in ? r : 0) - tok * G);
+      const uint16_t* qp = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh + ch * 8;
+      const uint16_t* gp = args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh + ch * 8;
+      copy16_to_lds(in ? static_cast<const void*>(qp) : g_attn_zeros, qt + (wave * (W / RPI) + x) * 1024);
+      copy16_to_lds(in ? static_cast<const void*>(gp) : g_attn_zeros, gt + (wave * (W / RPI) + x) * 1024);
+    }
+    if (wave == 0) {
+      const int r = t * kRows + lane;
+      n_limit = -1;
+      n_lse = n_delta = 0.0f;
+      if (r < rows) {
+        const int tok = div_by(r, a.G);
+        const int64_t at = static_cast<int64_t>(s.q0 + tok) * a.H + hk * G + (r - tok * G);
+        n_lse = a.lse[at];
+        n_delta = args.delta[at];
+        n_limit = last_key(a, s, tok);
+      }
+    }
+  };
+  auto keep = [&](int buf) {
+    if (wave == 0) {
+      stats[buf][0][lane] = n_lse;
+      stats[buf][1][lane] = n_delta;
+      limits[buf][lane] = n_limit;
+    }
+  };
+  auto use = [&](int t, int buf, const lds_u8* qt, const lds_u8* gt) {
+    const int r0 = t * kRows + 32 * n;
+    if (r0 >= rows) return;
+    const int r1 = r0 + 31 < rows ? r0 + 31 : rows - 1;
+    if (last_key(a, s, div_by(r1, a.G)) < kw) return;  // no row of these sees a key of the wave
+    const bool masked = r0 + 31 >= rows || last_key(a, s, div_by(r0, a.G)) < kw + 31;
+    f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+    for (int d = 0; d < DT / 16; ++d) {
+      sc = mma32<kBF16>(row_operand<DT>(qt, 32 * n, d, lane), kf[d], sc);
+      dp = mma32<kBF16>(row_operand<DT>(gt, 32 * n, d, lane), vf[d], dp);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * n + 8 * j + 4 * half]);
+      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * n + 8 * j + 4 * half]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 4 * j + e;
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, (kBF16 ? 0.0f : kWeightShift) - lse[e]));
+        dp[i] = p * (dp[i] - delta[e]) * up;
+        sc[i] = p;
+      }
+      if (masked) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const i32x4 lim = *reinterpret_cast<const i32x4*>(&limits[buf][32 * n + 8 * j + 4 * half]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key > lim[e]) sc[4 * j + e] = 0.0f, dp[4 * j + e] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const u32x4 p = operand_of<kBF16>(sc, 8 * ks), x = operand_of<kBF16>(dp, 8 * ks);
+#pragma unroll
+      for (int db = 0; db < DT / 32; ++db) {
+        dv[db] = mma32<kBF16>(column_operand<DT>(gt, 32 * n + 16 * ks, db, lane), p, dv[db]);
+        dk[db] = mma32<kBF16>(column_operand<DT>(qt, 32 * n + 16 * ks, db, lane), x, dk[db]);
+      }
+    }
+  };
+  if (t0 < t1) {
+    fetch(t0, g_back_a0<DT>, g_back_b0<DT>);
+    keep(0);
+    __syncthreads();
+    for (int t = t0; t < t1; t += 2) {
+      if (t + 1 < t1) fetch(t + 1, g_back_a1<DT>, g_back_b1<DT>);
+      use(t, 0, (const lds_u8*)&g_back_a0<DT>[0], (const lds_u8*)&g_back_b0<DT>[0]);
+      keep(1);
+      __syncthreads();
+      if (t + 1 >= t1) break;
+      if (t + 2 < t1) fetch(t + 2, g_back_a0<DT>, g_back_b0<DT>);
+      use(t + 1, 1, (const lds_u8*)&g_back_a1<DT>[0], (const lds_u8*)&g_back_b1<DT>[0]);
+      keep(0);
+      __syncthreads();
+    }
+  }
+  // (the tiles are done with: the last barrier is behind every wave's reads)
+  lds_f32* sum_k = (lds_f32*)((wave & 1) ? &g_back_a1<DT>[0] : &g_back_a0<DT>[0]);
+  lds_f32* sum_v = (lds_f32*)((wave & 1) ? &g_back_b1<DT>[0] : &g_back_b0<DT>[0]);
+  if (n == 1) {
+#pragma unroll
+    for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        sum_k[(16 * db + i) * 64 + lane] = dk[db][i];
+        sum_v[(16 * db + i) * 64 + lane] = dv[db][i];
+      }
+  }
+  __syncthreads();
+  if (n == 1 || !inside) return;
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      dk[db][i] += sum_k[(16 * db + i) * 64 + lane];
+      dv[db][i] += sum_v[(16 * db + i) * 64 + lane];
+    }
+  const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
+  store_rows<kBF16, DT>(args.dk + row, dk, args.scale * exp2f(-shift), a.D, half);
+  store_rows<kBF16, DT>(args.dv + row, dv, exp2f(kBF16 ? 0.0f : -kWeightShift), a.D, half);
+}
+
+template <bool kBF16, int DT>
+int launch(const BackArgs& a, hipStream_t st) {
+  const int64_t qs = slots_of(a.f.cu_q, a.f.B, a.f.T, a.f.G.d, 128), ks = slots_of(a.f.cu_k, a.f.B, a.f.S, 1, 64);
+  GPTQ_REQUIRE(qs * a.f.Hk < (int64_t{1} << 31) && ks * a.f.Hk < (int64_t{1} << 31), GPTQ_ERR_SHAPE,
+               "gptq_attention_backward: too many rows");
+  attn_delta_kernel<kBF16><<<kMaxima, 256, 0, st>>>(a);
+  int rc = check_launch("gptq_attention_backward");
+  if (rc != GPTQ_OK) return rc;
+  if (a.f.S > 0) attn_dkv_kernel<kBF16, DT><<<static_cast<uint32_t>(ks * a.f.Hk), 256, 0, st>>>(a);
+  rc = check_launch("gptq_attention_backward");
+  if (rc != GPTQ_OK) return rc;
+  if (a.f.T > 0)
+    attn_dq_kernel<kBF16, DT><<<static_cast<uint32_t>(qs * a.f.Hk), 256, 0, st>>>(a, static_cast<int>(qs));
+  return check_launch("gptq_attention_backward");
+}
+
+}  // namespace
+}  // namespace gptq
+
+using namespace gptq;
+
+extern "C" size_t gptq_attention_backward_workspace_size(int64_t T, int64_t H) {
+  if (T < 0 || H < 1) return 0;
+  return plan::add_sat(plan::mul_sat(plan::mul_sat(static_cast<size_t>(T), static_cast<size_t>(H)), sizeof(float)),
+                       2 * kMaxima * sizeof(float));
+}
+
+extern "C" int gptq_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                       const void* out_rest, const float* lse, int dtype, int64_t g_token, int64_t g_head, int64_t q_token,
+                                       int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                                       const int32_t* cu_q, const int32_t* cu_k, int64_t B, int64_t T, int64_t S,
+                                       int64_t H, int64_t Hk, int64_t D, int causal, float scale, void* dq, void* dk,
+                                       void* dv, void* workspace, size_t workspace_bytes, gptq_stream_t stream) {
+  clear_error();
+  int rc = plan::check_attention_args("gptq_attention_backward", dtype, B, T, S, H, Hk, D, scale);
+  if (rc != GPTQ_OK) return rc;
+  if (T == 0 && S == 0) return GPTQ_OK;
+  GPTQ_REQUIRE((T == 0 || (grad && q && out && out_rest && lse && dq)) && (S == 0 || (k && v && dk && dv)), GPTQ_ERR_ARG,
+               "gptq_attention_backward: null pointer");
+  GPTQ_REQUIRE(B == 1 || (cu_q && cu_k), GPTQ_ERR_ARG,
+               "gptq_attention_backward: %lld sequences without their offsets", static_cast<long long>(B));
+  const int64_t strides[] = {g_token, g_head, q_token, q_head, k_token, k_head, v_token, v_head};
+  rc = plan::check_attention_layout("gptq_attention_backward", q, k, v, strides, 8);
+  if (rc != GPTQ_OK) return rc;
+  rc = plan::check_attention_layout("gptq_attention_backward", grad, out, out_rest, strides, 2);
+  if (rc != GPTQ_OK) return rc;
+  const size_t need = gptq_attention_backward_workspace_size(T, H);
+  GPTQ_REQUIRE(workspace && workspace_bytes >= need, GPTQ_ERR_WORKSPACE,
+               "gptq_attention_backward: workspace of %zu bytes, needs %zu", workspace_bytes, need);
+  BackArgs a{};
+  a.f.q = {static_cast<const uint16_t*>(q), q_token, q_head};
+  a.f.k = {static_cast<const uint16_t*>(k), k_token, k_head};
+  a.f.v = {static_cast<const uint16_t*>(v), v_token, v_head};
+  a.g = {static_cast<const uint16_t*>(grad), g_token, g_head};
+  a.o = static_cast<const uint16_t*>(out);
+  a.o_rest = static_cast<const uint16_t*>(out_rest);
+  a.f.lse = const_cast<float*>(lse);
+  a.f.cu_q = cu_q;
+  a.f.cu_k = cu_k;
+  a.f.B = static_cast<int>(B), a.f.T = static_cast<int>(T), a.f.S = static_cast<int>(S);
+  a.f.H = static_cast<int>(H), a.f.Hk = static_cast<int>(Hk), a.f.D = static_cast<int>(D);
+  a.f.G = fast_div(static_cast<uint32_t>(H / Hk));
+  a.f.causal = causal != 0;
+  a.f.c = scale * kLog2e;
+  a.scale = scale;
+  a.f.splits = 1;
+  a.maxima = static_cast<float*>(workspace);
+  a.delta = a.maxima + 2 * kMaxima;
+  a.dq = static_cast<uint16_t*>(dq);
+  a.dk = static_cast<uint16_t*>(dk);
+  a.dv = static_cast<uint16_t*>(dv);
+  const bool wide = D > 64;
+  const hipStream_t st = as_hip(stream);
+  if (dtype == GPTQ_BF16) return wide ? launch<true, 128>(a, st) : launch<true, 64>(a, st);
+  return wide ? launch<false, 128>(a, st) : launch<false, 64>(a, st);
+}

@@ -1,0 +1,300 @@
+// What the attention kernels share: 32x32 MFMA tiles fed from swizzled LDS
+// rows, direct-to-LDS copies of key and value rows, the packed-row and paged
+// addressing, and the bounds of the causal mask.
+//
+// Every product is laid out so that a lane's accumulators belong to one column
+// (lane % 32), a query in the forward and dQ kernels, a key in the dK/dV
+// kernel: softmax statistics then are one value a lane, and the weights that
+// one product leaves in a lane's registers are the next product's operand
+// without moving between lanes.  With a 32x32x16 MFMA a lane ends with rows
+// 8 (i / 4) + 4 (lane / 32) + i % 4 of its column (i < 16), and as an operand
+// it gives 8 values of the contraction; both operands of the second product
+// take the contraction in that same order, so the order needs no shuffle.
+#pragma once
+
+#include "common.hpp"
+#include "mfma_lds.hpp"
+
+namespace gptq {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) float lds_f32;
+typedef __attribute__((address_space(1))) const void gbl_void;
+
+constexpr float kLog2e = 1.4426950408889634f;
+// what a running maximum starts from: finite, so that differences with it are
+// never NaN, and below every score
+constexpr float kLowest = -3.0e38f;
+
+// ------------------------------------------------------------ division ----
+// n / d for 0 <= n < 2^31 by a product: m = ceil(2^(31 + s) / d) with
+// s = ceil(log2 d) (Granlund and Montgomery, "Division by invariant integers
+// using multiplication")
+struct FastDiv {
+  uint32_t d, m, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t s = 0;
+  while ((uint64_t{1} << s) < d) ++s;
+  return FastDiv{d, static_cast<uint32_t>(((uint64_t{1} << (31 + s)) + d - 1) / d), 31 + s};
+}
+__device__ __forceinline__ int div_by(int n, const FastDiv& f) {
+  return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * f.m) >> f.shift);
+}
+
+// ---------------------------------------------------------- element types ----
+template <bool kBF16>
+__device__ __forceinline__ f32x16 mma32(const u32x4& a, const u32x4& b, const f32x16& c) {
+  if constexpr (kBF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                   0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+template <bool kBF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  return kBF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+}
+template <bool kBF16>
+__device__ __forceinline__ float value16(uint16_t b) {
+  return kBF16 ? bf16_bits_to_f32(b) : f16_bits_to_f32(b);
+}
+// the 8 values i0 .. i0 + 7 of a lane's accumulators as an operand
+template <bool kBF16>
+__device__ __forceinline__ u32x4 operand_of(const f32x16& p, int i0) {
+  return u32x4{pack16<kBF16>(p[i0], p[i0 + 1]), pack16<kBF16>(p[i0 + 2], p[i0 + 3]),
+               pack16<kBF16>(p[i0 + 4], p[i0 + 5]), pack16<kBF16>(p[i0 + 6], p[i0 + 7])};
+}
+// and what its rounding left, as an operand too
+template <bool kBF16>
+__device__ __forceinline__ u32x4 operand_rest(const f32x16& p, int i0, const u32x4& x) {
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r[j] = pack16<kBF16>(p[i0 + 2 * j] - value16<kBF16>(static_cast<uint16_t>(x[j])),
+                         p[i0 + 2 * j + 1] - value16<kBF16>(static_cast<uint16_t>(x[j] >> 16)));
+  return r;
+}
+// row of the 32 x 32 result that register i of this lane holds
+__device__ __forceinline__ int acc_row(int i, int half) { return 8 * (i >> 2) + 4 * half + (i & 3); }
+
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.0f;
+  return z;
+}
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+
+// ------------------------------------------------------------------- LDS ----
+// A tile row holds DT 16-bit values in 16-byte chunks, chunk c at slot
+// c ^ row_slot(row).  A 128-bit read of 32 rows at one chunk then meets 16
+// distinct quads of banks 16 lanes at a time, and a transposing read of 4 rows
+// x 32 values 4 distinct rows of quads (the low two bits of the row are the
+// slot's high bits).
+template <int DT>
+__device__ __forceinline__ int row_slot(int row) {
+  if constexpr (DT == 128)
+    return ((row & 3) << 2) | ((row >> 2) & 3);
+  else
+    return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+}
+
+// Operand of a product over the row's values: lane l gives row l % 32 (+ the
+// tile's first row), values 16 s + 8 (l / 32) .. + 7.
+template <int DT>
+__device__ __forceinline__ u32x4 row_operand(const lds_u8* tile, int row0, int s, int lane) {
+  const int r = lane & 31;
+  return *(const lds_u32x4*)(tile + (row0 + r) * (DT * 2) + (((2 * s + (lane >> 5)) ^ row_slot<DT>(r)) << 4));
+}
+
+// Operand of a product over the rows (the transposed tile): lane l gives value
+// 32 db + l % 32 of the rows row0 + 8 j + 4 (l / 32) + 0 .. 3, j = 0, 1.  A
+// transposing read takes from 16 lanes the addresses of 4 rows x 16 values, 4
+// values a lane, and gives lane i the 4 rows' value i.
+template <int DT>
+__device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, int db, int lane) {
+  const int i = lane & 15, h = lane >> 5;
+  const int chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  s16x4 v[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 8 * j + 4 * h + (i >> 2);
+    v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4*)(tile + (row0 + r) * (DT * 2) + ((chunk ^ row_slot<DT>(r)) << 4) + ((i & 1) << 3)));
+  }
+  return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// 16 bytes per lane from memory to LDS, lane l's at lds + 16 l.
+__device__ __forceinline__ void copy16_to_lds(const void* from, uint8_t* lds) {
+  __builtin_amdgcn_global_load_lds((gbl_void*)from, (lds_void*)lds, 16, 0, 0);
+}
+
+// what the copies of rows and channels outside the tensors read
+__device__ const uint32_t g_attn_zeros[4] = {0, 0, 0, 0};
+
+// ------------------------------------------------------------ the problem ----
+struct Rows16 {            // 16-bit rows of (token, head)
+  const uint16_t* p;
+  int64_t st, sh;          // strides of a token and of a head, in elements
+};
+
+struct Paged {
+  const int32_t* table;    // (B, width) page numbers
+  const int32_t* context;  // (B) cached tokens of each sequence
+  int64_t table_stride, k_page, v_page;  // elements
+  int most, pages;         // tokens that a table row reaches; pages of the cache
+  FastDiv page;            // tokens of a page
+};
+
+struct AttnArgs {
+  Rows16 q, k, v;
+  Paged paged;
+  const int32_t* cu_q;     // (B + 1) offsets, or null: B equal lengths
+  const int32_t* cu_k;
+  int B, T, S;             // sequences, packed queries, packed keys
+  int H, Hk, D;
+  FastDiv G;               // query heads of a key head
+  int causal;
+  float c;                 // scale * log2(e)
+  uint16_t* out;           // (T, H, D)
+  uint16_t* out_rest;      // (T, H, D): what the rounding of out left, for the gradient (or null)
+  float* lse;              // (T, H) or null: log2 of the sum of 2^(c q k)
+  float* part;             // with splits > 1: sums (splits, T H, D), then maxima, then sums of weights (splits, T H)
+  int splits;
+};
+
+// One sequence: its queries and keys.
+struct Seq {
+  int b, q0, Lq, k0, Lk;
+};
+
+__device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : v > hi ? hi : v; }
+
+// The first of sequence b's rows among `total`, those of B sequences.  Without
+// offsets the sequences are equally long (one sequence, or one token each).
+// With them the first is 0, rows past the last one are a sequence B of their
+// own (whose outputs are zeros), and offsets outside the tensor are clamped:
+// the kernels stay inside it.
+__device__ __forceinline__ int first_row(const int32_t* cu, int b, int B, int total) {
+  if (b == 0) return 0;
+  if (!cu) return b * (total / B);
+  return b > B ? total : clamp_int(__builtin_amdgcn_readfirstlane(cu[b]), 0, total);
+}
+
+// The sequence and tile of a slot, when a sequence of rows [r0, r1) takes the
+// slots from r0 / R + b on: at least ceil((r1 - r0) / R) of them, whatever the
+// lengths, so the host needs no lengths for the grid.  Rows are `per` to a
+// token.
+__device__ __forceinline__ int find_seq(const int32_t* cu, int B, int total, int per, int R, int slot, int* tile) {
+  int lo = 0, hi = B + (cu ? 1 : 0), start = 0;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    const int at = static_cast<int>(static_cast<int64_t>(first_row(cu, mid, B, total)) * per / R) + mid;
+    if (at <= slot) {
+      lo = mid;
+      start = at;
+    } else {
+      hi = mid;
+    }
+  }
+  *tile = slot - start;
+  return lo;
+}
+// what find_seq's grid needs
+inline int64_t slots_of(const int32_t* cu, int64_t B, int64_t total, int64_t per, int64_t R) {
+  return total * per / R + B + (cu ? 1 : 0);
+}
+
+template <bool kPaged>
+__device__ __forceinline__ Seq seq_of(const AttnArgs& a, int b) {
+  Seq s;
+  s.b = b;
+  s.q0 = first_row(a.cu_q, b, a.B, a.T);
+  const int qe = first_row(a.cu_q, b + 1, a.B, a.T);
+  s.Lq = qe > s.q0 ? qe - s.q0 : 0;
+  if constexpr (kPaged) {
+    s.k0 = 0;
+    s.Lk = b == a.B ? 0 : clamp_int(__builtin_amdgcn_readfirstlane(a.paged.context[b]), 0, a.paged.most);
+  } else {
+    s.k0 = first_row(a.cu_k, b, a.B, a.S);
+    const int ke = first_row(a.cu_k, b + 1, a.B, a.S);
+    s.Lk = ke > s.k0 ? ke - s.k0 : 0;
+    if (b == a.B) s.Lk = 0;
+  }
+  return s;
+}
+
+// the last key that query token i of the sequence sees (-1: none)
+__device__ __forceinline__ int last_key(const AttnArgs& a, const Seq& s, int i) {
+  const int last = a.causal ? i + s.Lk - s.Lq : s.Lk - 1;
+  return last < s.Lk ? last : s.Lk - 1;
+}
+
+// Where row `key` of a sequence's keys and values is: in the pages of a cache
+// (page number and place in it) or in the packed rows.  Page numbers outside
+// the cache are clamped.
+struct KvAt {
+  int page, at;
+};
+template <bool kPaged>
+__device__ __forceinline__ KvAt kv_at(const AttnArgs& a, const Seq& s, int key) {
+  if constexpr (kPaged) {
+    const int n = div_by(key, a.paged.page);
+    return KvAt{clamp_int(a.paged.table[s.b * a.paged.table_stride + n], 0, a.paged.pages - 1),
+                key - n * static_cast<int>(a.paged.page.d)};
+  } else {
+    return KvAt{0, s.k0 + key};
+  }
+}
+template <bool kPaged>
+__device__ __forceinline__ const uint16_t* kv_row(const Rows16& r, int64_t page_stride, int hk, KvAt k) {
+  const uint16_t* p = r.p + hk * r.sh + k.at * r.st;
+  if constexpr (kPaged) p += k.page * page_stride;
+  return p;
+}
+
+// Copies a wave's W consecutive rows of a tile (the first of them row `row0` of
+// the tile) into LDS: keys and values, zeros past the sequence's end and past
+// D.  `mine` is where the row of lane % W is (row0 + lane % W).
+template <int DT, int W, bool kPaged>
+__device__ __forceinline__ void fetch_rows(const AttnArgs& a, int hk, KvAt mine, int key0, int row0, int end,
+                                           uint8_t* kt, uint8_t* vt, int lane) {
+  constexpr int CH = DT / 8, RPI = 64 / CH;
+#pragma unroll
+  for (int x = 0; x < W / RPI; ++x) {
+    const int i = x * RPI + lane / CH, row = row0 + i;
+    KvAt at = mine;
+    if constexpr (kPaged) {
+      at.page = __shfl(mine.page, i);
+      at.at = __shfl(mine.at, i);
+    } else {
+      at.at = mine.at - lane % W + i;
+    }
+    const int ch = (lane % CH) ^ row_slot<DT>(row);
+    const bool in = key0 + row < end && ch * 8 < a.D;
+    const uint16_t* kp = kv_row<kPaged>(a.k, a.paged.k_page, hk, at) + ch * 8;
+    const uint16_t* vp = kv_row<kPaged>(a.v, a.paged.v_page, hk, at) + ch * 8;
+    copy16_to_lds(in ? static_cast<const void*>(kp) : g_attn_zeros, kt + (row0 / RPI + x) * 1024);
+    copy16_to_lds(in ? static_cast<const void*>(vp) : g_attn_zeros, vt + (row0 / RPI + x) * 1024);
+  }
+}
+
+// kv_at of a key that may lie past the end (in a cache then the last one's)
+template <bool kPaged>
+__device__ __forceinline__ KvAt kv_at_clamped(const AttnArgs& a, const Seq& s, int key) {
+  if constexpr (!kPaged) return kv_at<kPaged>(a, s, key);
+  if (s.Lk == 0) return KvAt{0, 0};  // (no copy uses it)
+  return kv_at<kPaged>(a, s, clamp_int(key, 0, s.Lk - 1));
+}
+
+}  // namespace
+}  // namespace gptq

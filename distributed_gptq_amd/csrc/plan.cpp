@@ -249,6 +249,64 @@ int check_linear_args(const void* x, int x_dtype, int64_t M, const void* packed,
   return GPTQ_OK;
 }
 
+// ------------------------------------------------------------ attention ----
+
+namespace {
+bool attention_sizes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D) {
+  constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
+  return B >= 1 && T >= 0 && S >= 0 && H >= 1 && Hk >= 1 && H % Hk == 0 && D >= 8 && D <= 128 && D % 8 == 0 &&
+         H <= 65536 && B < kMost && S < kMost && T < kMost / H;
+}
+}  // namespace
+
+PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context) {
+  PagedPlan p;
+  if (!attention_sizes(B, T, 0, H, Hk, 8)) return p;
+  const int64_t rows = ceil_div(T * (H / Hk), B);  // of a sequence and key head, on average
+  p.few = rows <= 32;
+  const int64_t groups = (p.few ? ceil_div(rows, 32) : ceil_div(rows, 128)) * B * Hk;
+  const int64_t want = ceil_div(p.few ? 256 : 512, groups);
+  const int64_t most = ceil_div(std::max<int64_t>(max_context, 1), p.few ? 256 : 512);
+  p.splits = static_cast<int>(std::min<int64_t>({want, most, 128}));
+  return p;
+}
+
+size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context) {
+  if (!attention_sizes(B, T, 0, H, Hk, D)) return 0;
+  const PagedPlan p = paged_plan(B, T, H, Hk, max_context);
+  if (p.splits == 1) return 0;
+  return mul_sat(mul_sat(static_cast<size_t>(T * H), static_cast<size_t>(D + 2)), 4 * static_cast<size_t>(p.splits));
+}
+
+int64_t cached_most(int64_t width, int64_t page_size) {
+  constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
+  if (width <= 0 || page_size <= 0) return 0;
+  return width < kMost / page_size ? width * page_size : kMost;
+}
+
+int check_attention_args(const char* fn, int dtype, int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D,
+                         float scale) {
+  GPTQ_REQUIRE(dtype == GPTQ_F16 || dtype == GPTQ_BF16, GPTQ_ERR_DTYPE, "%s: expected fp16 or bf16", fn);
+  GPTQ_REQUIRE(H >= 1 && Hk >= 1 && H % Hk == 0, GPTQ_ERR_SHAPE, "%s: %lld query heads over %lld key heads", fn,
+               static_cast<long long>(H), static_cast<long long>(Hk));
+  GPTQ_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, GPTQ_ERR_SHAPE,
+               "%s: heads of %lld values (multiples of 8 up to 128 are supported)", fn, static_cast<long long>(D));
+  GPTQ_REQUIRE(attention_sizes(B, T, S, H, Hk, D), GPTQ_ERR_SHAPE,
+               "%s: %lld sequences, %lld queries, %lld keys, %lld heads", fn, static_cast<long long>(B),
+               static_cast<long long>(T), static_cast<long long>(S), static_cast<long long>(H));
+  GPTQ_REQUIRE(scale >= 1e-30f && scale <= 1e30f, GPTQ_ERR_ARG, "%s: scale %g (it has to lie in [1e-30, 1e30])", fn, scale);
+  return GPTQ_OK;
+}
+
+int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides, int n) {
+  GPTQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0,
+               GPTQ_ERR_ARG, "%s: q, k and v have to be 16-byte aligned", fn);
+  for (int i = 0; i < n; ++i)
+    GPTQ_REQUIRE(strides[i] % 8 == 0, GPTQ_ERR_SHAPE, "%s: strides have to be multiples of 8 elements (got %lld)", fn,
+                 static_cast<long long>(strides[i]));
+  return GPTQ_OK;
+}
+
 }  // namespace plan
 }  // namespace gptq
 

@@ -98,5 +98,22 @@ int check_linear_args(const void* x, int x_dtype, int64_t M, const void* packed,
                       const void* zeros, int sz_dtype, const int32_t* g_idx, int group_size, int64_t ngroups,
                       const void* bias, int bias_dtype, int64_t N, int64_t K, const void* y);
 
+// ------------------------------------------------------------ attention ----
+// How new tokens' attention over a paged cache runs: the kernel for few rows of
+// a key head (32 a workgroup) or for many (128), and into how many parts each
+// sequence's keys are cut.
+struct PagedPlan {
+  bool few = true;
+  int splits = 1;
+};
+PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context);
+size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context);
+// tokens that a row of `width` pages reaches, as far as the kernels count
+int64_t cached_most(int64_t width, int64_t page_size);
+// argument checks of the attention entry points (a gptq_status)
+int check_attention_args(const char* fn, int dtype, int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D,
+                         float scale);
+int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides, int n);
+
 }  // namespace plan
 }  // namespace gptq

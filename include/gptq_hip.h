@@ -343,6 +343,113 @@ int gptq_dequantize_tensor(const int8_t* q, int64_t n, int group_size,
                            const float* scales, const float* zeros, float* out,
                            gptq_stream_t stream);
 
+/* -------------------------------------------------------------- attention --
+ * What stands between a decoder layer's quantized projections.  No counterpart
+ * in the reference, which leaves a model's attention to its own modules.
+ *
+ * o_i = sum_j softmax_j(scale q_i k_j) v_j over the keys that query i sees, for
+ * packed sequences: rows of (token, head), T queries and S keys together,
+ * sequence b's queries being rows cu_q[b] .. cu_q[b + 1] - 1 and its keys rows
+ * cu_k[b] .. (B + 1 offsets each; both NULL for one sequence).  With `causal`
+ * the last query sees the last key, the one before it one key less, and so on
+ * (query i of Lq sees keys 0 .. i + Lk - Lq); a query that sees no key gives
+ * zeros.  Query head h uses key head h / (H / Hk).
+ * fp16 or bf16; D a multiple of 8 up to 128, its values contiguous, 16-byte
+ * aligned; the strides (elements, multiples of 8) are those of a token and of
+ * a head.  out: (T, H, D) contiguous.  lse (T x H fp32, or NULL): the base-2
+ * logarithm of sum_j 2^(log2(e) scale q_i k_j), -infinity without keys; out_rest
+ * (T, H, D), or NULL: what the rounding of out left, in the same type (16 bits
+ * of out together).  gptq_attention_backward takes both.
+ * Scores, weights' sums and outputs are fp32 sums; a weight is rounded to the
+ * inputs' type before it multiplies v (with out_rest, to twice its bits). */
+int gptq_attention(const void* q, const void* k, const void* v, int dtype,
+                   int64_t q_token, int64_t q_head, int64_t k_token,
+                   int64_t k_head, int64_t v_token, int64_t v_head,
+                   const int32_t* cu_q, const int32_t* cu_k, int64_t B,
+                   int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D,
+                   int causal, float scale, void* out, void* out_rest,
+                   float* lse, gptq_stream_t stream);
+
+/* Its gradients, from the out, out_rest and lse that gptq_attention gave: dq (T, H, D),
+ * dk and dv (S, Hk, D), contiguous.  With g = dL/dout and p the weights,
+ * ds_ij = p_ij (g_i v_j - g_i out_i), dv_j = sum_i p_ij g_i,
+ * dk_j = scale sum_i ds_ij q_i, dq_i = scale sum_j ds_ij k_j, a key head's sums
+ * over its query heads too; the same bits from call to call.  p and ds are
+ * rounded to the inputs' type (fp16: times a power of two that keeps them in
+ * its range) before they multiply rows; sums are fp32.  A row that is not
+ * finite may leave any gradient of its own sequence not finite. */
+size_t gptq_attention_backward_workspace_size(int64_t T, int64_t H);
+int gptq_attention_backward(const void* grad, const void* q, const void* k,
+                            const void* v, const void* out,
+                            const void* out_rest, const float* lse, int dtype,
+                            int64_t g_token, int64_t g_head,
+                            int64_t q_token, int64_t q_head, int64_t k_token,
+                            int64_t k_head, int64_t v_token, int64_t v_head,
+                            const int32_t* cu_q, const int32_t* cu_k,
+                            int64_t B, int64_t T, int64_t S, int64_t H,
+                            int64_t Hk, int64_t D, int causal, float scale,
+                            void* dq, void* dk, void* dv, void* workspace,
+                            size_t workspace_bytes, gptq_stream_t stream);
+
+/* The same for new tokens over a paged cache: key j of sequence b is row
+ * j % page_size of page block_table[b][j / page_size] (rows of the table
+ * `table_stride` apart, `width` pages each, `pages` pages in the cache).
+ * context[b] tokens of sequence b are cached, the new ones among them: the
+ * last query sees all of them, the one before it one less.  cu_q as above, or
+ * NULL: one new token a sequence (T == B).  max_context bounds the context
+ * lengths for the choice of kernel (a larger context is read all the same).
+ * Page numbers, offsets and lengths out of range are clamped: whatever the
+ * device arrays hold, no row outside the cache is read. */
+size_t gptq_paged_attention_workspace_size(int64_t B, int64_t T, int64_t H,
+                                           int64_t Hk, int64_t D,
+                                           int64_t max_context);
+int gptq_paged_attention(const void* q, const void* k_cache,
+                         const void* v_cache, int dtype, int64_t q_token,
+                         int64_t q_head, int64_t k_page, int64_t k_token,
+                         int64_t k_head, int64_t v_page, int64_t v_token,
+                         int64_t v_head, const int32_t* block_table,
+                         int64_t table_stride, int64_t width,
+                         int64_t page_size, int64_t pages,
+                         const int32_t* context, const int32_t* cu_q, int64_t B,
+                         int64_t T, int64_t H, int64_t Hk, int64_t D,
+                         float scale, int64_t max_context, void* out,
+                         void* workspace, size_t workspace_bytes,
+                         gptq_stream_t stream);
+
+/* ----------------------------------------------------------------- rotary --
+ * Rotary positions: the first rotary_dim channels of each head of token t are
+ * turned in pairs by the angles of positions[t], a' = a cos - b sin,
+ * b' = b cos + a sin; pairs are channels (i, i + rotary_dim / 2), or with
+ * `interleaved` (2i, 2i + 1); the other channels are copied.  table
+ * (table_rows, 2, rotary_dim / 2) fp32 holds each position's cosines, then
+ * sines; positions outside it are clamped.  `inverse` turns back: the gradient
+ * of the input from that of the output.  fp32, fp16 or bf16, computed in fp32
+ * and rounded once.  q (T, H, D) and k (T, Hk, D) with the strides of a token
+ * and of a head; q_out and k_out contiguous, not overlapping the inputs.  D
+ * even.  No counterpart in the reference. */
+int gptq_rotary(const void* q, const void* k, int dtype, int64_t q_token,
+                int64_t q_head, int64_t k_token, int64_t k_head,
+                const float* table, int64_t table_rows, int64_t rotary_dim,
+                const int32_t* positions, int interleaved, int inverse,
+                int64_t T, int64_t H, int64_t Hk, int64_t D, void* q_out,
+                void* k_out, gptq_stream_t stream);
+
+/* The same, the keys and the values (not turned) written into a paged cache:
+ * token t into place slots[t] % page_size of page slots[t] / page_size; a token
+ * whose slot is negative or past the cache is not written.  table NULL: nothing
+ * is turned.  No two tokens of a call may have the same slot. */
+int gptq_rotary_append(const void* q, const void* k, const void* v, int dtype,
+                       int64_t q_token, int64_t q_head, int64_t k_token,
+                       int64_t k_head, int64_t v_token, int64_t v_head,
+                       const float* table, int64_t table_rows,
+                       int64_t rotary_dim, const int32_t* positions,
+                       int interleaved, const int32_t* slots,
+                       int64_t page_size, int64_t pages, int64_t T, int64_t H,
+                       int64_t Hk, int64_t D, void* q_out, void* k_cache,
+                       int64_t k_page, int64_t kc_token, int64_t kc_head,
+                       void* v_cache, int64_t v_page, int64_t vc_token,
+                       int64_t vc_head, gptq_stream_t stream);
+
 /* ------------------------------------------------------- measurement aid --
  * No counterpart in the reference: a read-only streaming kernel for the
  * benchmark.  It reads `bytes` bytes of `buf` (both multiples of 16 bytes)

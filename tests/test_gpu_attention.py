@@ -1,0 +1,314 @@
+"""Attention of packed sequences and its gradient against 64 bits, within
+bounds derived in attention_check.py; masks that leave rows empty, values that
+are not finite in places that a row does not see, strides, streams and
+refusals."""
+import math
+
+import pytest
+import torch
+
+from attention_check import UNIT, check, one, packed
+
+pytestmark = pytest.mark.gpu
+
+HEADS = [(4, 4, 64), (8, 2, 128), (3, 1, 40), (6, 2, 96), (7, 1, 8), (16, 2, 80), (12, 12, 64)]
+TYPES = [torch.bfloat16, torch.float16]
+
+
+def A():
+    from distributed_gptq_amd.models import attention
+    return attention
+
+
+def rand(g, *shape, dtype, scale=1.0):
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def inputs(lens_q, lens_k, H, Hk, D, dtype, seed=0, extra=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(lens_q) + 7 * D)
+    T, S = sum(lens_q) + extra, sum(lens_k) + extra
+    q, k, v = rand(g, T, H, D, dtype=dtype, scale=2.0), rand(g, S, Hk, D, dtype=dtype), rand(g, S, Hk, D, dtype=dtype)
+    grad = rand(g, T, H, D, dtype=dtype, scale=1e-2)
+
+    def offsets(lens):
+        at = [0]
+        for n in lens:
+            at.append(at[-1] + n)
+        return at
+    return q, k, v, grad, offsets(lens_q), offsets(lens_k)
+
+
+def on_gpu(offsets, dtype=torch.int32):
+    return torch.tensor(offsets, dtype=dtype, device="cuda")
+
+
+def run(q, k, v, grad, cu_q, cu_k, causal=True, scale=None):
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    out = A().attention(q, k, v, cu_q, cu_k, causal=causal, scale=scale)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), grad)
+    return {"out": out.detach(), "dq": dq, "dk": dk, "dv": dv}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hk,D", HEADS)
+@pytest.mark.parametrize("lens", [(1,), (2, 31), (33, 64, 1, 65), (127, 0, 129), (513,)])
+def test_packed_causal(H, Hk, D, lens, dtype):
+    q, k, v, grad, cu, _ = inputs(lens, lens, H, Hk, D, dtype)
+    want = packed(q, k, v, cu, cu, grad)
+    got = run(q, k, v, grad, on_gpu(cu), None)
+    for name in want:
+        check(got[name], want[name])
+    with torch.no_grad():  # the form without a gradient to follow
+        check(A().attention(q, k, v, on_gpu(cu, torch.int64)), want["out"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens_q,lens_k", [
+    ((5,), (200,)), ((200,), (5,)), ((70, 3, 0, 64), (64, 0, 10, 130)), ((1, 1), (300, 1)), ((3,), (0,))])
+def test_lengths_of_their_own(lens_q, lens_k, causal, dtype):
+    """Queries and keys of different lengths: causal from the last ones on, so
+    that the first queries of a longer side see no key and give zeros."""
+    q, k, v, grad, cq, ck = inputs(lens_q, lens_k, 6, 3, 64, dtype, seed=3)
+    want = packed(q, k, v, cq, ck, grad, causal)
+    got = run(q, k, v, grad, on_gpu(cq), on_gpu(ck), causal)
+    for name in want:
+        check(got[name], want[name])
+    at = 0
+    for n, m in zip(lens_q, lens_k):
+        empty = n if m == 0 else max(0, n - m) if causal else 0
+        assert not got["out"][at:at + empty].any() and not got["dq"][at:at + empty].any()
+        at += n
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_past_the_offsets_are_zero(dtype):
+    q, k, v, grad, cu, _ = inputs((40, 9), (40, 9), 4, 2, 128, dtype, extra=100)
+    q[49:], k[49:], v[49:], grad[49:] = math.nan, math.nan, math.inf, math.nan
+    got = run(q, k, v, grad, on_gpu(cu), None)
+    for x in got.values():
+        assert not x[49:].any() and bool(torch.isfinite(x).all())
+    check(got["out"][:49], one_or_packed(q, k, v, cu))
+
+
+def one_or_packed(q, k, v, cu):
+    n = cu[-1]
+    return packed(q[:n], k[:n], v[:n], cu, cu)["out"]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_one_sequence_without_offsets_and_scale(dtype):
+    q, k, v, grad, _, _ = inputs((150,), (150,), 4, 4, 128, dtype, seed=5)
+    for scale in (0.3, 1e-6):
+        want = one(q, k, v, grad, True, scale)
+        got = run(q, k, v, grad, None, None, scale=scale)
+        for name in want:
+            check(got[name], want[name])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_maxima_that_grow_and_large_scores(dtype):
+    """Scores whose maximum rises with the key, far beyond the rescaling's slack
+    and back, and equal scores: nothing overflows."""
+    L, D = 400, 64
+    q = torch.ones(L, 2, D, device="cuda", dtype=dtype)
+    ramp = torch.linspace(-60, 60, L, device="cuda")
+    for shape in (ramp, ramp.flip(0), torch.where(torch.arange(L, device="cuda") % 97 == 5, 60.0, -60.0), ramp * 0):
+        k = (shape[:, None, None] / 8).expand(L, 2, D).to(dtype).contiguous()
+        g = torch.Generator(device="cuda").manual_seed(1)
+        v, grad = rand(g, L, 2, D, dtype=dtype), rand(g, L, 2, D, dtype=dtype)
+        want = one(q, k, v, grad)
+        got = run(q, k, v, grad, None, None)
+        for name in want:
+            check(got[name], want[name])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_not_finite_in_places_that_a_row_does_not_see(dtype):
+    """A token's row is the same whatever later tokens and other sequences hold,
+    an infinity or NaN in their keys and values too."""
+    lens = (100, 77)
+    q, k, v, _, cu, _ = inputs(lens, lens, 4, 2, 128, dtype, seed=9)
+    clean = A().attention(q, k, v, on_gpu(cu))
+    for bad in (math.nan, math.inf, -math.inf):
+        for place in (5, 63, 64, 99):
+            k2, v2 = k.clone(), v.clone()
+            k2[place], v2[place] = bad, bad
+            out = A().attention(q, k2, v2, on_gpu(cu))
+            # (a tile's row that is computed again sums in another order)
+            check(out[:place], tuple(x[:place] for x in packed(q, k, v, cu, cu)["out"]))
+            assert torch.equal(out[100:], clean[100:])
+            assert not torch.isfinite(out[place:100]).any()
+            v2 = v.clone()
+            v2[place, 1, 3] = bad
+            out = A().attention(q, k, v2, on_gpu(cu))
+            assert torch.equal(out[place:100, 2:, 3].isnan(), torch.full((100 - place, 2), math.isnan(bad), device="cuda"))
+            assert not torch.isfinite(out[place:100, 2:, 3]).any()
+            keep = [c for c in range(128) if c != 3]
+            want = packed(q, k, v, cu, cu)["out"]
+            check(out[:, :, keep], tuple(x[:, :, keep] for x in want))
+            check(out[:, :2], tuple(x[:, :2] for x in want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_scores_as_the_formula(dtype):
+    """All scores -infinity or one +infinity among those seen: NaN, as softmax
+    of them is; -infinity among finite ones: weight zero."""
+    q, k, v, _, cu, _ = inputs((70,), (70,), 1, 1, 64, dtype, seed=2)
+    q = q.abs() + 1
+    k2 = k.clone()
+    k2[10] = -math.inf
+    out = A().attention(q, k2, v)
+    want = one(q, k, v)["out"]
+    seen = torch.tensor([i for i in range(70) if i != 10], device="cuda")
+    ref = one(q[seen], k[seen], v[seen])["out"]
+    check(out[:10], tuple(x[:10] for x in want))
+    check(out[11:], tuple(x[10:] for x in ref))
+    assert A().attention(q[:1], k2[10:11], v[:1]).isnan().all()
+    k2[10] = math.inf
+    assert A().attention(q, k2, v)[10:].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides(dtype):
+    """Parts of a fused projection, heads before tokens, odd offsets and a last
+    dimension that is not contiguous: the same bits as contiguous inputs."""
+    T, H, Hk, D = 90, 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    fused = rand(g, T, (H + 2 * Hk) * D, dtype=dtype)
+    q, k, v = (x.unflatten(-1, (-1, D)) for x in fused.split([H * D, Hk * D, Hk * D], -1))
+    grad = rand(g, T, H, D, dtype=dtype)
+    want = run(q.contiguous(), k.contiguous(), v.contiguous(), grad, None, None)
+
+    def head_first(x):
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+
+    def odd(x):
+        return torch.empty(x.numel() + 1, device="cuda", dtype=dtype)[1:].view(x.shape).copy_(x)
+
+    def last(x):
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+    for f in (lambda x: x, head_first, odd, last):
+        got = run(f(q), f(k), f(v), f(grad), None, None)
+        assert all(torch.equal(got[n], want[n]) for n in want), f
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_grad_of_broadcast_and_sums(dtype):
+    """An expanded gradient (a sum's), an expanded input and a shared input get
+    the gradients of their formula."""
+    T, H, D = 70, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = rand(g, T, 1, D, dtype=dtype).requires_grad_(True)
+    q = rand(g, T, H, D, dtype=dtype)
+    out = A().attention(q, x, x)
+    dx, = torch.autograd.grad(out.sum(), x)
+    want = one(q, x.detach(), x.detach(), torch.ones_like(q))
+    u = UNIT[dtype]
+    ref = want["dk"][0] + want["dv"][0]
+    check(dx, (ref, want["dk"][1] + want["dv"][1] + u * ref.abs() + 2.0 ** -25))
+
+
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (2, 2, 128)])
+def test_gradient_against_differences(H, Hk, D):
+    """Directional derivatives from outputs at inputs that are exact in fp16: h
+    times the gradient is off from the outputs' difference by the truncation,
+    which the formula's 64-bit values give, and by the rounding of the outputs,
+    independent for each, taken at four times its root of squares."""
+    L, dt, h = 48, torch.float16, 2.0 ** -4
+    g = torch.Generator(device="cuda").manual_seed(11)
+    grid = [(torch.randn(L, n, D, generator=g, device="cuda").clamp(-3, 3) * 32).round() / 32 for n in (H, Hk, Hk)]
+    step = [torch.randint(-1, 2, x.shape, generator=g, device="cuda") * h for x in grid]
+    grad = rand(g, L, H, D, dtype=dt)
+    got = run(*[x.to(dt) for x in grid], grad, None, None)
+
+    def loss64(sign, which):
+        return one(*[(x + sign * (s if i == which else 0)).to(dt) for i, (x, s) in enumerate(zip(grid, step))])["out"]
+    for which, name in enumerate(("dq", "dk", "dv")):
+        exact, noise, outs = [], 0.0, []
+        for sign in (1, -1):
+            ref, bound = loss64(sign, which)
+            exact.append((ref * grad.double()).sum())
+            noise += ((bound * grad.double()) ** 2).sum()
+            args = [(x + sign * (s if i == which else 0)).to(dt) for i, (x, s) in enumerate(zip(grid, step))]
+            outs.append((A().attention(*args).double() * grad.double()).sum())
+        slope = (got[name].double() * step[which].double()).sum() * 2
+        want = one(*[x.to(dt) for x in grid], grad)[name]
+        truncation = (exact[0] - exact[1] - 2 * (want[0] * step[which].double()).sum()).abs()
+        own = ((want[1] * step[which].double()) ** 2).sum()
+        assert (outs[0] - outs[1] - slope).abs() <= truncation + 4 * (noise + 4 * own).sqrt(), name
+
+
+def test_same_bits_from_call_to_call_and_on_another_stream():
+    q, k, v, grad, cu, _ = inputs((700, 300), (700, 300), 8, 2, 128, torch.bfloat16)
+    want = run(q, k, v, grad, on_gpu(cu), None)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = run(q, k, v, grad, on_gpu(cu), None)
+    torch.cuda.current_stream().wait_stream(s)
+    again = run(q, k, v, grad, on_gpu(cu), None)
+    for n in want:
+        assert torch.equal(want[n], again[n]) and torch.equal(want[n], other[n])
+
+
+def test_offsets_out_of_range_stay_inside():
+    """Offsets that lie outside the tensors or go back read and write nothing
+    outside them (the rows they name are not defined)."""
+    q, k, v, grad, _, _ = inputs((64,), (64,), 2, 1, 64, torch.float16)
+    pad = [torch.full((64, 2, 64), 7.0, device="cuda", dtype=torch.float16) for _ in range(2)]
+    for cu in ([0, 1000], [5, 64], [0, 50, 20, 64], [-4, 30, 64], [0, 2 ** 31 - 1, -2 ** 31]):
+        run(q, k, v, grad, on_gpu(cu), None)
+    torch.cuda.synchronize()
+    assert all(bool((p == 7.0).all()) for p in pad)
+
+
+def test_empty():
+    for T, S in ((0, 0), (0, 5), (5, 0)):
+        q, k = torch.zeros(T, 4, 64, device="cuda").half(), torch.zeros(S, 2, 64, device="cuda").half()
+        got = run(q, k, k.clone(), torch.zeros_like(q), on_gpu([0, T]), on_gpu([0, S]))
+        assert [tuple(got[n].shape) for n in ("out", "dq", "dk", "dv")] == [(T, 4, 64), (T, 4, 64), (S, 2, 64), (S, 2, 64)]
+        assert not any(bool(x.any()) for x in got.values())
+
+
+def test_refusals():
+    f = A().attention
+    x = torch.zeros(8, 4, 64, device="cuda").half()
+    cu = on_gpu([0, 8])
+    for q, k, v, args in [
+            (x, x[:, :3], x[:, :3], ()),                      # 4 heads over 3
+            (x, x, x[:, :2], ()),                             # k and v differ
+            (x, x[..., :32], x[..., :32], ()),                # head sizes differ
+            (x[..., :12], x[..., :12], x[..., :12], ()),      # 12 values
+            (x[0], x[0], x[0], ()),                           # no heads
+            (x, x[:4], x[:4], (cu,)),                         # keys without offsets of their own
+            (x, x, x, (cu[:1],)), (x, x, x, (cu, on_gpu([0, 4, 8]))), (x, x, x, (None, cu))]:
+        with pytest.raises(ValueError):
+            f(q, k, v, *args)
+    big = torch.zeros(2, 1, 136, device="cuda").half()
+    with pytest.raises(ValueError, match="136"):
+        f(big, big, big)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            f(x, x, x, scale=scale)
+    for bad in (x.float(), x.double(), x.to(torch.int32)):
+        with pytest.raises(TypeError):
+            f(bad, bad, bad)
+    with pytest.raises(TypeError):
+        f(x, x.bfloat16(), x.bfloat16())
+    with pytest.raises(TypeError, match="cu_seqlens"):
+        f(x, x, x, cu.float())
+    with pytest.raises((ValueError, RuntimeError)):
+        f(x.cpu(), x.cpu(), x.cpu())
+    with pytest.raises(ValueError):
+        f(x, x, x, cu.cpu())
+
+
+def test_second_derivative_is_refused():
+    x = torch.randn(8, 2, 64, device="cuda").half().requires_grad_(True)
+    out = A().attention(x, x, x)
+    g, = torch.autograd.grad(out.float().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        g.float().sum().backward()
