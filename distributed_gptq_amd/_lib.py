@@ -71,7 +71,7 @@ SIGNATURES = {
     "gptq_quantize_tensor": (_i, [_p, _i, _i64, _i, _i, _i, _p, _p, _p, _p]),
     "gptq_dequantize_tensor": (_i, [_p, _i64, _i, _p, _p, _p, _p]),
     "gptq_attention": (_i, [_p, _p, _p, _i] + [_i64] * 6 + [_p, _p] + [_i64] * 6 + [_i, _f, _p, _p, _p, _p]),
-    "gptq_attention_backward_workspace_size": (_sz, [_i64, _i64]),
+    "gptq_attention_backward_workspace_size": (_sz, [_i64] * 6),
     "gptq_attention_backward": (_i, [_p] * 7 + [_i] + [_i64] * 8 + [_p, _p] + [_i64] * 6 + [_i, _f, _p, _p, _p, _p, _sz,
                                                                                          _p]),
     "gptq_rotary": (_i, [_p, _p, _i] + [_i64] * 4 + [_p, _i64, _i64, _p, _i, _i] + [_i64] * 4 + [_p, _p, _p]),

@@ -251,6 +251,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
 
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
   auto use = [&](int t, const lds_u8* kt, const lds_u8* vt) {
     const int key0 = t * kKeys;
     if (key0 >= wave_end) return;
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) sc[n] = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, lane), q[d], sc[n]);
+      for (int n = 0; n < 2; ++n) sc[n] = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, where), q[d], sc[n]);
     if (key0 + kKeys - 1 > full) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -266,14 +267,14 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
         for (int i = 0; i < 16; ++i)
           if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = -INFINITY;
     }
-    softmax_step<kBF16, DT, 2, kTrain>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, lane); });
+    softmax_step<kBF16, DT, 2, kTrain>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
   };
 
   // the rows that this wave copies of a tile, and where the next tile's are
   constexpr int W = kKeys / 4;
   KvAt at = kv_at_clamped<kPaged>(a, s, t0 * kKeys + wave * W + lane % W);
   auto fetch = [&](int t, uint8_t* kt, uint8_t* vt) {
-    fetch_rows<DT, W, kPaged>(a, hk, at, t * kKeys, wave * W, s.Lk, kt, vt, lane);
+    fetch_rows<DT, W, kPaged>(a, s, hk, at, t * kKeys, wave * W, kt, vt, lane);
     at = kv_at_clamped<kPaged>(a, s, (t + 1) * kKeys + wave * W + lane % W);
   };
   if (t0 < t1) {
@@ -364,20 +365,21 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a, int slots)
 
   KvAt at = kv_at_clamped<true>(a, s, (t0 + wave) * kFew + (lane & 31));
   auto fetch = [&](int t, uint8_t* kt, uint8_t* vt) {
-    fetch_rows<DT, kFew, true>(a, hk, at, t * kFew, 0, s.Lk, kt, vt, lane);
+    fetch_rows<DT, kFew, true>(a, s, hk, at, t * kFew, 0, kt, vt, lane);
     at = kv_at_clamped<true>(a, s, (t + 4) * kFew + (lane & 31));
   };
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
   auto use = [&](int t, const lds_u8* kt, const lds_u8* vt) {
     const int key0 = t * kFew;
     f32x16 sc[1] = {zero16()};
 #pragma unroll
-    for (int d = 0; d < DT / 16; ++d) sc[0] = mma32<kBF16>(row_operand<DT>(kt, 0, d, lane), q[d], sc[0]);
+    for (int d = 0; d < DT / 16; ++d) sc[0] = mma32<kBF16>(row_operand<DT>(kt, 0, d, where), q[d], sc[0]);
     if (key0 + kFew - 1 > full) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         if (key0 + acc_row(i, half) > limit) sc[0][i] = -INFINITY;
     }
-    softmax_step<kBF16, DT, 1, false>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, lane); });
+    softmax_step<kBF16, DT, 1, false>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
   };
   // one wave's copies are only its own: they have to have landed before its
   // reads, and its reads of a buffer to be done before the next copies into it
@@ -642,6 +644,7 @@ extern "C" int gptq_paged_attention(const void* q, const void* k_cache, const vo
   a.paged.most = static_cast<int>(plan::cached_most(width, page_size));
   a.paged.pages = static_cast<int>(pages);
   a.paged.page = fast_div(static_cast<uint32_t>(page_size));
+  a.paged.whole = page_size % 16 == 0;
   a.cu_q = cu_q;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T);
   a.H = static_cast<int>(H), a.Hk = static_cast<int>(Hk), a.D = static_cast<int>(D);

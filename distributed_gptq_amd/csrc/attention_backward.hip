@@ -12,7 +12,7 @@ namespace gptq {
 namespace {
 
 constexpr int kRows = 64;        // packed query rows, or keys, of a tile
-constexpr int kMaxima = 1024;    // workgroups of the first kernel
+constexpr int kMaxima = plan::kBackMaxima;  // workgroups of the first kernel
 
 struct BackArgs {
   AttnArgs f;                    // q, k, v, offsets, sizes; lse as input
@@ -20,6 +20,8 @@ struct BackArgs {
   const uint16_t *o, *o_rest;    // (T, H, D): the output, and what its rounding left
   float* delta;                  // (T, H)
   float* maxima;                 // 2 x kMaxima: largest |g_i|^2 and |v_j|^2 of each workgroup (fp16)
+  float* part;                   // with splits > 1: dk and dv of each split (S, Hk, D) each
+  int splits;                    // parts of the rows of each 64 keys
   float scale;
   uint16_t *dq, *dk, *dv;        // contiguous
 };
@@ -36,17 +38,19 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// e for all of a kernel's ds, by all threads of a workgroup (one barrier)
+// e for all of a kernel's ds, by the first 256 threads of a workgroup (one barrier)
 __device__ __forceinline__ float ds_shift(const BackArgs& a, float (*room)[4]) {
   float g = 0.0f, v = 0.0f;
+  if (threadIdx.x < 256) {
 #pragma unroll
-  for (int x = 0; x < kMaxima / 256; ++x) {
-    g = fmaxf(g, a.maxima[256 * x + threadIdx.x]);
-    v = fmaxf(v, a.maxima[kMaxima + 256 * x + threadIdx.x]);
+    for (int x = 0; x < kMaxima / 256; ++x) {
+      g = fmaxf(g, a.maxima[256 * x + threadIdx.x]);
+      v = fmaxf(v, a.maxima[kMaxima + 256 * x + threadIdx.x]);
+    }
   }
   g = wave_max(g);
   v = wave_max(v);
-  if ((threadIdx.x & 63) == 0) room[0][threadIdx.x >> 6] = g, room[1][threadIdx.x >> 6] = v;
+  if (threadIdx.x < 256 && (threadIdx.x & 63) == 0) room[0][threadIdx.x >> 6] = g, room[1][threadIdx.x >> 6] = v;
   __syncthreads();
   g = fmaxf(fmaxf(room[0][0], room[0][1]), fmaxf(room[0][2], room[0][3]));
   v = fmaxf(fmaxf(room[1][0], room[1][1]), fmaxf(room[1][2], room[1][3]));
@@ -187,8 +191,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
   KvAt at = kv_at<false>(a, s, wave * W + lane % W);
   auto fetch = [&](int t, uint8_t* kt, uint8_t* vt) {
     at.at = s.k0 + t * kRows + wave * W + lane % W;
-    fetch_rows<DT, W, false>(a, hk, at, t * kRows, wave * W, s.Lk, kt, vt, lane);
+    fetch_rows<DT, W, false>(a, s, hk, at, t * kRows, wave * W, kt, vt, lane);
   };
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
   auto use = [&](int t, const lds_u8* kt, const lds_u8* vt) {
     const int key0 = t * kRows;
     if (key0 >= wave_end) return;
@@ -198,8 +203,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
       f32x16 sc = zero16(), dp = zero16();
 #pragma unroll
       for (int d = 0; d < DT / 16; ++d) {
-        sc = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, lane), q[d], sc);
-        dp = mma32<kBF16>(row_operand<DT>(vt, 32 * n, d, lane), g[d], dp);
+        sc = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, where), q[d], sc);
+        dp = mma32<kBF16>(row_operand<DT>(vt, 32 * n, d, where), g[d], dp);
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -216,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
         const u32x4 x = operand_of<kBF16>(sc, 8 * ks);
 #pragma unroll
         for (int db = 0; db < DT / 32; ++db)
-          acc[db] = mma32<kBF16>(column_operand<DT>(kt, 32 * n + 16 * ks, db, lane), x, acc[db]);
+          acc[db] = mma32<kBF16>(column_operand<DT>(kt, 32 * n + 16 * ks, db, where), x, acc[db]);
       }
     }
   };
@@ -236,25 +241,65 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
   if (inside) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale * exp2f(-shift), a.D, half);
 }
 
-// dk and dv: a workgroup has 64 keys and passes tiles of 64 packed query rows
-// and their gradients through LDS, with each row's lse, delta and last key.
-// Wave w has keys 32 (w % 2) .. (a lane's column) and each tile's rows
-// 32 (w / 2) ..; the two waves of a key are joined at the end.  (With all four
-// waves on keys of their own, 128 to a workgroup, the workgroups of the first
-// keys, which all queries see, ran twice as long as the average.)
+// dk and dv: a workgroup of 4 waves has 64 keys, whose value rows stay in LDS,
+// and passes tiles of 64 query rows (of one head) and their gradients through
+// two LDS buffers.  Wave w has keys 32 (w % 2) .. (a lane's column) and each
+// tile's rows 32 (w / 2) ..; the two waves of a key are joined at the end.
+//
+// Two workgroups run on a CU, the vector work of one beside the MFMAs of the
+// other, which takes all registers (256 a lane) and all of LDS (80 KB each): the
+// rows' lse and delta have no place in either, and are added by one MFMA more
+// each, as 16 further channels of q and g (their parts, below) and of k and v
+// (the parts' units).
+constexpr int kBackRows = 64;
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_dkv_q0[kBackRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_dkv_q1[kBackRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_dkv_g0[kBackRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_dkv_g1[kBackRows * DT * 2];
+template <int DT>
+__shared__ __attribute__((aligned(1024))) uint8_t g_dkv_v[64 * DT * 2];
+
+// A float as three values of 16 bits, x = sum of part i times unit i, to 24 bits:
+// bf16 has its range; fp16 takes units that keep the parts in its range, scores
+// (up to 2^31) as 2^15, 1 and 2^-10 and deltas as 1, 2^-14 and 0.
+template <bool kBF16, bool kScore>
+__device__ __forceinline__ u32x2 parts_of(float x) {
+  if constexpr (kBF16) {
+    const uint32_t hi = pack16<true>(x, 0.0f) & 0xFFFFu;
+    const float r1 = x - bf16_bits_to_f32(static_cast<uint16_t>(hi));
+    const uint32_t mid = pack16<true>(r1, 0.0f) & 0xFFFFu;
+    return u32x2{hi | mid << 16, pack16<true>(r1 - bf16_bits_to_f32(static_cast<uint16_t>(mid)), 0.0f)};
+  } else {
+    const float u0 = kScore ? 32768.0f : 1.0f, u1 = kScore ? 1.0f : 6.103515625e-5f;
+    const uint32_t hi = pack16<false>(x / u0, 0.0f) & 0xFFFFu;
+    const float r1 = x - f16_bits_to_f32(static_cast<uint16_t>(hi)) * u0;
+    const uint32_t mid = pack16<false>(r1 / u1, 0.0f) & 0xFFFFu;
+    const float r2 = r1 - f16_bits_to_f32(static_cast<uint16_t>(mid)) * u1;
+    return u32x2{hi | mid << 16, kScore ? pack16<false>(r2 * 1024.0f, 0.0f) : 0u};
+  }
+}
+template <bool kBF16, bool kScore>
+__device__ __forceinline__ u32x4 units() {
+  if constexpr (kBF16) return u32x4{0x3F803F80u, 0x3F80u, 0, 0};
+  return kScore ? u32x4{0x3C007800u, 0x1400u, 0, 0} : u32x4{0x04003C00u, 0, 0, 0};
+}
+
 template <bool kBF16, int DT>
-__global__ __launch_bounds__(256, DT == 128 ? 1 : 2) void attn_dkv_kernel(BackArgs args) {
-  constexpr int R = 64, W = kRows / 4, CH = DT / 8, RPI = 64 / CH;
-  __shared__ float room[2][4];
-  __shared__ __attribute__((aligned(16))) float stats[2][2][kRows];
-  __shared__ __attribute__((aligned(16))) int limits[2][kRows];
+__global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
+  constexpr int R = 64, W = kBackRows / 4, CH = DT / 8, RPI = 64 / CH;
   const AttnArgs& a = args.f;
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int G = static_cast<int>(a.G.d);
   const int hk = blockIdx.x % a.Hk;
+  // (causal: the first keys' workgroups, with the most rows, go first)
+  const int rest = static_cast<int>(blockIdx.x / a.Hk), split = rest % args.splits;
   int tile;
-  const int b = find_seq(a.cu_k, a.B, a.S, 1, R, static_cast<int>(blockIdx.x / a.Hk), &tile);
+  const int b = find_seq(a.cu_k, a.B, a.S, 1, R, rest / args.splits, &tile);
   Seq s = seq_of<false>(a, b);
   if (b == a.B) {  // rows past the offsets
     s.Lk = a.S - s.k0;
@@ -262,124 +307,131 @@ __global__ __launch_bounds__(256, DT == 128 ? 1 : 2) void attn_dkv_kernel(BackAr
   }
   if (tile * R >= s.Lk) return;
   float shift = 0.0f;
-  if constexpr (!kBF16) shift = ds_shift(args, room);
+  if constexpr (!kBF16) {
+    shift = ds_shift(args, reinterpret_cast<float(*)[4]>(&g_dkv_q0<DT>[0]));
+    __syncthreads();
+  }
   const float up = exp2f(kBF16 ? 0.0f : shift - kWeightShift);
 
-  const int rows = s.Lq * G;
   const int key0 = tile * R, kw = key0 + 32 * (wave & 1), n = wave >> 1;
   const int key = kw + (lane & 31);
   const bool inside = key < s.Lk;
   const int off = s.Lk - s.Lq;
-  // the first token that sees the workgroup's first key
+  // tiles of 64 tokens of one query head after the other, from the first token
+  // that sees the workgroup's first key on
   const int i0 = a.causal && key0 > off ? key0 - off : 0;
-  const int t0 = (i0 < s.Lq ? i0 * G : rows) / kRows, t1 = (rows + kRows - 1) / kRows;
+  const int t0 = (i0 < s.Lq ? i0 : s.Lq) / kBackRows, nt = (s.Lq + kBackRows - 1) / kBackRows - t0;
 
-  u32x4 kf[DT / 16], vf[DT / 16];
-  {
-    const int64_t kr = s.k0 + (inside ? key : 0);
-    load_operand<DT>(kf, a.k.p + kr * a.k.st + hk * a.k.sh, inside, a.D, half);
-    load_operand<DT>(vf, a.v.p + kr * a.v.st + hk * a.v.sh, inside, a.D, half);
+  u32x4 kf[DT / 16];
+  load_operand<DT>(kf, a.k.p + static_cast<int64_t>(s.k0 + (inside ? key : 0)) * a.k.st + hk * a.k.sh, inside, a.D, half);
+#pragma unroll
+  for (int x = 0; x < W / RPI; ++x) {  // 16 of the values' rows a wave
+    const int i = wave * W + x * RPI + lane / CH;
+    const int ch = (lane % CH) ^ row_slot<DT>(i);
+    const bool in = key0 + i < s.Lk && ch * 8 < a.D;
+    const uint16_t* vp = a.v.p + static_cast<int64_t>(s.k0 + (in ? key0 + i : 0)) * a.v.st + hk * a.v.sh + ch * 8;
+    copy16_to_lds(in ? static_cast<const void*>(vp) : g_attn_zeros, g_dkv_v<DT> + (wave * (W / RPI) + x) * 1024);
   }
   f32x16 dk[DT / 32], dv[DT / 32];
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db) dk[db] = zero16(), dv[db] = zero16();
 
-  float n_lse = 0.0f, n_delta = 0.0f;
-  int n_limit = -1;
-  auto fetch = [&](int t, uint8_t* qt, uint8_t* gt) {
-#pragma unroll
-    for (int x = 0; x < W / RPI; ++x) {
-      const int i = wave * W + x * RPI + lane / CH;
-      const int r = t * kRows + i;
-      const int ch = (lane % CH) ^ row_slot<DT>(i);
-      const bool in = r < rows && ch * 8 < a.D;
-      const int tok = div_by(in ? r : 0, a.G);
-      const int head = hk * G + ((in ? r : 0) - tok * G);
-      const uint16_t* qp = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh + ch * 8;
-      const uint16_t* gp = args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh + ch * 8;
-      copy16_to_lds(in ? static_cast<const void*>(qp) : g_attn_zeros, qt + (wave * (W / RPI) + x) * 1024);
-      copy16_to_lds(in ? static_cast<const void*>(gp) : g_attn_zeros, gt + (wave * (W / RPI) + x) * 1024);
+  const float inv_c = -1.0f / a.c;
+  float n_lse = 0.0f, n_delta = 0.0f;  // of the next tile's row n 32 + lane % 32
+  const int my_lane = lane;
+  // tile x: of head x / nt, from the last tokens (which see all keys) on, so that
+  // the workgroups of a key head read the same rows at the same time
+  auto fetch = [&](int x, uint8_t* qt, uint8_t* gt) {
+    const int g = x / nt, head = hk * G + g, tok0 = (t0 + nt - 1 - (x - g * nt)) * kBackRows;
+    const uint16_t* qp = a.q.p + s.q0 * a.q.st + head * a.q.sh;
+    const uint16_t* gp = args.g.p + s.q0 * args.g.st + head * args.g.sh;
+    const int first = tok0 + wave * W;
+    int lane = my_lane;
+    asm volatile("" : "+v"(lane));
+    {
+      int tok = tok0 + 32 * n + (lane & 31);
+      tok = tok < s.Lq ? tok : s.Lq - 1;  // (rows past the last are masked)
+      const int64_t at = static_cast<int64_t>(s.q0 + tok) * a.H + head;
+      n_lse = a.lse[at];
+      n_delta = args.delta[at];
     }
-    if (wave == 0) {
-      const int r = t * kRows + lane;
-      n_limit = -1;
-      n_lse = n_delta = 0.0f;
-      if (r < rows) {
-        const int tok = div_by(r, a.G);
-        const int64_t at = static_cast<int64_t>(s.q0 + tok) * a.H + hk * G + (r - tok * G);
-        n_lse = a.lse[at];
-        n_delta = args.delta[at];
-        n_limit = last_key(a, s, tok);
+    if (first + W <= s.Lq && a.D == DT) {
+      copy_rows<DT, W>(qp + first * a.q.st, a.q.st, qt, wave * W, lane);
+      copy_rows<DT, W>(gp + first * args.g.st, args.g.st, gt, wave * W, lane);
+    } else {
+#pragma unroll
+      for (int y = 0; y < W / RPI; ++y) {
+        const int i = wave * W + y * RPI + lane / CH;
+        const int64_t tok = tok0 + i;
+        const int ch = (lane % CH) ^ row_slot<DT>(i);
+        const bool in = tok < s.Lq && ch * 8 < a.D;
+        copy16_to_lds(in ? static_cast<const void*>(qp + tok * a.q.st + ch * 8) : g_attn_zeros,
+                      qt + (wave * (W / RPI) + y) * 1024);
+        copy16_to_lds(in ? static_cast<const void*>(gp + tok * args.g.st + ch * 8) : g_attn_zeros,
+                      gt + (wave * (W / RPI) + y) * 1024);
       }
     }
   };
-  auto keep = [&](int buf) {
-    if (wave == 0) {
-      stats[buf][0][lane] = n_lse;
-      stats[buf][1][lane] = n_delta;
-      limits[buf][lane] = n_limit;
-    }
-  };
-  auto use = [&](int t, int buf, const lds_u8* qt, const lds_u8* gt) {
-    const int r0 = t * kRows + 32 * n;
-    if (r0 >= rows) return;
-    const int r1 = r0 + 31 < rows ? r0 + 31 : rows - 1;
-    if (last_key(a, s, div_by(r1, a.G)) < kw) return;  // no row of these sees a key of the wave
-    const bool masked = r0 + 31 >= rows || last_key(a, s, div_by(r0, a.G)) < kw + 31;
+  const LaneAt<DT> where = lane_at<DT>(lane, 32 * n * (DT * 2));  // of the wave's rows of a tile
+  auto use = [&](int x, float lse, float delta, const lds_u8* qt, const lds_u8* gt) {
+    const int r0 = (t0 + nt - 1 - x % nt) * kBackRows + 32 * n;
+    if (r0 >= s.Lq) return;
+    if (last_key(a, s, r0 + 31 < s.Lq ? r0 + 31 : s.Lq - 1) < kw) return;  // no row of these sees a key of the wave
+    const bool masked = r0 + 31 >= s.Lq || last_key(a, s, r0) < kw + 31;
+    const lds_u8* vt = (const lds_u8*)&g_dkv_v<DT>[0] + (32 * (wave & 1) - 32 * n) * (DT * 2);
     f32x16 sc = zero16(), dp = zero16();
+    {
+      const u32x2 l = parts_of<kBF16, true>(half ? 0.0f : lse * inv_c), d = parts_of<kBF16, false>(half ? 0.0f : -delta);
+      sc = mma32<kBF16>(u32x4{l[0], l[1], 0, 0}, units<kBF16, true>(), sc);
+      dp = mma32<kBF16>(u32x4{d[0], d[1], 0, 0}, units<kBF16, false>(), dp);
+    }
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d) {
-      sc = mma32<kBF16>(row_operand<DT>(qt, 32 * n, d, lane), kf[d], sc);
-      dp = mma32<kBF16>(row_operand<DT>(gt, 32 * n, d, lane), vf[d], dp);
+      sc = mma32<kBF16>(row_operand<DT>(qt, 0, d, where), kf[d], sc);
+      dp = mma32<kBF16>(row_operand<DT>(gt, 0, d, where), row_operand<DT>(vt, 0, d, where), dp);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&stats[buf][0][32 * n + 8 * j + 4 * half]);
-      const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats[buf][1][32 * n + 8 * j + 4 * half]);
+    for (int i = 0; i < 16; ++i) {
+      sc[i] = __builtin_amdgcn_exp2f(kBF16 ? sc[i] * a.c : fmaf(sc[i], a.c, kWeightShift));
+      dp[i] = sc[i] * dp[i] * up;
+    }
+    if (masked) {
+      // row r0 + 4 half + i sees the key where i >= seen, and is one where i < rows
+      const int seen = a.causal ? key - off - r0 - 4 * half : 0, rows = s.Lq - r0 - 4 * half;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = 4 * j + e;
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[i], a.c, (kBF16 ? 0.0f : kWeightShift) - lse[e]));
-        dp[i] = p * (dp[i] - delta[e]) * up;
-        sc[i] = p;
-      }
-      if (masked) {
-        typedef int i32x4 __attribute__((ext_vector_type(4)));
-        const i32x4 lim = *reinterpret_cast<const i32x4*>(&limits[buf][32 * n + 8 * j + 4 * half]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key > lim[e]) sc[4 * j + e] = 0.0f, dp[4 * j + e] = 0.0f;
-      }
+      for (int i = 0; i < 16; ++i)
+        if (acc_row(i, 0) < seen || acc_row(i, 0) >= rows) sc[i] = 0.0f, dp[i] = 0.0f;
     }
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const u32x4 p = operand_of<kBF16>(sc, 8 * ks), x = operand_of<kBF16>(dp, 8 * ks);
+      const u32x4 p = operand_of<kBF16>(sc, 8 * ks), w = operand_of<kBF16>(dp, 8 * ks);
 #pragma unroll
       for (int db = 0; db < DT / 32; ++db) {
-        dv[db] = mma32<kBF16>(column_operand<DT>(gt, 32 * n + 16 * ks, db, lane), p, dv[db]);
-        dk[db] = mma32<kBF16>(column_operand<DT>(qt, 32 * n + 16 * ks, db, lane), x, dk[db]);
+        dv[db] = mma32<kBF16>(column_operand<DT>(gt, 16 * ks, db, where), p, dv[db]);
+        dk[db] = mma32<kBF16>(column_operand<DT>(qt, 16 * ks, db, where), w, dk[db]);
       }
     }
   };
-  if (t0 < t1) {
-    fetch(t0, g_back_a0<DT>, g_back_b0<DT>);
-    keep(0);
+  const int per = (nt * G + args.splits - 1) / args.splits;
+  const int first = split * per, last = first + per < nt * G ? first + per : nt * G;
+  if (first < last) {
+    fetch(first, g_dkv_q0<DT>, g_dkv_g0<DT>);
     __syncthreads();
-    for (int t = t0; t < t1; t += 2) {
-      if (t + 1 < t1) fetch(t + 1, g_back_a1<DT>, g_back_b1<DT>);
-      use(t, 0, (const lds_u8*)&g_back_a0<DT>[0], (const lds_u8*)&g_back_b0<DT>[0]);
-      keep(1);
+    for (int t = first; t < last; t += 2) {
+      float lse = n_lse, delta = n_delta;
+      if (t + 1 < last) fetch(t + 1, g_dkv_q1<DT>, g_dkv_g1<DT>);
+      use(t, lse, delta, (const lds_u8*)&g_dkv_q0<DT>[0], (const lds_u8*)&g_dkv_g0<DT>[0]);
       __syncthreads();
-      if (t + 1 >= t1) break;
-      if (t + 2 < t1) fetch(t + 2, g_back_a0<DT>, g_back_b0<DT>);
-      use(t + 1, 1, (const lds_u8*)&g_back_a1<DT>[0], (const lds_u8*)&g_back_b1<DT>[0]);
-      keep(0);
+      if (t + 1 >= last) break;
+      lse = n_lse, delta = n_delta;
+      if (t + 2 < last) fetch(t + 2, g_dkv_q0<DT>, g_dkv_g0<DT>);
+      use(t + 1, lse, delta, (const lds_u8*)&g_dkv_q1<DT>[0], (const lds_u8*)&g_dkv_g1<DT>[0]);
       __syncthreads();
     }
   }
   // (the tiles are done with: the last barrier is behind every wave's reads)
-  lds_f32* sum_k = (lds_f32*)((wave & 1) ? &g_back_a1<DT>[0] : &g_back_a0<DT>[0]);
-  lds_f32* sum_v = (lds_f32*)((wave & 1) ? &g_back_b1<DT>[0] : &g_back_b0<DT>[0]);
+  lds_f32* sum_k = (lds_f32*)((wave & 1) ? &g_dkv_q1<DT>[0] : &g_dkv_q0<DT>[0]);
+  lds_f32* sum_v = (lds_f32*)((wave & 1) ? &g_dkv_g1<DT>[0] : &g_dkv_g0<DT>[0]);
   if (n == 1) {
 #pragma unroll
     for (int db = 0; db < DT / 32; ++db)
@@ -399,19 +451,54 @@ __global__ __launch_bounds__(256, DT == 128 ? 1 : 2) void attn_dkv_kernel(BackAr
       dv[db][i] += sum_v[(16 * db + i) * 64 + lane];
     }
   const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
-  store_rows<kBF16, DT>(args.dk + row, dk, args.scale * exp2f(-shift), a.D, half);
-  store_rows<kBF16, DT>(args.dv + row, dv, exp2f(kBF16 ? 0.0f : -kWeightShift), a.D, half);
+  const float rk = args.scale * exp2f(-shift), rv = exp2f(kBF16 ? 0.0f : -kWeightShift);
+  if (args.splits == 1) {
+    store_rows<kBF16, DT>(args.dk + row, dk, rk, a.D, half);
+    store_rows<kBF16, DT>(args.dv + row, dv, rv, a.D, half);
+    return;
+  }
+  const int64_t all = static_cast<int64_t>(a.S) * a.Hk * a.D;
+  float* part = args.part + 2 * split * all + row;
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * db + acc_row(i, half);
+      if (d >= a.D) continue;
+      *reinterpret_cast<f32x4*>(part + d) = f32x4{dk[db][i], dk[db][i + 1], dk[db][i + 2], dk[db][i + 3]} * rk;
+      *reinterpret_cast<f32x4*>(part + all + d) = f32x4{dv[db][i], dv[db][i + 1], dv[db][i + 2], dv[db][i + 3]} * rv;
+    }
+}
+
+// The splits' sums of dk and dv, 4 values a thread.
+template <bool kBF16>
+__global__ __launch_bounds__(256) void attn_dkv_join_kernel(BackArgs args, int64_t all) {
+  const int64_t at = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (at >= 2 * all) return;
+  f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (int split = 0; split < args.splits; ++split) x += *reinterpret_cast<const f32x4*>(args.part + 2 * split * all + at);
+  *reinterpret_cast<u32x2*>((at < all ? args.dk + at : args.dv + (at - all))) =
+      u32x2{pack16<kBF16>(x[0], x[1]), pack16<kBF16>(x[2], x[3])};
 }
 
 template <bool kBF16, int DT>
 int launch(const BackArgs& a, hipStream_t st) {
   const int64_t qs = slots_of(a.f.cu_q, a.f.B, a.f.T, a.f.G.d, 128), ks = slots_of(a.f.cu_k, a.f.B, a.f.S, 1, 64);
-  GPTQ_REQUIRE(qs * a.f.Hk < (int64_t{1} << 31) && ks * a.f.Hk < (int64_t{1} << 31), GPTQ_ERR_SHAPE,
+  GPTQ_REQUIRE(qs * a.f.Hk < (int64_t{1} << 31) && ks * a.f.Hk * a.splits < (int64_t{1} << 31), GPTQ_ERR_SHAPE,
                "gptq_attention_backward: too many rows");
   attn_delta_kernel<kBF16><<<kMaxima, 256, 0, st>>>(a);
   int rc = check_launch("gptq_attention_backward");
   if (rc != GPTQ_OK) return rc;
-  if (a.f.S > 0) attn_dkv_kernel<kBF16, DT><<<static_cast<uint32_t>(ks * a.f.Hk), 256, 0, st>>>(a);
+  if (a.f.S > 0) {
+    attn_dkv_kernel<kBF16, DT><<<static_cast<uint32_t>(ks * a.f.Hk * a.splits), 256, 0, st>>>(a);
+    if (a.splits > 1) {
+      rc = check_launch("gptq_attention_backward");
+      if (rc != GPTQ_OK) return rc;
+      const int64_t all = static_cast<int64_t>(a.f.S) * a.f.Hk * a.f.D;
+      attn_dkv_join_kernel<kBF16><<<static_cast<uint32_t>(cdiv(2 * all, 1024)), 256, 0, st>>>(a, all);
+    }
+  }
   rc = check_launch("gptq_attention_backward");
   if (rc != GPTQ_OK) return rc;
   if (a.f.T > 0)
@@ -424,10 +511,9 @@ int launch(const BackArgs& a, hipStream_t st) {
 
 using namespace gptq;
 
-extern "C" size_t gptq_attention_backward_workspace_size(int64_t T, int64_t H) {
-  if (T < 0 || H < 1) return 0;
-  return plan::add_sat(plan::mul_sat(plan::mul_sat(static_cast<size_t>(T), static_cast<size_t>(H)), sizeof(float)),
-                       2 * kMaxima * sizeof(float));
+extern "C" size_t gptq_attention_backward_workspace_size(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk,
+                                                         int64_t D) {
+  return plan::backward_workspace(B, T, S, H, Hk, D);
 }
 
 extern "C" int gptq_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
@@ -449,7 +535,7 @@ extern "C" int gptq_attention_backward(const void* grad, const void* q, const vo
   if (rc != GPTQ_OK) return rc;
   rc = plan::check_attention_layout("gptq_attention_backward", grad, out, out_rest, strides, 2);
   if (rc != GPTQ_OK) return rc;
-  const size_t need = gptq_attention_backward_workspace_size(T, H);
+  const size_t need = plan::backward_workspace(B, T, S, H, Hk, D);
   GPTQ_REQUIRE(workspace && workspace_bytes >= need, GPTQ_ERR_WORKSPACE,
                "gptq_attention_backward: workspace of %zu bytes, needs %zu", workspace_bytes, need);
   BackArgs a{};
@@ -471,6 +557,8 @@ extern "C" int gptq_attention_backward(const void* grad, const void* q, const vo
   a.f.splits = 1;
   a.maxima = static_cast<float*>(workspace);
   a.delta = a.maxima + 2 * kMaxima;
+  a.part = a.delta + plan::ceil_div(T * H, 4) * 4;
+  a.splits = plan::backward_splits(B, S, Hk);
   a.dq = static_cast<uint16_t*>(dq);
   a.dk = static_cast<uint16_t*>(dk);
   a.dv = static_cast<uint16_t*>(dv);

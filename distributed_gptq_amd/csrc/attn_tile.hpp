@@ -107,12 +107,41 @@ __device__ __forceinline__ int row_slot(int row) {
     return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// Operand of a product over the row's values: lane l gives row l % 32 (+ the
-// tile's first row), values 16 s + 8 (l / 32) .. + 7.
+// Where a lane reads its operands of a tile.  The offsets are opaque to the
+// compiler, so that a read's constant part (the tile and its rows) goes into
+// the instruction instead of an addition each.
 template <int DT>
-__device__ __forceinline__ u32x4 row_operand(const lds_u8* tile, int row0, int s, int lane) {
-  const int r = lane & 31;
-  return *(const lds_u32x4*)(tile + (row0 + r) * (DT * 2) + (((2 * s + (lane >> 5)) ^ row_slot<DT>(r)) << 4));
+struct LaneAt {
+  int row[DT / 16];     // values 16 s + 8 (l / 32) .. of row l % 32
+  int col[DT / 32][2];  // the rows 8 j + 4 (l / 32) .., for a transposing read
+};
+template <int DT>
+__device__ __forceinline__ LaneAt<DT> lane_at(int lane, int more) {
+  LaneAt<DT> at;
+  const int h = lane >> 5, r = lane & 31;
+#pragma unroll
+  for (int s = 0; s < DT / 16; ++s) {
+    at.row[s] = more + r * (DT * 2) + (((2 * s + h) ^ row_slot<DT>(r)) << 4);
+    asm volatile("" : "+v"(at.row[s]));
+  }
+  const int i = lane & 15;
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+      const int row = 8 * j + 4 * h + (i >> 2);
+      at.col[db][j] = more + row * (DT * 2) + ((chunk ^ row_slot<DT>(row)) << 4) + ((i & 1) << 3);
+      asm volatile("" : "+v"(at.col[db][j]));
+    }
+  return at;
+}
+
+// Operand of a product over the row's values: lane l gives row l % 32 (+ row0,
+// a multiple of 16), values 16 s + 8 (l / 32) .. + 7.
+template <int DT>
+__device__ __forceinline__ u32x4 row_operand(const lds_u8* tile, int row0, int s, const LaneAt<DT>& at) {
+  return *(const lds_u32x4*)(tile + at.row[s] + row0 * (DT * 2));
 }
 
 // Operand of a product over the rows (the transposed tile): lane l gives value
@@ -120,16 +149,11 @@ __device__ __forceinline__ u32x4 row_operand(const lds_u8* tile, int row0, int s
 // transposing read takes from 16 lanes the addresses of 4 rows x 16 values, 4
 // values a lane, and gives lane i the 4 rows' value i.
 template <int DT>
-__device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, int db, int lane) {
-  const int i = lane & 15, h = lane >> 5;
-  const int chunk = 4 * db + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+__device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, int db, const LaneAt<DT>& at) {
   s16x4 v[2];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int r = 8 * j + 4 * h + (i >> 2);
-    v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4*)(tile + (row0 + r) * (DT * 2) + ((chunk ^ row_slot<DT>(r)) << 4) + ((i & 1) << 3)));
-  }
+  for (int j = 0; j < 2; ++j)
+    v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + at.col[db][j] + row0 * (DT * 2)));
   return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -153,6 +177,7 @@ struct Paged {
   int64_t table_stride, k_page, v_page;  // elements
   int most, pages;         // tokens that a table row reaches; pages of the cache
   FastDiv page;            // tokens of a page
+  int whole;               // whether pages hold whole 16s of tokens
 };
 
 struct AttnArgs {
@@ -262,13 +287,41 @@ __device__ __forceinline__ const uint16_t* kv_row(const Rows16& r, int64_t page_
   return p;
 }
 
+// Copies N consecutive rows of DT values, all of them valid and the first at
+// the (wave-uniform) `row`, to rows slot0 .. of a tile.  The lanes differ by 32
+// bits of offset only: the address arithmetic of a tile is scalar.
+template <int DT, int N>
+__device__ __forceinline__ void copy_rows(const uint16_t* row, int64_t st, uint8_t* tile, int slot0, int lane) {
+  constexpr int CH = DT / 8, RPI = 64 / CH;
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(uniform_u64(reinterpret_cast<uint64_t>(row)));
+  const uint32_t step = static_cast<uint32_t>(st * 2);
+#pragma unroll
+  for (int x = 0; x < N / RPI; ++x) {
+    const int i = x * RPI + lane / CH;
+    const uint32_t off = (lane / CH) * step + (((lane % CH) ^ row_slot<DT>(i)) << 4);
+    copy16_to_lds(base + static_cast<int64_t>(x * RPI) * (st * 2) + off, tile + (slot0 / RPI + x) * 1024);
+  }
+}
+
 // Copies a wave's W consecutive rows of a tile (the first of them row `row0` of
-// the tile) into LDS: keys and values, zeros past the sequence's end and past
-// D.  `mine` is where the row of lane % W is (row0 + lane % W).
+// the tile, a multiple of 16) into LDS: keys and values, zeros past the
+// sequence's end and past D.  `mine` is where the row of lane % W is.
 template <int DT, int W, bool kPaged>
-__device__ __forceinline__ void fetch_rows(const AttnArgs& a, int hk, KvAt mine, int key0, int row0, int end,
+__device__ __forceinline__ void fetch_rows(const AttnArgs& a, const Seq& s, int hk, KvAt mine, int key0, int row0,
                                            uint8_t* kt, uint8_t* vt, int lane) {
   constexpr int CH = DT / 8, RPI = 64 / CH;
+  const int first = key0 + row0;
+  if (first + W <= s.Lk && a.D == DT && (!kPaged || a.paged.whole)) {
+    constexpr int N = kPaged ? 16 : W;  // 16 rows from a multiple of 16 on are in one page
+#pragma unroll
+    for (int h = 0; h < W; h += N) {
+      KvAt u{0, s.k0 + first};
+      if constexpr (kPaged) u = KvAt{__builtin_amdgcn_readlane(mine.page, h), __builtin_amdgcn_readlane(mine.at, h)};
+      copy_rows<DT, N>(kv_row<kPaged>(a.k, a.paged.k_page, hk, u), a.k.st, kt, row0 + h, lane);
+      copy_rows<DT, N>(kv_row<kPaged>(a.v, a.paged.v_page, hk, u), a.v.st, vt, row0 + h, lane);
+    }
+    return;
+  }
 #pragma unroll
   for (int x = 0; x < W / RPI; ++x) {
     const int i = x * RPI + lane / CH, row = row0 + i;
@@ -280,7 +333,7 @@ __device__ __forceinline__ void fetch_rows(const AttnArgs& a, int hk, KvAt mine,
       at.at = mine.at - lane % W + i;
     }
     const int ch = (lane % CH) ^ row_slot<DT>(row);
-    const bool in = key0 + row < end && ch * 8 < a.D;
+    const bool in = key0 + row < s.Lk && ch * 8 < a.D;
     const uint16_t* kp = kv_row<kPaged>(a.k, a.paged.k_page, hk, at) + ch * 8;
     const uint16_t* vp = kv_row<kPaged>(a.v, a.paged.v_page, hk, at) + ch * 8;
     copy16_to_lds(in ? static_cast<const void*>(kp) : g_attn_zeros, kt + (row0 / RPI + x) * 1024);

@@ -255,7 +255,7 @@ namespace {
 bool attention_sizes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D) {
   constexpr int64_t kMost = (int64_t{1} << 31) - 4096;
   return B >= 1 && T >= 0 && S >= 0 && H >= 1 && Hk >= 1 && H % Hk == 0 && D >= 8 && D <= 128 && D % 8 == 0 &&
-         H <= 65536 && B < kMost && S < kMost && T < kMost / H;
+         H <= 65536 && B < kMost && S < kMost / Hk && T < kMost / H;
 }
 }  // namespace
 
@@ -276,6 +276,23 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
   const PagedPlan p = paged_plan(B, T, H, Hk, max_context);
   if (p.splits == 1) return 0;
   return mul_sat(mul_sat(static_cast<size_t>(T * H), static_cast<size_t>(D + 2)), 4 * static_cast<size_t>(p.splits));
+}
+
+// Workgroups of 64 keys, two to a CU: fewer than 1024 are cut until there are as
+// many, because those of the first keys run twice as long as the average and
+// hold up the end.  Measured (2 x 2048 tokens, 8 key heads, 528 workgroups, us
+// with the join): whole 275, in 2 parts 193, in 4 parts 218.
+int backward_splits(int64_t B, int64_t S, int64_t Hk) {
+  const int64_t groups = std::max<int64_t>(1, (ceil_div(S, 64) + B) * Hk);
+  return static_cast<int>(std::min<int64_t>(8, ceil_div(1024, groups)));
+}
+
+size_t backward_workspace(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D) {
+  if (!attention_sizes(B, T, S, H, Hk, D)) return 0;
+  const size_t rows = static_cast<size_t>(ceil_div(T * H, 4) * 4);  // (the parts stay 16-byte aligned)
+  const size_t splits = static_cast<size_t>(backward_splits(B, S, Hk));
+  const size_t part = mul_sat(mul_sat(static_cast<size_t>(S * Hk), static_cast<size_t>(D)), splits > 1 ? 2 * splits : 0);
+  return mul_sat(add_sat(add_sat(rows, part), 2 * kBackMaxima), sizeof(float));
 }
 
 int64_t cached_most(int64_t width, int64_t page_size) {
@@ -302,8 +319,8 @@ int check_attention_layout(const char* fn, const void* q, const void* k, const v
   GPTQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0,
                GPTQ_ERR_ARG, "%s: q, k and v have to be 16-byte aligned", fn);
   for (int i = 0; i < n; ++i)
-    GPTQ_REQUIRE(strides[i] % 8 == 0, GPTQ_ERR_SHAPE, "%s: strides have to be multiples of 8 elements (got %lld)", fn,
-                 static_cast<long long>(strides[i]));
+    GPTQ_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, GPTQ_ERR_SHAPE,
+                 "%s: strides have to be multiples of 8 elements (got %lld)", fn, static_cast<long long>(strides[i]));
   return GPTQ_OK;
 }
 

@@ -108,6 +108,11 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context);
 size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context);
+// The gradient: workgroups of the first kernel, into how many parts the query
+// rows of each 64 keys are cut, and the workspace.
+constexpr int kBackMaxima = 1024;
+int backward_splits(int64_t B, int64_t S, int64_t Hk);
+size_t backward_workspace(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D);
 // tokens that a row of `width` pages reaches, as far as the kernels count
 int64_t cached_most(int64_t width, int64_t page_size);
 // argument checks of the attention entry points (a gptq_status)

@@ -182,7 +182,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward(
   const int64_t T = q.size(0), H = q.size(1), D = q.size(2);
   at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
              dv = at::empty(v.sizes(), v.options());
-  const size_t bytes = gptq_attention_backward_workspace_size(T, H);
+  const size_t bytes = gptq_attention_backward_workspace_size(cu_q ? cq.numel() - 1 : 1, T, k.size(0), H, k.size(1), D);
   at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
   const int32_t* pq = cu_q ? cq.const_data_ptr<int32_t>() : nullptr;
   GPTQ_CALL(gptq_attention_backward, grad.const_data_ptr(), q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),

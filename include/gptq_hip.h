@@ -378,7 +378,9 @@ int gptq_attention(const void* q, const void* k, const void* v, int dtype,
  * rounded to the inputs' type (fp16: times a power of two that keeps them in
  * its range) before they multiply rows; sums are fp32.  A row that is not
  * finite may leave any gradient of its own sequence not finite. */
-size_t gptq_attention_backward_workspace_size(int64_t T, int64_t H);
+size_t gptq_attention_backward_workspace_size(int64_t B, int64_t T, int64_t S,
+                                              int64_t H, int64_t Hk,
+                                              int64_t D);
 int gptq_attention_backward(const void* grad, const void* q, const void* k,
                             const void* v, const void* out,
                             const void* out_rest, const float* lse, int dtype,

@@ -109,9 +109,13 @@ def test_workspaces(lib):
     for bad in [(0, 1, 4, 4, 64, 9), (1, -1, 4, 4, 64, 9), (1, 1, 4, 3, 64, 9), (1, 1, 4, 4, 60, 9),
                 (1, 1, 4, 4, 136, 9), (1, 2 ** 62, 4, 4, 64, 9), (2 ** 62, 1, 4, 4, 64, 9)]:
         assert size(*bad) == 0
-    assert lib.gptq_attention_backward_workspace_size(10, 4) == 4 * (40 + 2048)
-    assert lib.gptq_attention_backward_workspace_size(-1, 4) == 0
-    assert lib.gptq_attention_backward_workspace_size(2 ** 62, 2 ** 62) == 2 ** 64 - 1
+    back = lib.gptq_attention_backward_workspace_size
+    assert back(1, 10, 10, 4, 4, 64) == 4 * (40 + 2048 + 2 * 8 * 10 * 4 * 64)  # few keys: 8 parts of the rows
+    assert back(2, 4096, 4096, 32, 8, 128) == 4 * (4096 * 32 + 2048 + 2 * 2 * 4096 * 8 * 128)
+    assert back(1, 16384, 16384, 32, 8, 128) == 4 * (16384 * 32 + 2048)        # many: whole
+    assert back(1, 3, 3, 1, 1, 8) % 16 == 0
+    for bad in [(1, -1, 4, 4, 4, 64), (1, 2 ** 62, 4, 4, 4, 64), (1, 4, 2 ** 62, 4, 4, 64), (1, 4, 4, 4, 3, 64)]:
+        assert back(*bad) == 0
 
 
 def test_refusals_before_a_launch(lib):
