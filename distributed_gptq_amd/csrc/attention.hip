@@ -315,17 +315,17 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
 
 // -------------------------------------------------------------- few rows ----
 // A workgroup has up to 32 packed rows and its 4 waves share the keys, every
-// wave tiles of 32 of its own (t0 + wave, + 4, ...) through two LDS buffers of
-// its own, so that no wave waits for another before the end, where the four
-// sums are joined.  For one token a sequence: bound by the cache's bytes.
+// wave tiles of 32 of its own (t0 + wave, + 4, ...) through an LDS buffer of its
+// own, so that no wave waits for another before the end, where the four sums are
+// joined.  For one token a sequence: bound by the cache's bytes.  Two workgroups
+// run on a CU, so that of 8 waves with 16 KB each (heads of 128) most have their
+// copies in flight at any time, and one's start and end hide behind the other.
 constexpr int kFew = 32;
 template <int DT>
-__shared__ __attribute__((aligned(1024))) uint8_t g_few0[4][2][kFew * DT * 2];
-template <int DT>
-__shared__ __attribute__((aligned(1024))) uint8_t g_few1[4][2][kFew * DT * 2];
+__shared__ __attribute__((aligned(1024))) uint8_t g_few[4][2][kFew * DT * 2];
 
 template <bool kBF16, int DT>
-__global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a, int slots) {
+__global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots) {
   constexpr int R = 32;
   __shared__ float stats[2][4][R];
   __shared__ int redo[R];
@@ -351,7 +351,8 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a, int slots)
   const int last = last_key(a, s, div_by(last_r, a.G));
   const int end = last < 0 ? 0 : last + 1;
   const int tiles = (end + kFew - 1) / kFew;
-  const int per = (tiles + a.splits - 1) / a.splits;
+  int per = (tiles + a.splits - 1) / a.splits;
+  per = per < 4 ? 4 : per;  // (a tile for each wave)
   const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
   u32x4 q[DT / 16];
@@ -388,18 +389,11 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a, int slots)
     wait_lgkm<0>();
     wave_sync();
   };
-  int t = t0 + wave;
-  if (t < t1) {
-    fetch(t, &g_few0<DT>[wave][0][0], &g_few0<DT>[wave][1][0]);
-    for (; t < t1; t += 8) {
-      landed();
-      if (t + 4 < t1) fetch(t + 4, &g_few1<DT>[wave][0][0], &g_few1<DT>[wave][1][0]);
-      use(t, (const lds_u8*)&g_few0<DT>[wave][0][0], (const lds_u8*)&g_few0<DT>[wave][1][0]);
-      if (t + 4 >= t1) break;
-      landed();
-      if (t + 8 < t1) fetch(t + 8, &g_few0<DT>[wave][0][0], &g_few0<DT>[wave][1][0]);
-      use(t + 4, (const lds_u8*)&g_few1<DT>[wave][0][0], (const lds_u8*)&g_few1<DT>[wave][1][0]);
-    }
+  for (int t = t0 + wave; t < t1; t += 4) {
+    fetch(t, &g_few<DT>[wave][0][0], &g_few<DT>[wave][1][0]);
+    landed();
+    use(t, (const lds_u8*)&g_few<DT>[wave][0][0], (const lds_u8*)&g_few<DT>[wave][1][0]);
+    landed();
   }
   const float l1 = col.l + other_half(col.l);
   if (half == 0) {
@@ -410,13 +404,13 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a, int slots)
   __syncthreads();
 
   // joined: the waves' sums at the largest maximum, each wave's of channel d
-  // and column c at (wave * DT + d) * 32 + c of the first buffer
+  // and column c at (wave * DT + d) * 32 + c of the buffers
   const int c = lane & 31;
   const float m = fmaxf(fmaxf(stats[0][0][c], stats[0][1][c]), fmaxf(stats[0][2][c], stats[0][3][c]));
   float l = 0.0f;
 #pragma unroll
   for (int w = 0; w < 4; ++w) l += stats[1][w][c] * exp2f(stats[0][w][c] - m);
-  lds_f32* sums = (lds_f32*)&g_few0<DT>[0][0][0];
+  lds_f32* sums = (lds_f32*)&g_few<DT>[0][0][0];
   const float scale = exp2f(col.m - m);
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db)
@@ -490,18 +484,34 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   const float* mm = a.part + a.splits * rows * a.D;
   float m = -INFINITY, l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (inside) {
-#pragma unroll 4
-    for (int sp = group % kGroups; sp < a.splits; sp += kGroups) m = fmaxf(m, mm[sp * rows + row]);
-    const float m0 = m == -INFINITY ? 0.0f : m;
-#pragma unroll 4
-    for (int sp = group % kGroups; sp < a.splits; sp += kGroups) {
-      const float w = exp2f(mm[sp * rows + row] - m0);  // 0 without keys
-      const float ls = mm[(a.splits + sp) * rows + row];
-      const f32x4 x = d < a.D ? *reinterpret_cast<const f32x4*>(a.part + (sp * rows + row) * a.D + d) : o;
-      l = fmaf(w, ls, l);
+  // 8 splits at a time, all their loads together
+  for (int s0 = group % kGroups; inside && s0 < a.splits; s0 += 8 * kGroups) {
+    float ms[8], ls[8];
+    f32x4 x[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[e], o[e]);
+    for (int i = 0; i < 8; ++i) {
+      const int sp = s0 + i * kGroups;
+      const bool is = sp < a.splits;
+      const int64_t at = (is ? sp : s0) * rows + row;
+      ms[i] = is ? mm[at] : -INFINITY;
+      ls[i] = mm[a.splits * rows + at];
+      x[i] = *reinterpret_cast<const f32x4*>(a.part + at * a.D + (d < a.D ? d : 0));
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, ms[i]);
+    const float m0 = top == -INFINITY ? 0.0f : top;
+    const float keep = __builtin_amdgcn_exp2f(m - m0);
+    m = top;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = __builtin_amdgcn_exp2f(ms[i] - m0);  // 0 without keys
+      l = fmaf(w, ls[i], l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[i][e], o[e]);
     }
   }
   if constexpr (kGroups > 1) {
