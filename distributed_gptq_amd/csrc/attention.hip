@@ -34,19 +34,21 @@ struct Column {
 
 // Adds NK x 32 keys with scores s (raw q k) to the column's sums.  `value`
 // gives the operand of value rows 16 ks .. of the tile, channels 32 db ...
-// kTrain: what the rounding of the weights left is multiplied too.  The
-// gradient subtracts delta = g o from every g v of a row, so that an error of o
-// reaches all its keys alike and adds up in dq and dk where errors of single
-// weights cancel (measured on 2 x 2048 tokens, bf16: error of dq 1.55 times
-// that of one rounding with the rounded weights and output, 1.43 so).
-template <bool kBF16, int DT, int NK, bool kTrain, class Value>
+// kRest: what the rounding of the weights left is multiplied too.  For few rows
+// over a cache, whose bytes take longer than both products; and where the
+// gradient follows, which subtracts delta = g o from every g v of a row, so that
+// an error of o reaches all its keys alike and adds up in dq and dk where errors
+// of single weights cancel (2 x 2048 tokens, bf16: error of dq against 64 bits
+// 1.55 times that of its rounding alone with the rounded weights and output, 1.45
+// so).
+template <bool kBF16, int DT, int NK, bool kRest, class Value>
 __device__ __forceinline__ void softmax_step(Column<DT>& col, f32x16 (&s)[NK], float c, Value&& value) {
   float t = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t = fmaxf(t, s[kt][i]);
-  t = fmaxf(t, other_half(t)) * c - kBias<kBF16>;
+    for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);  // (fmaxf quiets its arguments first)
+  t = __builtin_elementwise_maximum(t, other_half(t)) * c - kBias<kBF16>;
   if (__builtin_expect(__ballot(t > col.m + kSlack) != 0, 0)) {
     const float m = fmaxf(col.m, t);
     const float alpha = __builtin_amdgcn_exp2f(col.m - m);
@@ -73,7 +75,7 @@ __device__ __forceinline__ void softmax_step(Column<DT>& col, f32x16 (&s)[NK], f
     for (int db = 0; db < DT / 32; ++db) {
       const u32x4 v = value(ks, db);
       col.o[db] = mma32<kBF16>(v, p, col.o[db]);
-      if constexpr (kTrain) col.o[db] = mma32<kBF16>(v, operand_rest<kBF16>(s[ks / 2], 8 * (ks % 2), p), col.o[db]);
+      if constexpr (kRest) col.o[db] = mma32<kBF16>(v, operand_rest<kBF16>(s[ks / 2], 8 * (ks % 2), p), col.o[db]);
     }
   }
 }
@@ -260,6 +262,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
     for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
       for (int n = 0; n < 2; ++n) sc[n] = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, where), q[d], sc[n]);
+    reads_ahead<DT / 8, 8>();
     if (key0 + kKeys - 1 > full) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -380,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
       for (int i = 0; i < 16; ++i)
         if (key0 + acc_row(i, half) > limit) sc[0][i] = -INFINITY;
     }
-    softmax_step<kBF16, DT, 1, false>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
+    softmax_step<kBF16, DT, 1, true>(col, sc, a.c, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
   };
   // one wave's copies are only its own: they have to have landed before its
   // reads, and its reads of a buffer to be done before the next copies into it

@@ -157,6 +157,18 @@ __device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, in
   return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The order of a run of N pairs of an LDS read and an MFMA (two pairs of them at
+// a time): kAhead reads first, so that no MFMA waits for a read just issued.
+template <int N, int kAhead>
+__device__ __forceinline__ void reads_ahead() {
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+  sfor<0, (N - kAhead) / 2>([](auto) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+  });
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+}
+
 // 16 bytes per lane from memory to LDS, lane l's at lds + 16 l.
 __device__ __forceinline__ void copy16_to_lds(const void* from, uint8_t* lds) {
   __builtin_amdgcn_global_load_lds((gbl_void*)from, (lds_void*)lds, 16, 0, 0);

@@ -99,7 +99,7 @@ int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 
 at::Tensor int32_of(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", the queries are on ", like.device());
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " has to be int32 or int64");
-  return t.to(at::kInt).contiguous();
+  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
 }
 
 void check_heads(const char* fn, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t dim) {

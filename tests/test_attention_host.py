@@ -145,3 +145,4 @@ def test_refusals_before_a_launch(lib):
     rc = lib.gptq_rotary_append(x, x, x, 1, 64, 64, 64, 64, 64, 64, null, 0, 0, null, 0, x, 0, 4, 1, 1, 1, 64, x, x, 64,
                                 64, 64, x, 64, 64, 64, null)
     assert rc == _lib.ERR_ARG
+    assert forward(T=0) == _lib.OK and lib.gptq_last_error() == b""  # (a call that succeeds clears the message)
