@@ -48,7 +48,7 @@ __device__ __forceinline__ void softmax_step(Column<DT>& col, f32x16 (&s)[NK], f
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);  // (fmaxf quiets its arguments first)
-  t = __builtin_elementwise_maximum(t, other_half(t)) * c - kBias<kBF16>;
+  t = half_max(t) * c - kBias<kBF16>;
   if (__builtin_expect(__ballot(t > col.m + kSlack) != 0, 0)) {
     const float m = fmaxf(col.m, t);
     const float alpha = __builtin_amdgcn_exp2f(col.m - m);
@@ -297,10 +297,10 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
   const int k0 = t0 * kKeys;
   const int k1 = t1 * kKeys < limit + 1 ? t1 * kKeys : limit + 1;
   const bool none = k1 <= k0;
-  const float l = col.l + other_half(col.l);
+  const float l = half_sum(col.l);
   const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
   const bool fine = finite_column(col);
-  const bool bad = inside && !none && !(fine && other_half(fine ? 0.0f : 1.0f) == 0.0f);
+  const bool bad = inside && !none && half_sum(fine ? 0.0f : 1.0f) != 0.0f;
   if (inside) {
     if (!bad) store_column<kBF16, DT, kTrain>(a, col, l, row, none, split, half);
     if (half == 0) store_stats(a, col.m, l, row, none, split);
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
     use(t, (const lds_u8*)&g_few<DT>[wave][0][0], (const lds_u8*)&g_few<DT>[wave][1][0]);
     landed();
   }
-  const float l1 = col.l + other_half(col.l);
+  const float l1 = half_sum(col.l);
   if (half == 0) {
     stats[0][wave][lane] = col.m;
     stats[1][wave][lane] = l1;

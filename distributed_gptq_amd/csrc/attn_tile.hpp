@@ -91,7 +91,22 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
+// a column's two lanes, l and l + 32: their values, in both
+__device__ __forceinline__ void both_halves(float v, float& low, float& high) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  low = __uint_as_float(r[0]);
+  high = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float half_max(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return __builtin_elementwise_maximum(a, b);
+}
+__device__ __forceinline__ float half_sum(float v) {
+  float a, b;
+  both_halves(v, a, b);
+  return a + b;
+}
 
 // ------------------------------------------------------------------- LDS ----
 // A tile row holds DT 16-bit values in 16-byte chunks, chunk c at slot
