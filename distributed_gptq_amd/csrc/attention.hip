@@ -594,8 +594,8 @@ extern "C" int gptq_attention(const void* q, const void* k, const void* v, int d
   GPTQ_REQUIRE(q && out && (S == 0 || (k && v)), GPTQ_ERR_ARG, "gptq_attention: null pointer");
   GPTQ_REQUIRE(B == 1 || (cu_q && cu_k), GPTQ_ERR_ARG, "gptq_attention: %lld sequences without their offsets",
                static_cast<long long>(B));
-  const int64_t strides[] = {q_token, q_head, k_token, k_head, v_token, v_head};
-  rc = plan::check_attention_layout("gptq_attention", q, k, v, strides, 6);
+  const int64_t strides[] = {q_token, k_token, v_token, q_head, k_head, v_head};
+  rc = plan::check_attention_layout("gptq_attention", q, k, v, strides, 3, 6);
   if (rc != GPTQ_OK) return rc;
   AttnArgs a{};
   a.q = {static_cast<const uint16_t*>(q), q_token, q_head};
@@ -639,8 +639,8 @@ extern "C" int gptq_paged_attention(const void* q, const void* k_cache, const vo
   GPTQ_REQUIRE(cu_q || T == B, GPTQ_ERR_SHAPE,
                "gptq_paged_attention: %lld new tokens of %lld sequences without their offsets", static_cast<long long>(T),
                static_cast<long long>(B));
-  const int64_t strides[] = {q_token, q_head, k_page, k_token, k_head, v_page, v_token, v_head};
-  rc = plan::check_attention_layout("gptq_paged_attention", q, k_cache, v_cache, strides, 8);
+  const int64_t strides[] = {q_token, k_token, v_token, q_head, k_page, k_head, v_page, v_head};
+  rc = plan::check_attention_layout("gptq_paged_attention", q, k_cache, v_cache, strides, 3, 8);
   if (rc != GPTQ_OK) return rc;
   const plan::PagedPlan p = plan::paged_plan(B, T, H, Hk, max_context);
   const size_t need = plan::paged_workspace(B, T, H, Hk, D, max_context);

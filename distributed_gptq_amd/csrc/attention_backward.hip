@@ -38,19 +38,17 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// e for all of a kernel's ds, by the first 256 threads of a workgroup (one barrier)
+// e for all of a kernel's ds, by the 256 threads of a workgroup (one barrier)
 __device__ __forceinline__ float ds_shift(const BackArgs& a, float (*room)[4]) {
   float g = 0.0f, v = 0.0f;
-  if (threadIdx.x < 256) {
 #pragma unroll
-    for (int x = 0; x < kMaxima / 256; ++x) {
-      g = fmaxf(g, a.maxima[256 * x + threadIdx.x]);
-      v = fmaxf(v, a.maxima[kMaxima + 256 * x + threadIdx.x]);
-    }
+  for (int x = 0; x < kMaxima / 256; ++x) {
+    g = fmaxf(g, a.maxima[256 * x + threadIdx.x]);
+    v = fmaxf(v, a.maxima[kMaxima + 256 * x + threadIdx.x]);
   }
   g = wave_max(g);
   v = wave_max(v);
-  if (threadIdx.x < 256 && (threadIdx.x & 63) == 0) room[0][threadIdx.x >> 6] = g, room[1][threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) room[0][threadIdx.x >> 6] = g, room[1][threadIdx.x >> 6] = v;
   __syncthreads();
   g = fmaxf(fmaxf(room[0][0], room[0][1]), fmaxf(room[0][2], room[0][3]));
   v = fmaxf(fmaxf(room[1][0], room[1][1]), fmaxf(room[1][2], room[1][3]));
@@ -539,10 +537,10 @@ extern "C" int gptq_attention_backward(const void* grad, const void* q, const vo
                "gptq_attention_backward: null pointer");
   GPTQ_REQUIRE(B == 1 || (cu_q && cu_k), GPTQ_ERR_ARG,
                "gptq_attention_backward: %lld sequences without their offsets", static_cast<long long>(B));
-  const int64_t strides[] = {g_token, g_head, q_token, q_head, k_token, k_head, v_token, v_head};
-  rc = plan::check_attention_layout("gptq_attention_backward", q, k, v, strides, 8);
+  const int64_t strides[] = {g_token, q_token, k_token, v_token, g_head, q_head, k_head, v_head};
+  rc = plan::check_attention_layout("gptq_attention_backward", q, k, v, strides, 4, 8);
   if (rc != GPTQ_OK) return rc;
-  rc = plan::check_attention_layout("gptq_attention_backward", grad, out, out_rest, strides, 2);
+  rc = plan::check_attention_layout("gptq_attention_backward", grad, out, out_rest, nullptr, 0, 0);
   if (rc != GPTQ_OK) return rc;
   const size_t need = plan::backward_workspace(B, T, S, H, Hk, D);
   GPTQ_REQUIRE(workspace && workspace_bytes >= need, GPTQ_ERR_WORKSPACE,

@@ -320,12 +320,14 @@ int check_attention_args(const char* fn, int dtype, int64_t B, int64_t T, int64_
   return GPTQ_OK;
 }
 
-int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides, int n) {
+int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides,
+                           int tokens, int n) {
   GPTQ_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0,
                GPTQ_ERR_ARG, "%s: q, k and v have to be 16-byte aligned", fn);
   for (int i = 0; i < n; ++i)
-    GPTQ_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0, GPTQ_ERR_SHAPE,
-                 "%s: strides have to be multiples of 8 elements (got %lld)", fn, static_cast<long long>(strides[i]));
+    GPTQ_REQUIRE(strides[i] % 8 == 0 && strides[i] >= 0 && (i >= tokens || strides[i] < (int64_t{1} << 28)),
+                 GPTQ_ERR_SHAPE, "%s: strides have to be multiples of 8 elements, a token's below 2^28 (got %lld)", fn,
+                 static_cast<long long>(strides[i]));
   return GPTQ_OK;
 }
 

@@ -118,7 +118,10 @@ int64_t cached_most(int64_t width, int64_t page_size);
 // argument checks of the attention entry points (a gptq_status)
 int check_attention_args(const char* fn, int dtype, int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int64_t D,
                          float scale);
-int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides, int n);
+// `tokens` of the `n` strides, the first ones, are those of a token (the copies
+// of a few of them take 32-bit offsets), the others those of heads and pages
+int check_attention_layout(const char* fn, const void* q, const void* k, const void* v, const int64_t* strides,
+                           int tokens, int n);
 
 }  // namespace plan
 }  // namespace gptq

@@ -126,7 +126,8 @@ def test_refusals_before_a_launch(lib):
         return lib.gptq_attention(q, x, x, dtype, *strides, cu, cu, B, T, S, H, Hk, D, 1, f(scale), x, null, null, null)
     assert forward(dtype=0) == _lib.ERR_DTYPE and b"fp16" in lib.gptq_last_error()
     assert forward(q=null) == _lib.ERR_ARG and forward(q=P(8)) == _lib.ERR_ARG
-    assert forward(strides=(128, 60) * 3) == _lib.ERR_SHAPE
+    assert forward(strides=(128, 60) * 3) == _lib.ERR_SHAPE and forward(strides=(-128, 64) * 3) == _lib.ERR_SHAPE
+    assert forward(strides=(2 ** 28, 64) * 3) == _lib.ERR_SHAPE
     assert forward(Hk=3) == _lib.ERR_SHAPE and forward(D=20) == _lib.ERR_SHAPE and forward(D=256) == _lib.ERR_SHAPE
     assert forward(B=2) == _lib.ERR_ARG and forward(B=0) == _lib.ERR_SHAPE and forward(T=-1) == _lib.ERR_SHAPE
     assert forward(T=2 ** 40) == _lib.ERR_SHAPE and forward(scale=0.0) == _lib.ERR_ARG
