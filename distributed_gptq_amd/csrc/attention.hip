@@ -179,8 +179,12 @@ __device__ __forceinline__ void redo_row(const AttnArgs& a, Seq s, int hk, const
       a.part[(split * (static_cast<int64_t>(a.T) * a.H) + row) * a.D + d] = o[x];
     } else {
       const float y = o[x] / l;
-      a.out[row * a.D + d] = kBF16 ? f32_to_bf16_bits(y) : f32_to_f16_bits(y);
-      if (a.out_rest) a.out_rest[row * a.D + d] = 0;
+      const uint16_t w = kBF16 ? f32_to_bf16_bits(y) : f32_to_f16_bits(y);
+      a.out[row * a.D + d] = w;
+      if (a.out_rest) {
+        const float rest = fabsf(y) < INFINITY ? y - value16<kBF16>(w) : 0.0f;
+        a.out_rest[row * a.D + d] = kBF16 ? f32_to_bf16_bits(rest) : f32_to_f16_bits(rest);
+      }
     }
   }
 }
@@ -499,6 +503,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
       ms[i] = is ? mm[at] : -INFINITY;
       ls[i] = mm[a.splits * rows + at];
       x[i] = *reinterpret_cast<const f32x4*>(a.part + at * a.D + (d < a.D ? d : 0));
+      if (!is) x[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (a part may hold infinities)
     }
     float top = m;
 #pragma unroll

@@ -80,6 +80,25 @@ def test_long_context(dtype):
     check(A().paged_attention(q, kc, vc, table, torch.tensor(context, device="cuda")), expect(q, rows, new))
 
 
+@pytest.mark.parametrize("context", [100, 700, 2500])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_infinite_values_that_a_row_sees(context, dtype):
+    """An infinite value of a key gives that channel its infinity, in however
+    many parts the keys are taken; the other channels are as without it."""
+    q, kc, vc, table, rows = case((1,), (context,), 16, 8, 2, 128, dtype)
+    want = expect(q, rows, (1,))
+    for key in (3, context - 1):
+        for bad in (math.inf, -math.inf):
+            v2 = vc.clone()
+            v2[int(table[0, key // 16]), key % 16, 0, 5] = bad
+            out = A().paged_attention(q, kc, v2, table, torch.tensor([context], device="cuda"))
+            assert bool((out[:, :4, 5] == bad).all())
+            out[:, :4, 5] = 0
+            ref = want[0].clone()
+            ref[:, :4, 5] = 0
+            check(out, (ref, want[1]))
+
+
 def test_strided_cache_and_same_bits():
     """A cache with heads before tokens, and one that is a part of a larger
     tensor, give the same bits as a contiguous one; so do two calls."""
