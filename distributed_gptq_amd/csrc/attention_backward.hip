@@ -19,7 +19,7 @@ struct BackArgs {
   Rows16 g;                      // dL/do
   const uint16_t *o, *o_rest;    // (T, H, D): the output, and what its rounding left
   float* delta;                  // (T, H)
-  float* maxima;                 // 2 x kMaxima: largest |g_i|^2 and |v_j|^2 of each workgroup (fp16)
+  float* maxima;                 // 2 x kMaxima: largest finite |g_i|^2 and |v_j|^2 of each workgroup (fp16)
   float* part;                   // with splits > 1: dk and dv of each split (S, Hk, D) each
   int splits;                    // parts of the rows of each 64 keys
   float scale;
@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
 #pragma unroll
     for (int m = 8; m; m >>= 1) dot += __shfl_xor(dot, m), sq += __shfl_xor(sq, m);
     if (sub == 0) a.delta[row] = dot;
-    most[0] = fmaxf(most[0], sq);
+    if (sq < INFINITY) most[0] = fmaxf(most[0], sq);  // (an infinity makes its ds infinite at any scale)
   }
   if constexpr (!kBF16) {
     const int64_t vrows = static_cast<int64_t>(first_row(a.f.cu_k, a.f.B, a.f.B, a.f.S)) * a.f.Hk;
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
       for (int e = 0; e < 8; ++e) sq = fmaf(v[e], v[e], sq);
 #pragma unroll
       for (int m = 8; m; m >>= 1) sq += __shfl_xor(sq, m);
-      most[1] = fmaxf(most[1], sq);
+      if (sq < INFINITY) most[1] = fmaxf(most[1], sq);
     }
     __shared__ float room[2][4];
 #pragma unroll
@@ -142,6 +142,58 @@ template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_back_b0[kRows * DT * 2];
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_back_b1[kRows * DT * 2];
+
+template <bool kBF16>
+__device__ __forceinline__ uint16_t round16(float x) {
+  return kBF16 ? f32_to_bf16_bits(x) : f32_to_f16_bits(x);
+}
+template <int DT>
+__device__ __forceinline__ bool all_finite(const f32x16 (&x)[DT / 32]) {
+  float worst = 0.0f;
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) worst = fmaf(x[db][i], 0.0f, worst);  // 0, or NaN
+  return worst == 0.0f;
+}
+
+// A row's dq again over the keys up to `limit`, which it sees: where the product
+// of tiles is not finite, which multiplies the zero ds of other keys with those
+// keys.  A lane has a key's ds, then channels lane and lane + 64.
+template <bool kBF16>
+__device__ __forceinline__ void redo_dq(const BackArgs& args, const Seq& s, int hk, int tok, int head, int limit) {
+  const AttnArgs& a = args.f;
+  const int lane = threadIdx.x & 63;
+  const uint16_t* q = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh;
+  const uint16_t* g = args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh;
+  const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
+  float dq[2] = {0.0f, 0.0f};
+  for (int base = 0; base <= limit; base += 64) {
+    const int key = base + lane;
+    float ds = 0.0f;
+    if (key <= limit) {
+      const uint16_t* k = kv_row<false>(a.k, 0, hk, KvAt{0, s.k0 + key});
+      const uint16_t* v = kv_row<false>(a.v, 0, hk, KvAt{0, s.k0 + key});
+      float sc = 0.0f, dp = 0.0f;
+      for (int d = 0; d < a.D; ++d) {
+        sc = fmaf(value16<kBF16>(q[d]), value16<kBF16>(k[d]), sc);
+        dp = fmaf(value16<kBF16>(g[d]), value16<kBF16>(v[d]), dp);
+      }
+      ds = exp2f(fmaf(sc, a.c, -a.lse[row])) * (dp - args.delta[row]);
+    }
+    const int n = limit + 1 - base < 64 ? limit + 1 - base : 64;
+    for (int t = 0; t < n; ++t) {
+      const float w = __shfl(ds, t);
+      const uint16_t* k = kv_row<false>(a.k, 0, hk, KvAt{0, s.k0 + base + t});
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (lane + 64 * x < a.D) dq[x] = fmaf(w, value16<kBF16>(k[lane + 64 * x]), dq[x]);
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    if (lane + 64 * x < a.D) args.dq[row * a.D + lane + 64 * x] = round16<kBF16>(dq[x] * args.scale);
+}
 
 // dq: as the forward pass, 32 packed rows a wave (a lane's column), tiles of 64
 // keys and values in LDS.
@@ -245,7 +297,16 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
       __syncthreads();
     }
   }
-  if (inside) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale * exp2f(-shift), a.D, half);
+  const bool fine = all_finite<DT>(acc);
+  // (with a NaN for delta or lse all of the row is, from its own keys)
+  const bool bad = inside && half_sum(fine ? 0.0f : 1.0f) != 0.0f && lse == lse && delta == delta;
+  if (inside && !bad) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale * exp2f(-shift), a.D, half);
+  uint64_t todo = __ballot(bad && half == 0);
+  while (todo) {
+    const int src = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    redo_dq<kBF16>(args, s, hk, __shfl(tok, src), __shfl(head, src), __shfl(limit, src));
+  }
 }
 
 // dk and dv: a workgroup of 4 waves has 64 keys, whose value rows stay in LDS,
@@ -270,10 +331,12 @@ __shared__ __attribute__((aligned(1024))) uint8_t g_dkv_g1[kBackRows * DT * 2];
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_dkv_v[64 * DT * 2];
 
-// A float as three values of 16 bits, x = sum of part i times unit i, to 24 bits:
-// bf16 has its range; fp16 takes units that keep the parts in its range, scores
-// (up to 2^31) as 2^15, 1 and 2^-10 and deltas as 1, 2^-14 and 0.
-template <bool kBF16, bool kScore>
+// A float x as values of 16 bits, x = sum of part i times unit i: in bf16, which
+// has fp32's range, three parts of unit 1; in fp16 four of 2^15, 2^4, 2^-7 and
+// 2^-14, the rest of each within the next one's range, for |x| < 2^31 to 2^-33 of
+// it or to 2^-39.  (fp16 queries, keys and gradients of a few hundred already give
+// scores and deltas beyond fp16's 65504.)
+template <bool kBF16>
 __device__ __forceinline__ u32x2 parts_of(float x) {
   if constexpr (kBF16) {
     const uint32_t hi = pack16<true>(x, 0.0f) & 0xFFFFu;
@@ -281,18 +344,76 @@ __device__ __forceinline__ u32x2 parts_of(float x) {
     const uint32_t mid = pack16<true>(r1, 0.0f) & 0xFFFFu;
     return u32x2{hi | mid << 16, pack16<true>(r1 - bf16_bits_to_f32(static_cast<uint16_t>(mid)), 0.0f)};
   } else {
-    const float u0 = kScore ? 32768.0f : 1.0f, u1 = kScore ? 1.0f : 6.103515625e-5f;
-    const uint32_t hi = pack16<false>(x / u0, 0.0f) & 0xFFFFu;
-    const float r1 = x - f16_bits_to_f32(static_cast<uint16_t>(hi)) * u0;
-    const uint32_t mid = pack16<false>(r1 / u1, 0.0f) & 0xFFFFu;
-    const float r2 = r1 - f16_bits_to_f32(static_cast<uint16_t>(mid)) * u1;
-    return u32x2{hi | mid << 16, kScore ? pack16<false>(r2 * 1024.0f, 0.0f) : 0u};
+    constexpr float kUnit[4] = {0x1p15f, 0x1p4f, 0x1p-7f, 0x1p-14f}, kInverse[4] = {0x1p-15f, 0x1p-4f, 0x1p7f, 0x1p14f};
+    uint32_t part[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      part[i] = pack16<false>(x * kInverse[i], 0.0f) & 0xFFFFu;
+      x = fmaf(-f16_bits_to_f32(static_cast<uint16_t>(part[i])), kUnit[i], x);
+    }
+    return u32x2{part[0] | part[1] << 16, part[2] | part[3] << 16};
   }
 }
-template <bool kBF16, bool kScore>
+template <bool kBF16>
 __device__ __forceinline__ u32x4 units() {
-  if constexpr (kBF16) return u32x4{0x3F803F80u, 0x3F80u, 0, 0};
-  return kScore ? u32x4{0x3C007800u, 0x1400u, 0, 0} : u32x4{0x04003C00u, 0, 0, 0};
+  return kBF16 ? u32x4{0x3F803F80u, 0x3F80u, 0, 0} : u32x4{0x4C007800u, 0x04002000u, 0, 0};
+}
+
+// A key's gradients again, over the rows that see it only (as redo_dq): tiles
+// [first, last) of 64 rows, a row's weight and ds in a lane, then channels lane
+// and lane + 64.
+template <bool kBF16>
+__device__ __forceinline__ void redo_dkv(const BackArgs& args, const Seq& s, int hk, int key, int t0, int nt, int first,
+                                         int last, int split) {
+  const AttnArgs& a = args.f;
+  const int lane = threadIdx.x & 63, G = static_cast<int>(a.G.d);
+  const uint16_t* k = a.k.p + static_cast<int64_t>(s.k0 + key) * a.k.st + hk * a.k.sh;
+  const uint16_t* v = a.v.p + static_cast<int64_t>(s.k0 + key) * a.v.st + hk * a.v.sh;
+  float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
+  for (int x = first; x < last; ++x) {
+    const int head = hk * G + x / nt, tok0 = (t0 + nt - 1 - x % nt) * kBackRows, tok = tok0 + lane;
+    const uint16_t* q = a.q.p + s.q0 * a.q.st + head * a.q.sh;
+    const uint16_t* g = args.g.p + s.q0 * args.g.st + head * args.g.sh;
+    const bool sees = tok < s.Lq && last_key(a, s, tok) >= key;
+    float p = 0.0f, ds = 0.0f;
+    if (sees) {
+      float sc = 0.0f, dp = 0.0f;
+      for (int d = 0; d < a.D; ++d) {
+        sc = fmaf(value16<kBF16>(q[tok * a.q.st + d]), value16<kBF16>(k[d]), sc);
+        dp = fmaf(value16<kBF16>(g[tok * args.g.st + d]), value16<kBF16>(v[d]), dp);
+      }
+      const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
+      p = exp2f(fmaf(sc, a.c, -a.lse[row]));
+      ds = p * (dp - args.delta[row]);
+    }
+    uint64_t todo = __ballot(sees);
+    while (todo) {
+      const int t = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const float wp = __shfl(p, t), wd = __shfl(ds, t);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int d = lane + 64 * y;
+        if (d >= a.D) continue;
+        dv[y] = fmaf(wp, value16<kBF16>(g[(tok0 + t) * args.g.st + d]), dv[y]);
+        dk[y] = fmaf(wd, value16<kBF16>(q[(tok0 + t) * a.q.st + d]), dk[y]);
+      }
+    }
+  }
+  const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
+  const int64_t all = static_cast<int64_t>(a.S) * a.Hk * a.D;
+#pragma unroll
+  for (int y = 0; y < 2; ++y) {
+    const int d = lane + 64 * y;
+    if (d >= a.D) continue;
+    if (args.splits > 1) {
+      args.part[2 * split * all + row + d] = dk[y] * args.scale;
+      args.part[(2 * split + 1) * all + row + d] = dv[y];
+    } else {
+      args.dk[row + d] = round16<kBF16>(dk[y] * args.scale);
+      args.dv[row + d] = round16<kBF16>(dv[y]);
+    }
+  }
 }
 
 template <bool kBF16, int DT>
@@ -388,9 +509,9 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
     const lds_u8* vt = (const lds_u8*)&g_dkv_v<DT>[0] + (32 * (wave & 1) - 32 * n) * (DT * 2);
     f32x16 sc = zero16(), dp = zero16();
     {
-      const u32x2 l = parts_of<kBF16, true>(half ? 0.0f : lse * inv_c), d = parts_of<kBF16, false>(half ? 0.0f : -delta);
-      sc = mma32<kBF16>(u32x4{l[0], l[1], 0, 0}, units<kBF16, true>(), sc);
-      dp = mma32<kBF16>(u32x4{d[0], d[1], 0, 0}, units<kBF16, false>(), dp);
+      const u32x2 l = parts_of<kBF16>(half ? 0.0f : lse * inv_c), d = parts_of<kBF16>(half ? 0.0f : -delta);
+      sc = mma32<kBF16>(u32x4{l[0], l[1], 0, 0}, units<kBF16>(), sc);
+      dp = mma32<kBF16>(u32x4{d[0], d[1], 0, 0}, units<kBF16>(), dp);
     }
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d) {
@@ -449,7 +570,7 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
       }
   }
   __syncthreads();
-  if (n == 1 || !inside) return;
+  if (n == 1) return;
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
@@ -459,6 +580,15 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
     }
   const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
   const float rk = args.scale * exp2f(-shift), rv = exp2f(kBF16 ? 0.0f : -kWeightShift);
+  const bool fine = all_finite<DT>(dk) && all_finite<DT>(dv);
+  const bool bad = inside && half_sum(fine ? 0.0f : 1.0f) != 0.0f;
+  uint64_t todo = __ballot(bad && half == 0);
+  while (todo) {
+    const int src = __builtin_ctzll(todo);
+    todo &= todo - 1;
+    redo_dkv<kBF16>(args, s, hk, kw + src, t0, nt, first, last, split);
+  }
+  if (!inside || bad) return;
   if (args.splits == 1) {
     store_rows<kBF16, DT>(args.dk + row, dk, rk, a.D, half);
     store_rows<kBF16, DT>(args.dv + row, dv, rv, a.D, half);

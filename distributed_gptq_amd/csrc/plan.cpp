@@ -316,7 +316,8 @@ int check_attention_args(const char* fn, int dtype, int64_t B, int64_t T, int64_
   GPTQ_REQUIRE(attention_sizes(B, T, S, H, Hk, D), GPTQ_ERR_SHAPE,
                "%s: %lld sequences, %lld queries, %lld keys, %lld heads", fn, static_cast<long long>(B),
                static_cast<long long>(T), static_cast<long long>(S), static_cast<long long>(H));
-  GPTQ_REQUIRE(scale >= 1e-30f && scale <= 1e30f, GPTQ_ERR_ARG, "%s: scale %g (it has to lie in [1e-30, 1e30])", fn, scale);
+  // (the logarithm of a row's sum over the scale has to stay among the fp16 parts, below 2^31)
+  GPTQ_REQUIRE(scale >= 1e-7f && scale <= 1e7f, GPTQ_ERR_ARG, "%s: scale %g (it has to lie in [1e-7, 1e7])", fn, scale);
   return GPTQ_OK;
 }
 

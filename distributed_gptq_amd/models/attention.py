@@ -149,7 +149,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
     of their keys unless ``cu_seqlens_k`` gives those.  ``causal``: the last
     query sees the last key, the one before it one key less, and so on; a query
     without a key gives zeros, and gradients of zero.  ``scale``: 1 / sqrt(head_dim)
-    by default."""
+    by default, else within [1e-7, 1e7].  Infinities and NaN reach only the rows
+    and gradients whose sums they are terms of."""
     return _op("attention", q, k, v, cu_seqlens, cu_seqlens_k, causal, _scale(q, scale))
 
 

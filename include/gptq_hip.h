@@ -355,8 +355,8 @@ int gptq_dequantize_tensor(const int8_t* q, int64_t n, int group_size,
  * (query i of Lq sees keys 0 .. i + Lk - Lq); a query that sees no key gives
  * zeros.  Query head h uses key head h / (H / Hk).
  * fp16 or bf16; D a multiple of 8 up to 128, its values contiguous, 16-byte
- * aligned; the strides (elements, multiples of 8) are those of a token and of
- * a head.  out: (T, H, D) contiguous.  lse (T x H fp32, or NULL): the base-2
+ * aligned; the strides (elements, multiples of 8, a token's below 2^28) are
+ * those of a token and of a head.  scale: within [1e-7, 1e7].  out: (T, H, D) contiguous.  lse (T x H fp32, or NULL): the base-2
  * logarithm of sum_j 2^(log2(e) scale q_i k_j), -infinity without keys; out_rest
  * (T, H, D), or NULL: what the rounding of out left, in the same type (16 bits
  * of out together).  gptq_attention_backward takes both.
@@ -376,8 +376,8 @@ int gptq_attention(const void* q, const void* k, const void* v, int dtype,
  * dk_j = scale sum_i ds_ij q_i, dq_i = scale sum_j ds_ij k_j, a key head's sums
  * over its query heads too; the same bits from call to call.  p and ds are
  * rounded to the inputs' type (fp16: times a power of two that keeps them in
- * its range) before they multiply rows; sums are fp32.  A row that is not
- * finite may leave any gradient of its own sequence not finite. */
+ * its range; ds for dq to twice its bits) before they multiply rows; sums are
+ * fp32.  Infinities and NaN reach the gradients whose sums they are terms of. */
 size_t gptq_attention_backward_workspace_size(int64_t B, int64_t T, int64_t S,
                                               int64_t H, int64_t Hk,
                                               int64_t D);

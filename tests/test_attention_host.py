@@ -131,6 +131,7 @@ def test_refusals_before_a_launch(lib):
     assert forward(Hk=3) == _lib.ERR_SHAPE and forward(D=20) == _lib.ERR_SHAPE and forward(D=256) == _lib.ERR_SHAPE
     assert forward(B=2) == _lib.ERR_ARG and forward(B=0) == _lib.ERR_SHAPE and forward(T=-1) == _lib.ERR_SHAPE
     assert forward(T=2 ** 40) == _lib.ERR_SHAPE and forward(scale=0.0) == _lib.ERR_ARG
+    assert forward(scale=1e-8) == _lib.ERR_ARG and forward(scale=1e8) == _lib.ERR_ARG
     assert forward(T=0) == _lib.OK
 
     def paged(ws=0, page=16, pages=4, T=1, B=1, cu=null, n=100000):

@@ -312,3 +312,58 @@ def test_second_derivative_is_refused():
         torch.autograd.grad(g.float().sum(), x, retain_graph=True)
     with pytest.raises(RuntimeError, match="once"):
         g.float().sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("Hk,D", [(2, 128), (4, 40)])
+def test_gradient_not_finite_in_places_that_a_row_does_not_see(Hk, D, dtype):
+    """A token's dq is the same whatever later keys and values hold, a key's dk
+    and dv whatever earlier queries and gradients do, and those of another
+    sequence in any case."""
+    lens = (100, 77)
+    q, k, v, grad, cu, _ = inputs(lens, lens, 4, Hk, D, dtype, seed=12)
+    want = packed(q, k, v, cu, cu, grad)
+
+    def part(name, at):
+        return tuple(x[at] for x in want[name])
+    other = slice(100, None)
+    for bad in (math.nan, math.inf, -math.inf):
+        for place in (0, 5, 63, 64, 99):
+            k2, v2 = k.clone(), v.clone()
+            k2[place], v2[place] = bad, bad
+            got = run(q, k2, v2, grad, on_gpu(cu), None)
+            check(got["dq"][:place], part("dq", slice(0, place)))
+            assert not torch.isfinite(got["dq"][place:100]).any()
+            for name in ("dq", "dk", "dv"):
+                check(got[name][other], part(name, other))
+            for which in (0, 1):
+                q2, grad2 = q.clone(), grad.clone()
+                (q2, grad2)[which][place] = bad
+                got = run(q2, k, v, grad2, on_gpu(cu), None)
+                later = slice(place + 1, None)
+                for name in ("dq", "dk", "dv"):
+                    check(got[name][later], part(name, later))
+                check(got["dq"][:place], part("dq", slice(0, place)))
+                assert not torch.isfinite(got["dk"][:place + 1]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_large_products(dtype):
+    """Gradients whose products with the output pass 65504, and products of
+    queries and keys beyond 2^27, both of values well within fp16."""
+    L, H, Hk, D = 100, 4, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(21)
+    q, k = rand(g, L, H, D, dtype=dtype), rand(g, L, Hk, D, dtype=dtype)
+    v, grad = rand(g, L, Hk, D, dtype=dtype) + 60, rand(g, L, H, D, dtype=dtype) + 20
+    want = one(q, k, v, grad)
+    assert (want["out"][0] * grad.double()).sum(-1).min() > 65504
+    got = run(q, k, v, grad, None, None)
+    for name in want:
+        check(got[name], want[name])
+    q, k = q * 100 + 1500, k * 100 + 1500
+    v, grad = v - 60, grad - 20
+    assert (q.double() @ k[0].double().t()).min() > 2 ** 27
+    want = one(q, k, v, grad, scale=1e-6)
+    got = run(q, k, v, grad, None, None, scale=1e-6)
+    for name in want:
+        check(got[name], want[name])
