@@ -58,7 +58,8 @@ __device__ __forceinline__ float ds_shift(const BackArgs& a, float (*room)[4]) {
   return e < -100.0f ? -100.0f : e > 100.0f ? 100.0f : e;
 }
 
-// delta, and for fp16 the maxima.  16 lanes a row, 8 values a lane.
+// delta, and for fp16 the maxima.  16 lanes a row, 8 values a lane.  Bound by
+// memory: 12 us for 4096 tokens of 32 heads of 128 (101 MB, in part cached).
 template <bool kBF16>
 __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
   const int sub = threadIdx.x & 15, d = 8 * sub;
@@ -203,6 +204,9 @@ __device__ __forceinline__ void redo_dq(const BackArgs& args, const Seq& s, int 
 // (along q) cancels in dq, but not in the errors of rounded ds: with them alone
 // the error of dq against 64 bits is 1.45 times that of its own rounding for 2048
 // tokens and heads of 128, 1.50 for 3400 and heads of 64, and grows on.
+//
+// Bound by the MFMAs (busy 55% of the cycles) beside the vector instructions: 146
+// us for 2 x 2048 tokens, 32 over 8 heads of 128, of which the rests take 29.
 template <bool kBF16, int DT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slots) {
   constexpr int R = 128, W = kRows / 4;
@@ -319,6 +323,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
 // rows' lse and delta have no place in either, and are added by one MFMA more
 // each, as 16 further channels of q and g (their parts, below) and of k and v
 // (the parts' units).
+//
+// 183 us and 13 of the join for 2 x 2048 tokens, 32 over 8 heads of 128 (MFMAs
+// busy 43% of the cycles, no LDS conflicts); one workgroup of 8 waves a CU, lse
+// and delta in registers: 218.
 constexpr int kBackRows = 64;
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_dkv_q0[kBackRows * DT * 2];

@@ -262,8 +262,11 @@ bool attention_sizes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int
 // Few rows: two workgroups of 4 waves run on each of the 256 CUs, so 512 for one
 // sequence, whose parts are equal; twice that for several, whose lengths differ.
 // Measured (us with the join, 512 / 1024 wanted): 24 sequences of up to 8192
-// tokens 79 / 73, one of 131072 105 / 110.  A part has at least a tile of 32
-// keys for each wave.
+// tokens 78.2 / 70.1, one of 131072 102.8 / 104.9.  A part has at least a tile of
+// 32 keys for each wave.  More rows than 32 go to the kernel of 128, though neither
+// is ahead throughout (us, that kernel / tiles of 32, heads 32 over 8 of 128: 16 new
+// tokens over 8192 26.0 / 21.5, 16 for each of 8 sequences over 4096 35.8 / 42.3, 32
+// for each of 32 over 2048 116 / 94).
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context) {
   PagedPlan p;
   if (!attention_sizes(B, T, 0, H, Hk, 8)) return p;
@@ -285,8 +288,8 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
 
 // Workgroups of 64 keys, two to a CU: fewer than 1024 are cut until there are as
 // many, because those of the first keys run twice as long as the average and
-// hold up the end.  Measured (2 x 2048 tokens, 8 key heads, 528 workgroups, us
-// with the join): whole 275, in 2 parts 193, in 4 parts 218.
+// hold up the end.  Measured (2 x 2048 tokens, 8 key heads, 528 workgroups, us of
+// forward and gradients): whole 535, in 2 parts 456, in 4 parts 479.
 int backward_splits(int64_t B, int64_t S, int64_t Hk) {
   const int64_t groups = std::max<int64_t>(1, (ceil_div(S, 64) + B) * Hk);
   return static_cast<int>(std::min<int64_t>(8, ceil_div(1024, groups)));
