@@ -474,7 +474,11 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
 
   const float inv_c = -1.0f / a.c;
   float n_lse = 0.0f, n_delta = 0.0f;  // of the next tile's row n 32 + lane % 32
-  const int my_lane = lane;
+  // a lane's part of the copies' offsets and of those of lse and delta; opaque in
+  // the loop, where what follows from them is cheaper than registers
+  const uint32_t q_step = (lane / CH) * static_cast<uint32_t>(a.q.st * 2);
+  const uint32_t g_step = (lane / CH) * static_cast<uint32_t>(args.g.st * 2);
+  uint32_t chunk = ((lane % CH) ^ row_slot<DT>(lane / CH)) << 4;
   // tile x: of head x / nt, from the last tokens (which see all keys) on, so that
   // the workgroups of a key head read the same rows at the same time
   auto fetch = [&](int x, uint8_t* qt, uint8_t* gt) {
@@ -482,18 +486,24 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
     const uint16_t* qp = a.q.p + s.q0 * a.q.st + head * a.q.sh;
     const uint16_t* gp = args.g.p + s.q0 * args.g.st + head * args.g.sh;
     const int first = tok0 + wave * W;
-    int lane = my_lane;
-    asm volatile("" : "+v"(lane));
+    asm volatile("" : "+v"(chunk));
     {
-      int tok = tok0 + 32 * n + (lane & 31);
-      tok = tok < s.Lq ? tok : s.Lq - 1;  // (rows past the last are masked)
-      const int64_t at = static_cast<int64_t>(s.q0 + tok) * a.H + head;
-      n_lse = a.lse[at];
-      n_delta = args.delta[at];
+      const int row = tok0 + 32 * n < s.Lq ? tok0 + 32 * n : s.Lq - 1, left = s.Lq - 1 - row;
+      const int64_t at = static_cast<int64_t>(s.q0 + row) * a.H + head;
+      const int more = ((lane & 31) < left ? lane & 31 : left) * a.H;  // (rows past the last are masked)
+      n_lse = a.lse[at + more];
+      n_delta = args.delta[at + more];
     }
     if (first + W <= s.Lq && a.D == DT) {
-      copy_rows<DT, W>(qp + first * a.q.st, a.q.st, qt, wave * W, lane);
-      copy_rows<DT, W>(gp + first * args.g.st, args.g.st, gt, wave * W, lane);
+      auto copy = [&](const uint16_t* p, int64_t st, uint32_t step, uint8_t* tile) {
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(uniform_u64(reinterpret_cast<uint64_t>(p + first * st)));
+#pragma unroll
+        for (int y = 0; y < W / RPI; ++y)  // (row_slot of rows y RPI apart: its other bits)
+          copy16_to_lds(base + static_cast<int64_t>(y * RPI) * (st * 2) + (step + (chunk ^ (row_slot<DT>(y * RPI) << 4))),
+                        tile + (wave * (W / RPI) + y) * 1024);
+      };
+      copy(qp, a.q.st, q_step, qt);
+      copy(gp, args.g.st, g_step, gt);
     } else {
 #pragma unroll
       for (int y = 0; y < W / RPI; ++y) {
