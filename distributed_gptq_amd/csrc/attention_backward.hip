@@ -58,9 +58,9 @@ __device__ __forceinline__ float ds_shift(const BackArgs& a, float (*room)[4]) {
   return e < -100.0f ? -100.0f : e > 100.0f ? 100.0f : e;
 }
 
-// delta, and for fp16 the maxima.  16 lanes a row, 8 values a lane.  Bound by
-// memory: 12 us for 4096 tokens of 32 heads of 128 (101 MB, in part cached).
-template <bool kBF16>
+// For fp16, whose ds need their scale first: delta and the maxima, 16 lanes a row,
+// 8 values a lane.  Bound by memory: 12 us for 4096 tokens of 32 heads of 128 (101
+// MB, in part cached).  In bf16 the dq kernel, which runs first, gives delta.
 __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
   const int sub = threadIdx.x & 15, d = 8 * sub;
   // (rows past the offsets have no gradient, and may hold anything)
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
   auto values = [&](const uint16_t* p, float (&x)[8]) {
     const u32x4 w = d < a.f.D ? *reinterpret_cast<const u32x4*>(p + d) : u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = value16<kBF16>(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
+    for (int e = 0; e < 8; ++e) x[e] = value16<false>(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
   };
   for (int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); row < rows; row += step) {
     const int64_t t = row / a.f.H;
@@ -87,29 +87,27 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(BackArgs a) {
     if (sub == 0) a.delta[row] = dot;
     if (sq < INFINITY) most[0] = fmaxf(most[0], sq);  // (an infinity makes its ds infinite at any scale)
   }
-  if constexpr (!kBF16) {
-    const int64_t vrows = static_cast<int64_t>(first_row(a.f.cu_k, a.f.B, a.f.B, a.f.S)) * a.f.Hk;
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); row < vrows; row += step) {
-      const int64_t t = row / a.f.Hk;
-      float v[8], sq = 0.0f;
-      values(a.f.v.p + t * a.f.v.st + (row - t * a.f.Hk) * a.f.v.sh, v);
+  const int64_t vrows = static_cast<int64_t>(first_row(a.f.cu_k, a.f.B, a.f.B, a.f.S)) * a.f.Hk;
+  for (int64_t row = static_cast<int64_t>(blockIdx.x) * 16 + (threadIdx.x >> 4); row < vrows; row += step) {
+    const int64_t t = row / a.f.Hk;
+    float v[8], sq = 0.0f;
+    values(a.f.v.p + t * a.f.v.st + (row - t * a.f.Hk) * a.f.v.sh, v);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) sq = fmaf(v[e], v[e], sq);
+    for (int e = 0; e < 8; ++e) sq = fmaf(v[e], v[e], sq);
 #pragma unroll
-      for (int m = 8; m; m >>= 1) sq += __shfl_xor(sq, m);
-      if (sq < INFINITY) most[1] = fmaxf(most[1], sq);
-    }
-    __shared__ float room[2][4];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float w = wave_max(most[x]);
-      if ((threadIdx.x & 63) == 0) room[x][threadIdx.x >> 6] = w;
-    }
-    __syncthreads();
-    if (threadIdx.x < 2)
-      a.maxima[threadIdx.x * kMaxima + blockIdx.x] =
-          fmaxf(fmaxf(room[threadIdx.x][0], room[threadIdx.x][1]), fmaxf(room[threadIdx.x][2], room[threadIdx.x][3]));
+    for (int m = 8; m; m >>= 1) sq += __shfl_xor(sq, m);
+    if (sq < INFINITY) most[1] = fmaxf(most[1], sq);
   }
+  __shared__ float room[2][4];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    const float w = wave_max(most[x]);
+    if ((threadIdx.x & 63) == 0) room[x][threadIdx.x >> 6] = w;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2)
+    a.maxima[threadIdx.x * kMaxima + blockIdx.x] =
+        fmaxf(fmaxf(room[threadIdx.x][0], room[threadIdx.x][1]), fmaxf(room[threadIdx.x][2], room[threadIdx.x][3]));
 }
 
 // 32 columns' channels to memory: y = x * r, rounded
@@ -242,7 +240,29 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
   u32x4 q[DT / 16], g[DT / 16];
   load_operand<DT>(q, a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh, inside, a.D, half);
   load_operand<DT>(g, args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh, inside, a.D, half);
-  const float lse = a.lse[row], delta = args.delta[row];
+  const float lse = a.lse[row];
+  float delta;
+  if constexpr (kBF16) {
+    float dot = 0.0f;
+#pragma unroll
+    for (int x = 0; x < DT / 16; ++x) {
+      const int d = 16 * x + 8 * half;
+      if (!inside || d >= a.D) continue;
+      const u32x4 o = *reinterpret_cast<const u32x4*>(args.o + row * a.D + d);
+      const u32x4 rest = *reinterpret_cast<const u32x4*>(args.o_rest + row * a.D + d);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int to = 16 * (e % 2);
+        dot = fmaf(value16<true>(static_cast<uint16_t>(g[x][e / 2] >> to)),
+                   value16<true>(static_cast<uint16_t>(o[e / 2] >> to)) + value16<true>(static_cast<uint16_t>(rest[e / 2] >> to)),
+                   dot);
+      }
+    }
+    delta = half_sum(dot);
+    if (inside && half == 0) args.delta[row] = delta;
+  } else {
+    delta = args.delta[row];
+  }
 
   f32x16 acc[DT / 32];
 #pragma unroll
@@ -642,7 +662,13 @@ int launch(const BackArgs& a, hipStream_t st) {
   const int64_t qs = slots_of(a.f.cu_q, a.f.B, a.f.T, a.f.G.d, 128), ks = slots_of(a.f.cu_k, a.f.B, a.f.S, 1, 64);
   GPTQ_REQUIRE(qs * a.f.Hk < (int64_t{1} << 31) && ks * a.f.Hk * a.splits < (int64_t{1} << 31), GPTQ_ERR_SHAPE,
                "gptq_attention_backward: too many rows");
-  attn_delta_kernel<kBF16><<<kMaxima, 256, 0, st>>>(a);
+  if constexpr (!kBF16) {
+    attn_delta_kernel<<<kMaxima, 256, 0, st>>>(a);
+    const int rc = check_launch("gptq_attention_backward");
+    if (rc != GPTQ_OK) return rc;
+  }
+  if (a.f.T > 0)
+    attn_dq_kernel<kBF16, DT><<<static_cast<uint32_t>(qs * a.f.Hk), 256, 0, st>>>(a, static_cast<int>(qs));
   int rc = check_launch("gptq_attention_backward");
   if (rc != GPTQ_OK) return rc;
   if (a.f.S > 0) {
@@ -654,10 +680,6 @@ int launch(const BackArgs& a, hipStream_t st) {
       attn_dkv_join_kernel<kBF16><<<static_cast<uint32_t>(cdiv(2 * all, 1024)), 256, 0, st>>>(a, all);
     }
   }
-  rc = check_launch("gptq_attention_backward");
-  if (rc != GPTQ_OK) return rc;
-  if (a.f.T > 0)
-    attn_dq_kernel<kBF16, DT><<<static_cast<uint32_t>(qs * a.f.Hk), 256, 0, st>>>(a, static_cast<int>(qs));
   return check_launch("gptq_attention_backward");
 }
 
