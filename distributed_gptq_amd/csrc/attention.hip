@@ -212,7 +212,7 @@ __device__ __forceinline__ bool finite_column(const Column<DT>& col) {
 // overlap these to 2/3 of their sum.  Measured (us; TFLOP/s of the products that
 // the mask leaves): 8192 tokens in four prompts, 32 over 8 heads of 128, 214-221
 // (850-870); 16 x 2048 tokens, 12 heads of 64, 163-166 (630); 512 tokens over
-// 16384 cached ones, 32 over 8 heads, 163-166 (850).  Tiles of 32 keys with 3
+// 16384 cached ones, 32 over 8 heads, 159-166 (840-880).  Tiles of 32 keys with 3
 // workgroups a CU: 3% faster on the prompts, 8% slower with gradients, 50% over a
 // cache.
 template <int DT>

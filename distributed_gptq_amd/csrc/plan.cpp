@@ -289,7 +289,7 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
 // Workgroups of 64 keys, two to a CU: fewer than 1024 are cut until there are as
 // many, because those of the first keys run twice as long as the average and
 // hold up the end.  Measured (2 x 2048 tokens, 8 key heads, 528 workgroups, us of
-// forward and gradients): whole 535, in 2 parts 456, in 4 parts 479.
+// forward and gradients, before two later steps): whole 535, in 2 parts 456, in 4 479.
 int backward_splits(int64_t B, int64_t S, int64_t Hk) {
   const int64_t groups = std::max<int64_t>(1, (ceil_div(S, 64) + B) * Hk);
   return static_cast<int>(std::min<int64_t>(8, ceil_div(1024, groups)));
