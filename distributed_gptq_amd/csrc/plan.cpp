@@ -269,7 +269,7 @@ bool attention_sizes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int
 // for each of 32 over 2048 116 / 94).
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context) {
   PagedPlan p;
-  if (!attention_sizes(B, T, 0, H, Hk, 8)) return p;
+  if (T == 0 || !attention_sizes(B, T, 0, H, Hk, 8)) return p;  // (nothing to launch)
   const int64_t rows = ceil_div(T * (H / Hk), B);  // of a sequence and key head, on average
   p.few = rows <= 32;
   const int64_t groups = (p.few ? ceil_div(rows, 32) : ceil_div(rows, 128)) * B * Hk;
