@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
+#include <limits>
+
 #include "gptq_hip.h"
 
 namespace {
@@ -99,7 +101,9 @@ int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) <= 1 ? 
 at::Tensor int32_of(const at::Tensor& t, const at::Tensor& like, const char* name) {
   TORCH_CHECK_VALUE(t.device() == like.device(), name, " is on ", t.device(), ", the queries are on ", like.device());
   TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " has to be int32 or int64");
-  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+  if (t.scalar_type() == at::kInt) return t.contiguous();
+  // what 32 bits do not hold stays out of every range that the kernels check
+  return t.clamp(std::numeric_limits<int32_t>::min(), std::numeric_limits<int32_t>::max()).to(at::kInt).contiguous();
 }
 
 void check_heads(const char* fn, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t dim) {

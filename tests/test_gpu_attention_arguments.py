@@ -1,0 +1,52 @@
+"""What the attention calls do with index tensors and layouts beyond the
+ordinary ones."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FAR = 2 ** 32
+
+
+def A():
+    from distributed_gptq_amd.models import attention
+    return attention
+
+
+def rand(*shape, seed=0, dtype=torch.float16):
+    g = torch.Generator(device="cuda").manual_seed(seed + sum(shape))
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def long(*values):
+    return torch.tensor(values, dtype=torch.int64, device="cuda")
+
+
+def test_slots_beyond_32_bits_are_not_written():
+    m = A()
+    q, k, v = rand(5, 4, 64), rand(5, 2, 64, seed=1), rand(5, 2, 64, seed=2)
+    kc, vc = rand(3, 16, 2, 64, seed=3), rand(3, 16, 2, 64, seed=4)
+    kw, vw = kc.clone(), vc.clone()
+    kw[0, 7], vw[0, 7] = k[3], v[3]
+    m.rotary_append(q, k, v, None, None, kc, vc, long(FAR, FAR + 5, 3 - FAR, 7, 2 ** 63 - 1))
+    assert torch.equal(kc, kw) and torch.equal(vc, vw)
+
+
+def test_positions_beyond_32_bits_are_those_of_the_tables_ends():
+    m = A()
+    table = m.rotary_table(64, 40)
+    q, k = rand(4, 4, 64), rand(4, 2, 64, seed=1)
+    got = m.rotary(q, k, table, long(FAR + 1, 1 - FAR, 5, 2 ** 63 - 1))
+    want = m.rotary(q, k, table, long(39, 0, 5, 39))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_lengths_pages_and_offsets_beyond_32_bits_are_clamped():
+    m = A()
+    q, kc, vc = rand(2, 4, 64), rand(6, 16, 2, 64, seed=1), rand(6, 16, 2, 64, seed=2)
+    got = m.paged_attention(q, kc, vc, long(0, FAR, 2, 4, -FAR, 1).view(2, 3), long(FAR + 5, 20), max_context=48)
+    want = m.paged_attention(q, kc, vc, long(0, 5, 2, 4, 0, 1).view(2, 3), long(48, 20), max_context=48)
+    assert torch.equal(got, want)
+    assert not m.paged_attention(q, kc, vc, long(0, 1, 2, 3, 4, 5).view(2, 3), long(5 - FAR, -FAR)).any()
+    q, k, v = rand(20, 4, 64), rand(20, 2, 64, seed=1), rand(20, 2, 64, seed=2)
+    assert torch.equal(m.attention(q, k, v, long(0, 9, FAR + 12)), m.attention(q, k, v, long(0, 9, 20)))
