@@ -7,6 +7,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
@@ -304,8 +305,14 @@ c10::TypedOperatorHandle<F> typed_op(const char* name) {
 bool follows(std::initializer_list<const at::Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const at::Tensor* t : ts)
-    if (t->requires_grad()) return true;
+    if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// A tangent of forward-mode differentiation would be lost below autograd.
+void no_tangents(const char* name, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), name, " has no forward-mode derivative");
 }
 
 using torch::autograd::AutogradContext;
@@ -340,6 +347,7 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     static const auto op = typed_op<decltype(attention_backward)>("gptq::attention_backward");
     const auto s = ctx->get_saved_variables();
+    no_tangents("gptq::attention", {&grads[0], &s[0], &s[1], &s[2]});
     at::Tensor dq, dk, dv;
     {
       at::AutoDispatchBelowADInplaceOrView below;
@@ -354,6 +362,7 @@ struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
 at::Tensor attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                               const std::optional<at::Tensor>& cu_q, const std::optional<at::Tensor>& cu_k, bool causal,
                               double scale) {
+  no_tangents("gptq::attention", {&q, &k, &v});
   if (follows({&q, &k, &v})) return AttentionGrad::apply(q, k, v, cu_q, cu_k, causal, scale);
   static const auto op = typed_op<decltype(attention)>("gptq::attention");
   at::AutoDispatchBelowADInplaceOrView below;
@@ -383,6 +392,7 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
 
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& table,
                                                    const at::Tensor& positions, bool interleaved, bool inverse) {
+  no_tangents("gptq::rotary", {&q, &k, &table});
   if (follows({&q, &k})) {
     const variable_list out = RotaryGrad::apply(q, k, table, positions, interleaved, inverse);
     return {out[0], out[1]};
@@ -390,6 +400,31 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
   static const auto op = typed_op<decltype(rotary)>("gptq::rotary");
   at::AutoDispatchBelowADInplaceOrView below;
   return op.call(q, k, table, positions, interleaved, inverse);
+}
+
+// Serving's operators have no gradient at all.
+void no_gradient(const char* name, std::initializer_list<const at::Tensor*> ts) {
+  no_tangents(name, ts);
+  TORCH_CHECK(!follows(ts), name, " records no gradient: call it under torch.no_grad()");
+}
+
+at::Tensor rotary_append_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                  const std::optional<at::Tensor>& table, const std::optional<at::Tensor>& positions,
+                                  at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots, bool interleaved) {
+  const at::Tensor angles = or_none(table);
+  no_gradient("gptq::rotary_append", {&q, &k, &v, &angles, &k_cache, &v_cache});
+  static const auto op = typed_op<decltype(rotary_append)>("gptq::rotary_append");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, table, positions, std::move(k_cache), std::move(v_cache), slots, interleaved);
+}
+
+at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                    const at::Tensor& block_table, const at::Tensor& context,
+                                    const std::optional<at::Tensor>& cu_q, double scale, int64_t max_context) {
+  no_gradient("gptq::paged_attention", {&q, &k_cache, &v_cache});
+  static const auto op = typed_op<decltype(paged_attention)>("gptq::paged_attention");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k_cache, v_cache, block_table, context, cu_q, scale, max_context);
 }
 
 }  // namespace
@@ -424,4 +459,9 @@ TORCH_LIBRARY_IMPL(gptq, CUDA, m) {
 TORCH_LIBRARY_IMPL(gptq, Autograd, m) {
   m.impl("attention", attention_autograd);
   m.impl("rotary", rotary_autograd);
+  m.impl("rotary_append", rotary_append_autograd);
+  m.impl("paged_attention", paged_attention_autograd);
+  // (parts of attention's own derivative)
+  m.impl("attention_forward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("attention_backward", torch::autograd::autogradNotImplementedFallback());
 }
