@@ -393,6 +393,7 @@ struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
 std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& table,
                                                    const at::Tensor& positions, bool interleaved, bool inverse) {
   no_tangents("gptq::rotary", {&q, &k, &table});
+  TORCH_CHECK(!follows({&table}), "gptq::rotary: the table gets no gradient: detach it");
   if (follows({&q, &k})) {
     const variable_list out = RotaryGrad::apply(q, k, table, positions, interleaved, inverse);
     return {out[0], out[1]};

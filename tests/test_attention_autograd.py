@@ -132,3 +132,20 @@ def test_forward_over_reverse_raises(stand_ins):
             y = f(x)
             with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
                 torch.autograd.grad(y, x, fw.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+def test_a_table_that_requires_a_gradient_raises(stand_ins):
+    """It would get none: the tables are constants."""
+    q, k, v = heads()
+    table, pos = table_and_positions()
+    table.requires_grad_(True)
+    cache = torch.zeros(2, 4, Hk, D)
+    for x in (q, q.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="table"):
+            A.rotary(x, k, table, pos)
+    with pytest.raises(RuntimeError, match="gradient"):
+        A.rotary_append(q, k, v, table, pos, cache, cache.clone(), pos)
+    with torch.no_grad():
+        want = A.rotary(q, k, table, pos)
+        A.rotary_append(q, k, v, table, pos, cache, cache.clone(), pos)
+    assert torch.equal(A.rotary(q, k, table.detach(), pos)[0], want[0])
