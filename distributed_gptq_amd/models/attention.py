@@ -279,6 +279,14 @@ class QuantizedAttention(nn.Module):
         self.interleaved, self.scale = interleaved, scale
         self.register_buffer("table", table, persistent=False)
 
+    def _apply(self, fn, recurse=True):
+        # a cast of the module's dtype leaves the angles in 32 bits
+        table = self.table
+        super()._apply(fn, recurse)
+        if table is not None and table.dtype == torch.float32 and self.table.dtype != torch.float32:
+            self.table = table.to(self.table.device)
+        return self
+
     def _heads(self, x: torch.Tensor):
         q, k, v = self.qkv(x)
         d = self.head_dim

@@ -1,0 +1,34 @@
+"""QuantizedAttention and its cache: what they do on the host.  No GPU."""
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from distributed_gptq_amd.models import attention as A
+
+
+def module(table=None):
+    return A.QuantizedAttention(nn.Linear(8, 8), nn.Linear(8, 8), 4, 2, 8, table)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.half(), lambda m: m.bfloat16(), lambda m: m.to(torch.bfloat16),
+                                  lambda m: m.double(), lambda m: m.half().float()])
+def test_casts_leave_the_table(cast):
+    """The rotary table stays float32, bit for bit, when the module or one that
+    holds it is cast; it is found among the module's buffers and follows its
+    device."""
+    table = A.rotary_table(8, 100, device="cpu")
+    for wrap in (lambda m: m, lambda m: nn.Sequential(nn.Linear(8, 8), m)):
+        m = wrap(module(table.clone()))
+        m = copy.deepcopy(cast(m))
+        inner = m if isinstance(m, A.QuantizedAttention) else m[1]
+        assert inner.table.dtype == torch.float32 and torch.equal(inner.table, table)
+        assert any(b is inner.table for b in m.buffers())
+    assert cast(module()).table is None
+    assert cast(module(table)).qkv.weight.dtype == cast(nn.Linear(8, 8)).weight.dtype
+
+
+def test_device_moves_take_the_table():
+    m = module(A.rotary_table(8, 100, device="cpu")).to("meta", torch.float16)
+    assert m.table.is_meta and m.table.dtype == torch.float32 and m.qkv.weight.dtype == torch.float16
