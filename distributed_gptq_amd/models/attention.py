@@ -85,7 +85,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
             raise ValueError("ntk scaling needs rotary_dim >= 4")
         base = base * factor ** (rotary_dim / (rotary_dim - 2))
     inv = float(base) ** (-i / rotary_dim)
-    if kind in (None, "ntk"):
+    if not scaling or kind == "ntk":
         return inv, 1.0
     if kind == "linear":
         return inv / factor, 1.0

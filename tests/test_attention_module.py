@@ -32,3 +32,19 @@ def test_casts_leave_the_table(cast):
 def test_device_moves_take_the_table():
     m = module(A.rotary_table(8, 100, device="cpu")).to("meta", torch.float16)
     assert m.table.is_meta and m.table.dtype == torch.float32 and m.qkv.weight.dtype == torch.float16
+
+
+@pytest.mark.parametrize("scaling", [{"factor": 4.0}, {"rope_type": "linear", "factor": 4.0},
+                                     {"type": None, "factor": 4.0}])
+def test_scaling_without_a_type_raises(scaling):
+    """It was taken for no scaling at all."""
+    with pytest.raises(ValueError, match="scaling"):
+        A.rotary_frequencies(8, 1e4, scaling)
+    with pytest.raises(ValueError, match="scaling"):
+        A.rotary_table(8, 4, scaling=scaling, device="cpu")
+
+
+def test_no_scaling():
+    want = A.rotary_frequencies(8, 1e4)[0]
+    for scaling in (None, {}):
+        assert torch.equal(A.rotary_frequencies(8, 1e4, scaling)[0], want)
