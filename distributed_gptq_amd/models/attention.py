@@ -120,7 +120,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: tor
     """q (T, heads, head_dim) and k (T, kv_heads, head_dim), fp32, fp16 or
     bf16, with the first 2 * table.shape[2] channels of each head turned by the
     angles of ``positions`` (T): pairs (i, i + half), or with ``interleaved``
-    (2i, 2i + 1).  ``table`` is ``rotary_table``'s."""
+    (2i, 2i + 1).  ``table`` is ``rotary_table``'s; positions outside it are
+    turned by the angles of its ends."""
     return _op("rotary", q, k, table, positions, interleaved, False)
 
 
@@ -131,7 +132,8 @@ def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Opti
     the turned queries and writes the turned keys and the values of token t into
     place ``slots[t]`` (page * page_size + row) of the cache.  Tokens with a
     negative slot (padding) are not written.  ``table`` None: positions are not
-    rotary, nothing is turned.  For serving: no gradient is recorded."""
+    rotary, nothing is turned; positions outside it are turned by the angles of
+    its ends.  For serving: no gradient is recorded."""
     if _needs_grad(q, k, v):
         raise RuntimeError("rotary_append records no gradient: call it under torch.no_grad()")
     return _op("rotary_append", q, k, v, table, positions, k_cache, v_cache, slots, interleaved)
@@ -267,7 +269,11 @@ class QuantizedAttention(nn.Module):
     positions are not rotary.
 
     ``forward`` runs whole packed sequences, for prompts, calibration and
-    training; ``step`` runs new tokens over a ``PagedKVCache``."""
+    training; ``step`` runs new tokens over a ``PagedKVCache``.  Both raise
+    ValueError where the host knows that a position is past the table: one
+    sequence longer than it, a step whose longest context is.  Sequences by
+    ``cu_seqlens`` and given positions are not looked at; positions past the
+    table are turned by its last angles."""
 
     def __init__(self, qkv: nn.Module, o: nn.Module, heads: int, kv_heads: int, head_dim: int,
                  table: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None):
@@ -287,6 +293,10 @@ class QuantizedAttention(nn.Module):
             self.table = table.to(self.table.device)
         return self
 
+    def _check_length(self, n: int) -> None:
+        if self.table is not None and n > self.table.shape[0]:
+            raise ValueError(f"a sequence of {n} tokens: the rotary table has {self.table.shape[0]} positions")
+
     def _heads(self, x: torch.Tensor):
         q, k, v = self.qkv(x)
         d = self.head_dim
@@ -296,6 +306,8 @@ class QuantizedAttention(nn.Module):
     def forward(self, x: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """x (T, hidden): packed sequences (None: one), causal."""
+        if cu_seqlens is None and positions is None:
+            self._check_length(x.shape[0])
         q, k, v = self._heads(x)
         if self.table is not None:
             if positions is None:
@@ -309,6 +321,7 @@ class QuantizedAttention(nn.Module):
     def step(self, x: torch.Tensor, cache: PagedKVCache, batch: PagedBatch, layer: int = 0) -> torch.Tensor:
         """x (T, hidden): the batch's new tokens (``cache.extend``), whose keys
         and values are stored on the way."""
+        self._check_length(batch.max_context)
         q, k, v = self._heads(x)
         kc, vc = cache.k[layer], cache.v[layer]
         q = rotary_append(q, k, v, self.table, batch.positions, kc, vc, batch.slots, self.interleaved)

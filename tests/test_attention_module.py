@@ -48,3 +48,37 @@ def test_no_scaling():
     want = A.rotary_frequencies(8, 1e4)[0]
     for scaling in (None, {}):
         assert torch.equal(A.rotary_frequencies(8, 1e4, scaling)[0], want)
+
+
+def test_positions_past_the_table_raise(monkeypatch):
+    """Where the host knows them: a step's longest context, one sequence's
+    length.  (They would all be turned by the table's last angles.)"""
+    called = []
+
+    def op(name, *args):
+        called.append(name)
+        return torch.zeros(args[0].shape[0], 4, 8) if name != "rotary" else args[:2]
+    monkeypatch.setattr(A, "_op", op)
+
+    class Heads(nn.Module):
+        def forward(self, x):
+            return x.new_zeros(len(x), 32), x.new_zeros(len(x), 16), x.new_zeros(len(x), 16)
+    for table, most in ((A.rotary_table(8, 20, device="cpu"), 20), (None, 1 << 30)):
+        m = A.QuantizedAttention(Heads(), nn.Identity(), 4, 2, 8, table)
+        cache = A.PagedKVCache(8, 8, 2, 8, device="cpu")
+        for new, total in ((15, 15), (5, 20), (1, 21)):
+            batch = cache.extend(["a"], [new])
+            if total > most:
+                called.clear()
+                with pytest.raises(ValueError, match="20"):
+                    m.step(torch.zeros(new, 8), cache, batch)
+                assert not called
+            else:
+                assert m.step(torch.zeros(new, 8), cache, batch).shape == (new, 32)
+        assert m(torch.zeros(20, 8)).shape == (20, 32)
+        if table is not None:
+            with pytest.raises(ValueError, match="20"):
+                m(torch.zeros(21, 8))
+        # offsets or positions of the caller's are on the GPU: the operator clamps
+        assert m(torch.zeros(21, 8), positions=torch.zeros(21, dtype=torch.int32)).shape == (21, 32)
+        assert m(torch.zeros(21, 8), torch.tensor([0, 11, 21])).shape == (21, 32)
