@@ -87,12 +87,17 @@ at::Tensor linear_rows(const at::Tensor& x, const at::Tensor& qweight, const at:
 
 gptq_stream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-// t with contiguous, 16-byte aligned rows of whole 8s of values, as the kernels
-// read them; t itself wherever it is so already (a part of a fused projection)
-at::Tensor aligned_rows(const at::Tensor& t) {
+// whether t has contiguous, 16-byte aligned rows of whole 8s of values, as the
+// kernels read them
+bool rows_aligned(const at::Tensor& t) {
   bool ok = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.stride(i) % 8 == 0 || t.size(i) <= 1);
-  if (ok) return t;
+  return ok;
+}
+// t with such rows: itself wherever it has them already (a part of a fused
+// projection)
+at::Tensor aligned_rows(const at::Tensor& t) {
+  if (rows_aligned(t)) return t;
   const at::Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
 }
@@ -211,7 +216,7 @@ at::Tensor paged_attention(const at::Tensor& q_, const at::Tensor& k_cache, cons
   const c10::DeviceGuard guard(q_.device());
   const at::Tensor q = aligned_rows(q_);
   // (a cache is never copied)
-  TORCH_CHECK_VALUE(aligned_rows(k_cache).is_same(k_cache) && aligned_rows(v_cache).is_same(v_cache),
+  TORCH_CHECK_VALUE(rows_aligned(k_cache) && rows_aligned(v_cache),
                     "gptq::paged_attention: the cache's heads have to be contiguous and 16-byte aligned");
   at::Tensor out = at::empty({T, H, D}, q.options());
   if (T == 0) return out;

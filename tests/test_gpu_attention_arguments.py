@@ -50,3 +50,15 @@ def test_lengths_pages_and_offsets_beyond_32_bits_are_clamped():
     assert not m.paged_attention(q, kc, vc, long(0, 1, 2, 3, 4, 5).view(2, 3), long(5 - FAR, -FAR)).any()
     q, k, v = rand(20, 4, 64), rand(20, 2, 64, seed=1), rand(20, 2, 64, seed=2)
     assert torch.equal(m.attention(q, k, v, long(0, 9, FAR + 12)), m.attention(q, k, v, long(0, 9, 20)))
+
+
+def test_a_refused_cache_is_not_copied():
+    m = A()
+    q = rand(1, 4, 64)
+    kc = torch.zeros(512, 64, 64, 2, device="cuda", dtype=torch.float16).transpose(2, 3)  # heads that are not contiguous
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="cache"):
+        m.paged_attention(q, kc, kc, torch.zeros(1, 4, dtype=torch.int32, device="cuda"), long(5))
+    assert torch.cuda.max_memory_allocated() - before < kc.numel()
