@@ -94,10 +94,10 @@ bool rows_aligned(const at::Tensor& t) {
   for (int64_t i = 0; i + 1 < t.dim(); ++i) ok = ok && (t.stride(i) % 8 == 0 || t.size(i) <= 1);
   return ok;
 }
-// t with such rows: itself wherever it has them already (a part of a fused
-// projection)
+// t (tokens, heads, values) with such rows, tokens below 2^28 values apart:
+// itself wherever it has them already (a part of a fused projection)
 at::Tensor aligned_rows(const at::Tensor& t) {
-  if (rows_aligned(t)) return t;
+  if (rows_aligned(t) && (t.size(0) <= 1 || t.stride(0) < (int64_t{1} << 28))) return t;
   const at::Tensor c = t.contiguous();
   return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
 }

@@ -62,3 +62,34 @@ def test_a_refused_cache_is_not_copied():
     with pytest.raises(ValueError, match="cache"):
         m.paged_attention(q, kc, kc, torch.zeros(1, 4, dtype=torch.int32, device="cuda"), long(5))
     assert torch.cuda.max_memory_allocated() - before < kc.numel()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_tokens_2_to_the_28_values_apart_are_copied(dtype):
+    """As other layouts that the kernels do not read: the same bits as from
+    contiguous tensors; a cache is refused."""
+    m = A()
+    far = 2 ** 28
+    room = torch.empty(2 * far + 4096, device="cuda", dtype=dtype)
+
+    def spread(x, at):
+        y = room.as_strided(x.shape, (far, x.shape[2], 1), at)
+        return y.copy_(x)
+    x = [rand(3, n, 64, seed=i, dtype=dtype) for i, n in enumerate((4, 2, 2, 4))]
+    far_x = [spread(t, 512 * i) for i, t in enumerate(x)]
+
+    def run(q, k, v, g):
+        q, k, v = (t.detach().requires_grad_(True) for t in (q, k, v))
+        out = m.attention(q, k, v)
+        return [out.detach(), *torch.autograd.grad(out, (q, k, v), g)]
+    want = run(*x)
+    assert all(torch.equal(a, b) for a, b in zip(run(*far_x), want))
+    for i in range(4):  # each of them alone
+        assert all(torch.equal(a, b) for a, b in zip(run(*x[:i], far_x[i], *x[i + 1:]), want))
+    kc, vc = x[1][None], x[2][None]
+    table, context = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), long(3)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    assert torch.equal(m.paged_attention(far_x[0], kc, vc, table, context, cu),
+                       m.paged_attention(x[0], kc, vc, table, context, cu))
+    with pytest.raises(ValueError):
+        m.paged_attention(x[0], far_x[1][None], vc, table, context, cu)
