@@ -1,7 +1,9 @@
 """The attention calls' host-side plans, workspace queries and argument checks
 at zero, the smallest and the largest sizes, under AddressSanitizer and
 UndefinedBehaviorSanitizer (tests/host/attention_plan_check.cpp, CPU only), and
-the same queries of the shipped library."""
+the same queries of the shipped library; the kernels' index arithmetic with
+whatever the device arrays may hold, likewise
+(tests/host/attention_index_check.cpp)."""
 import os
 import shutil
 import subprocess
@@ -39,3 +41,14 @@ def test_the_shipped_library_agrees(checked):
         call, value = line.split(" = ")
         name, *args = call.split()
         assert getattr(lib, name)(*[int(a) for a in args]) == int(value), line
+
+
+def test_index_arithmetic(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    exe = str(tmp_path / "attention_index_check")
+    subprocess.run([gxx, "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all",
+                    os.path.join(ROOT, "tests", "host", "attention_index_check.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and " 0 check(s) failed" in r.stderr, r.stderr[-2000:]
