@@ -147,11 +147,18 @@ __device__ __forceinline__ void store_stats(const AttnArgs& a, float m, float l,
 // are not finite.  A product of tiles multiplies the zero weights of keys that
 // a row does not see with their values, and zero times an infinity is no term
 // of the sum.  The wave works together: a lane has a key's score, then channels
-// lane and lane + 64.  m, l: the row's statistics (l over [k0, k1) too).
+// lane and lane + 64.  m, l: the row's statistics (l over [k0, k1) too), which
+// thread `src` of the wave has stored if this is a part.
+//
+// The weights are multiplied by 2^-e, which leaves a sum of at most 1: sums of
+// bf16's largest values, which end at fp32's end, pass it with the tiles'
+// weights of up to 2^kSlack, but not here.
 template <bool kBF16, bool kPaged>
 __device__ __forceinline__ void redo_row(const AttnArgs& a, Seq s, int hk, const uint16_t* q, int64_t row, int k0, int k1,
-                                      float m, float l, int split) {
+                                      float m, float l, int split, int src) {
   const int lane = threadIdx.x & 63;
+  const int e = l > 0.0f ? ilogbf(l) + 1 : 0;
+  l = ldexpf(l, -e);
   float o[2] = {0.0f, 0.0f};
   for (int base = k0; base < k1; base += 64) {
     const int key = base + lane;
@@ -160,7 +167,7 @@ __device__ __forceinline__ void redo_row(const AttnArgs& a, Seq s, int hk, const
       const uint16_t* k = kv_row<kPaged>(a.k, a.paged.k_page, hk, kv_at<kPaged>(a, s, key));
       float dot = 0.0f;
       for (int d = 0; d < a.D; ++d) dot = fmaf(value16<kBF16>(q[d]), value16<kBF16>(k[d]), dot);
-      w = exp2f(fmaf(dot, a.c, -m));
+      w = ldexpf(exp2f(fmaf(dot, a.c, -m)), -e);
     }
     const int n = k1 - base < 64 ? k1 - base : 64;
     for (int t = 0; t < n; ++t) {
@@ -171,6 +178,7 @@ __device__ __forceinline__ void redo_row(const AttnArgs& a, Seq s, int hk, const
         if (lane + 64 * x < a.D) o[x] = fmaf(wt, value16<kBF16>(v[lane + 64 * x]), o[x]);
     }
   }
+  if (a.splits > 1 && lane == src) store_stats(a, m + e, l, row, false, split);
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     const int d = lane + 64 * x;
@@ -326,7 +334,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
     const int tk = __shfl(tok, src), hd = __shfl(head, src);
     redo_row<kBF16, kPaged>(a, s, hk, a.q.p + (s.q0 + tk) * a.q.st + hd * a.q.sh,
                             static_cast<int64_t>(s.q0 + tk) * a.H + hd, k0, __shfl(k1, src), __shfl(col.m, src),
-                            __shfl(l, src), split);
+                            __shfl(l, src), split, src);
   }
 }
 
@@ -482,7 +490,7 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
       const int tk = __shfl(tok, src), hd = __shfl(head, src);
       redo_row<kBF16, true>(a, s, hk, a.q.p + (s.q0 + tk) * a.q.st + hd * a.q.sh,
                               static_cast<int64_t>(s.q0 + tk) * a.H + hd, k0, __shfl(k1, src), __shfl(m, src),
-                              __shfl(l, src), split);
+                              __shfl(l, src), split, src);
     }
   }
 }
@@ -493,6 +501,9 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
 // 32 lanes, 4 channels a lane, takes every kGroups-th split of a row, and the
 // groups of a row are joined through LDS.  With one group for 128 splits the
 // loads of a row waited for each other: 27 us, now 3.2 for 32 rows of 64 splits.
+// All weights are 2^-kJoinRoom of that: up to 128 sums that end at fp32's end do
+// not pass it together.
+constexpr float kJoinRoom = 8.0f;
 template <bool kBF16, int kGroups>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
   __shared__ float sm[8], sl[8];
@@ -529,7 +540,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     for (int e = 0; e < 4; ++e) o[e] *= keep;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float w = __builtin_amdgcn_exp2f(ms[i] - m0);  // 0 without keys
+      const float w = __builtin_amdgcn_exp2f(ms[i] - m0 - kJoinRoom);  // 0 without keys
       l = fmaf(w, ls[i], l);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[i][e], o[e]);
