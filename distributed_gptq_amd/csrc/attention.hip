@@ -91,8 +91,9 @@ __device__ __forceinline__ void load_query(u32x4 (&q)[DT / 16], const uint16_t* 
   }
 }
 
-// Writes a column's result: the output (and lse), or this split's sums.
-template <bool kBF16, int DT, bool kTrain>
+// Writes a column's result: the output (and lse), or this split's sums.  kExact:
+// of sums that may hold infinities (whose rounding leaves nothing).
+template <bool kBF16, int DT, bool kTrain, bool kExact>
 __device__ __forceinline__ void store_column(const AttnArgs& a, const Column<DT>& col, float l, int64_t row, bool none,
                                              int split, int half) {
   if (a.splits > 1) {
@@ -124,10 +125,20 @@ __device__ __forceinline__ void store_column(const AttnArgs& a, const Column<DT>
       *reinterpret_cast<u32x2*>(out + d) = w;
       if constexpr (kTrain) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] -= value16<kBF16>(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
+        for (int e = 0; e < 4; ++e) {
+          const float rest = y[e] - value16<kBF16>(static_cast<uint16_t>(w[e / 2] >> (16 * (e % 2))));
+          y[e] = !kExact || fabsf(y[e]) < INFINITY ? rest : 0.0f;
+        }
         *reinterpret_cast<u32x2*>(a.out_rest + row * a.D + d) = u32x2{pack16<kBF16>(y[0], y[1]), pack16<kBF16>(y[2], y[3])};
       }
     }
+}
+
+// The e of a sum of weights l that 2^-e brings to [1/2, 1) in bf16 (see
+// exact_columns; fp16's values are far from fp32's end).
+template <bool kBF16>
+__device__ __forceinline__ int down_bits(float l) {
+  return kBF16 && l > 0.0f ? ilogbf(l) + 1 : 0;
 }
 
 // The row's statistics: lse, or this split's maximum and sum.  A row that sees
@@ -143,57 +154,43 @@ __device__ __forceinline__ void store_stats(const AttnArgs& a, float m, float l,
   }
 }
 
-// A row again, one key at a time and only those that it sees: for results that
-// are not finite.  A product of tiles multiplies the zero weights of keys that
-// a row does not see with their values, and zero times an infinity is no term
-// of the sum.  The wave works together: a lane has a key's score, then channels
-// lane and lane + 64.  m, l: the row's statistics (l over [k0, k1) too), which
-// thread `src` of the wave has stored if this is a part.
+// The columns again where the sums are not finite, by one wave, col.m and l of
+// all the keys known: tiles of 32 keys t0, t0 + step, ... below t1 through `room`
+// in LDS (two tiles), their values added row by row.  Slower than the products
+// of tiles by the vector instructions: 64 for a row of 128 values instead of 4
+// MFMAs for 32 of them.
 //
-// The weights are multiplied by 2^-e, which leaves a sum of at most 1: sums of
-// bf16's largest values, which end at fp32's end, pass it with the tiles'
-// weights of up to 2^kSlack, but not here.
-template <bool kBF16, bool kPaged>
-__device__ __forceinline__ void redo_row(const AttnArgs& a, Seq s, int hk, const uint16_t* q, int64_t row, int k0, int k1,
-                                      float m, float l, int split, int src) {
-  const int lane = threadIdx.x & 63;
-  const int e = l > 0.0f ? ilogbf(l) + 1 : 0;
-  l = ldexpf(l, -e);
-  float o[2] = {0.0f, 0.0f};
-  for (int base = k0; base < k1; base += 64) {
-    const int key = base + lane;
-    float w = 0.0f;
-    if (key < k1) {
-      const uint16_t* k = kv_row<kPaged>(a.k, a.paged.k_page, hk, kv_at<kPaged>(a, s, key));
-      float dot = 0.0f;
-      for (int d = 0; d < a.D; ++d) dot = fmaf(value16<kBF16>(q[d]), value16<kBF16>(k[d]), dot);
-      w = ldexpf(exp2f(fmaf(dot, a.c, -m)), -e);
-    }
-    const int n = k1 - base < 64 ? k1 - base : 64;
-    for (int t = 0; t < n; ++t) {
-      const float wt = __shfl(w, t);
-      const uint16_t* v = kv_row<kPaged>(a.v, a.paged.v_page, hk, kv_at<kPaged>(a, s, base + t));
+// A key that is seen has a weight, however small, so that an infinite value of
+// it gives an infinity.  `down` (bf16) brings the sum of weights to at most 1:
+// sums of bf16's largest values, which end at fp32's end, pass it with weights of
+// up to 2^kSlack.
+template <bool kBF16, int DT, bool kPaged>
+__device__ __forceinline__ void exact_columns(Column<DT>& col, const AttnArgs& a, const Seq& s, int hk,
+                                              const u32x4 (&q)[DT / 16], float down, int limit, int t0, int t1, int step,
+                                              uint8_t* room, int lane) {
+  uint8_t* vroom = room + 32 * DT * 2;
+  const lds_u8 *kt = (const lds_u8*)room, *vt = (const lds_u8*)vroom;
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (lane + 64 * x < a.D) o[x] = fmaf(wt, value16<kBF16>(v[lane + 64 * x]), o[x]);
-    }
-  }
-  if (a.splits > 1 && lane == src) store_stats(a, m + e, l, row, false, split);
+  for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
+#pragma unroll 1
+  for (int t = t0; t < t1; t += step) {
+    const int key0 = 32 * t;
+    fetch_rows<DT, 32, kPaged>(a, s, hk, kv_at_clamped<kPaged>(a, s, key0 + (lane & 31)), key0, 0, room, vroom, lane);
+    landed();
+    f32x16 w = zero16();
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    const int d = lane + 64 * x;
-    if (d >= a.D) continue;
-    if (a.splits > 1) {
-      a.part[(split * (static_cast<int64_t>(a.T) * a.H) + row) * a.D + d] = o[x];
-    } else {
-      const float y = o[x] / l;
-      const uint16_t w = kBF16 ? f32_to_bf16_bits(y) : f32_to_f16_bits(y);
-      a.out[row * a.D + d] = w;
-      if (a.out_rest) {
-        const float rest = fabsf(y) < INFINITY ? y - value16<kBF16>(w) : 0.0f;
-        a.out_rest[row * a.D + d] = kBF16 ? f32_to_bf16_bits(rest) : f32_to_f16_bits(rest);
-      }
+    for (int d = 0; d < DT / 16; ++d) w = mma32<kBF16>(row_operand<DT>(kt, 0, d, where), q[d], w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float x = __builtin_amdgcn_exp2f(fmaf(w[i], a.c, -col.m)) * down;
+      w[i] = x < 0x1p-126f && w[i] > -INFINITY ? 0x1p-126f : x;
     }
+    wave_sync();
+    store_weights((lds_f32*)room, w, lane);  // (the keys are done with)
+    landed();
+    add_seen_rows<kBF16, DT>(col.o, (const lds_f32*)room, vt, lane, [&](int r) { return key0 + r <= limit; });
+    landed();
   }
 }
 
@@ -322,19 +319,23 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(AttnArgs a, int slots
   const float l = half_sum(col.l);
   const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
   const bool fine = finite_column(col);
-  const bool bad = inside && !none && half_sum(fine ? 0.0f : 1.0f) != 0.0f;
-  if (inside) {
-    if (!bad) store_column<kBF16, DT, kTrain>(a, col, l, row, none, split, half);
+  // (a NaN among the weights, whose sum then is one, makes all of the row one)
+  const bool bad = inside && !none && l == l && half_sum(fine ? 0.0f : 1.0f) != 0.0f;
+  if (inside && !bad) {
+    store_column<kBF16, DT, kTrain, false>(a, col, l, row, none, split, half);
     if (half == 0) store_stats(a, col.m, l, row, none, split);
   }
-  uint64_t todo = __ballot(bad && half == 0);
-  while (todo) {
-    const int src = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    const int tk = __shfl(tok, src), hd = __shfl(head, src);
-    redo_row<kBF16, kPaged>(a, s, hk, a.q.p + (s.q0 + tk) * a.q.st + hd * a.q.sh,
-                            static_cast<int64_t>(s.q0 + tk) * a.H + hd, k0, __shfl(k1, src), __shfl(col.m, src),
-                            __shfl(l, src), split, src);
+  if (__builtin_expect(__ballot(bad) != 0, 0)) {
+    const int e = down_bits<kBF16>(l);
+    uint8_t* const room = wave == 0 ? g_rows_k0<DT> : wave == 1 ? g_rows_k1<DT> : wave == 2 ? g_rows_v0<DT> : g_rows_v1<DT>;
+    const int last_tile = (wave_end + 31) / 32;
+    exact_columns<kBF16, DT, kPaged>(col, a, s, hk, q, exp2f(static_cast<float>(-e)), limit, 2 * t0,
+                                     2 * t1 < last_tile ? 2 * t1 : last_tile, 1, room, late_lane());
+    if (bad) {
+      const float le = ldexpf(l, -e);
+      store_column<kBF16, DT, kTrain, true>(a, col, le, row, none, split, half);
+      if (half == 0) store_stats(a, col.m + e, le, row, none, split);
+    }
   }
 }
 
@@ -412,11 +413,6 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
   };
   // one wave's copies are only its own: they have to have landed before its
   // reads, and its reads of a buffer to be done before the next copies into it
-  auto landed = [&]() {
-    wait_vm<0>();
-    wait_lgkm<0>();
-    wave_sync();
-  };
   for (int t = t0 + wave; t < t1; t += 4) {
     fetch(t, &g_few<DT>[wave][0][0], &g_few<DT>[wave][1][0]);
     landed();
@@ -439,11 +435,13 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
 #pragma unroll
   for (int w = 0; w < 4; ++w) l += stats[1][w][c] * exp2f(stats[0][w][c] - m);
   lds_f32* sums = (lds_f32*)&g_few<DT>[0][0][0];
-  const float scale = exp2f(col.m - m);
+  auto give = [&](float scale) {
 #pragma unroll
-  for (int db = 0; db < DT / 32; ++db)
+    for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sums[(wave * DT + 32 * db + acc_row(i, half)) * 32 + c] = col.o[db][i] * scale;
+      for (int i = 0; i < 16; ++i) sums[(wave * DT + 32 * db + acc_row(i, half)) * 32 + c] = col.o[db][i] * scale;
+  };
+  give(exp2f(col.m - m));
   __syncthreads();
 
   const int k0 = t0 * kFew;
@@ -453,16 +451,18 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
   constexpr int N = DT / 8;  // channels of a thread
   const int d0 = (threadIdx.x >> 5) * N;
   float o[N];
-  bool fine = true;
+  auto take = [&]() {
+    bool fine = true;
 #pragma unroll
-  for (int x = 0; x < N; ++x) {
-    o[x] = 0.0f;
+    for (int x = 0; x < N; ++x) {
+      o[x] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) o[x] += sums[(w * DT + d0 + x) * 32 + c];
-    fine = fine && fabsf(o[x]) < INFINITY;
-  }
-  if (inside) {
-    if (!none && !fine) redo[c] = 1;
+      for (int w = 0; w < 4; ++w) o[x] += sums[(w * DT + d0 + x) * 32 + c];
+      fine = fine && fabsf(o[x]) < INFINITY;
+    }
+    return fine;
+  };
+  auto store = [&](float m, float l) {
     if (threadIdx.x < R) store_stats(a, m, l, row, none, split);
     if (a.splits > 1) {
       float* part = a.part + (split * (static_cast<int64_t>(a.T) * a.H) + row) * a.D;
@@ -480,19 +480,21 @@ __global__ __launch_bounds__(256, 2) void attn_few_kernel(AttnArgs a, int slots)
               none ? u32x2{0, 0}
                    : u32x2{pack16<kBF16>(o[x] * rl, o[x + 1] * rl), pack16<kBF16>(o[x + 2] * rl, o[x + 3] * rl)};
     }
-  }
+  };
+  // (a NaN among the weights, whose sum then is one, makes all of the row one)
+  if (!take() && inside && !none && l == l) redo[c] = 1;
+  if (inside) store(m, l);
   __syncthreads();
-  if (wave == 0) {
-    uint64_t todo = __ballot(half == 0 && inside && redo[c] != 0);
-    while (todo) {
-      const int src = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      const int tk = __shfl(tok, src), hd = __shfl(head, src);
-      redo_row<kBF16, true>(a, s, hk, a.q.p + (s.q0 + tk) * a.q.st + hd * a.q.sh,
-                              static_cast<int64_t>(s.q0 + tk) * a.H + hd, k0, __shfl(k1, src), __shfl(m, src),
-                              __shfl(l, src), split, src);
-    }
-  }
+  if (__builtin_expect(__ballot(redo[c] != 0) == 0, 1)) return;  // (the same in all waves)
+  const int e = down_bits<kBF16>(l);
+  col.m = m;
+  exact_columns<kBF16, DT, true>(col, a, s, hk, q, exp2f(static_cast<float>(-e)), limit, t0 + wave, t1, 4,
+                                 &g_few<DT>[wave][0][0], late_lane());
+  __syncthreads();
+  give(1.0f);
+  __syncthreads();
+  take();
+  if (inside && redo[c] != 0) store(m + e, ldexpf(l, -e));
 }
 
 // ----------------------------------------------------------------- joining ----

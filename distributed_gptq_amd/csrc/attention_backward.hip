@@ -142,10 +142,6 @@ __shared__ __attribute__((aligned(1024))) uint8_t g_back_b0[kRows * DT * 2];
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_back_b1[kRows * DT * 2];
 
-template <bool kBF16>
-__device__ __forceinline__ uint16_t round16(float x) {
-  return kBF16 ? f32_to_bf16_bits(x) : f32_to_f16_bits(x);
-}
 template <int DT>
 __device__ __forceinline__ bool all_finite(const f32x16 (&x)[DT / 32]) {
   float worst = 0.0f;
@@ -156,42 +152,43 @@ __device__ __forceinline__ bool all_finite(const f32x16 (&x)[DT / 32]) {
   return worst == 0.0f;
 }
 
-// A row's dq again over the keys up to `limit`, which it sees: where the product
-// of tiles is not finite, which multiplies the zero ds of other keys with those
-// keys.  A lane has a key's ds, then channels lane and lane + 64.
-template <bool kBF16>
-__device__ __forceinline__ void redo_dq(const BackArgs& args, const Seq& s, int hk, int tok, int head, int limit) {
-  const AttnArgs& a = args.f;
-  const int lane = threadIdx.x & 63;
-  const uint16_t* q = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh;
-  const uint16_t* g = args.g.p + (s.q0 + tok) * args.g.st + head * args.g.sh;
-  const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
-  float dq[2] = {0.0f, 0.0f};
-  for (int base = 0; base <= limit; base += 64) {
-    const int key = base + lane;
-    float ds = 0.0f;
-    if (key <= limit) {
-      const uint16_t* k = kv_row<false>(a.k, 0, hk, KvAt{0, s.k0 + key});
-      const uint16_t* v = kv_row<false>(a.v, 0, hk, KvAt{0, s.k0 + key});
-      float sc = 0.0f, dp = 0.0f;
-      for (int d = 0; d < a.D; ++d) {
-        sc = fmaf(value16<kBF16>(q[d]), value16<kBF16>(k[d]), sc);
-        dp = fmaf(value16<kBF16>(g[d]), value16<kBF16>(v[d]), dp);
-      }
-      ds = exp2f(fmaf(sc, a.c, -a.lse[row])) * (dp - args.delta[row]);
-    }
-    const int n = limit + 1 - base < 64 ? limit + 1 - base : 64;
-    for (int t = 0; t < n; ++t) {
-      const float w = __shfl(ds, t);
-      const uint16_t* k = kv_row<false>(a.k, 0, hk, KvAt{0, s.k0 + base + t});
+// The weight of a score that is seen, however small: an infinity that it
+// multiplies gives one.
+__device__ __forceinline__ float seen_weight(float score, float c, float lse) {
+  const float p = __builtin_amdgcn_exp2f(fmaf(score, c, -lse));
+  return p < 0x1p-126f && score > -INFINITY ? 0x1p-126f : p;
+}
+
+// A wave's columns of dq again where the product of tiles is not finite: tiles of
+// 32 keys below t1 through `room` in LDS (two tiles), the keys added row by row.
+template <bool kBF16, int DT>
+__device__ __forceinline__ void exact_dq(f32x16 (&acc)[DT / 32], const AttnArgs& a, const Seq& s, int hk,
+                                         const u32x4 (&q)[DT / 16], const u32x4 (&g)[DT / 16], float lse, float delta,
+                                         int limit, int t1, uint8_t* room, int lane) {
+  uint8_t* vroom = room + 32 * DT * 2;
+  const lds_u8 *kt = (const lds_u8*)room, *vt = (const lds_u8*)vroom;
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-        if (lane + 64 * x < a.D) dq[x] = fmaf(w, value16<kBF16>(k[lane + 64 * x]), dq[x]);
+  for (int db = 0; db < DT / 32; ++db) acc[db] = zero16();
+#pragma unroll 1
+  for (int t = 0; t < t1; ++t) {
+    const int key0 = 32 * t;
+    fetch_rows<DT, 32, false>(a, s, hk, kv_at<false>(a, s, key0 + (lane & 31)), key0, 0, room, vroom, lane);
+    landed();
+    f32x16 sc = zero16(), dp = zero16();
+#pragma unroll
+    for (int d = 0; d < DT / 16; ++d) {
+      sc = mma32<kBF16>(row_operand<DT>(kt, 0, d, where), q[d], sc);
+      dp = mma32<kBF16>(row_operand<DT>(vt, 0, d, where), g[d], dp);
     }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sc[i] = seen_weight(sc[i], a.c, lse) * (dp[i] - delta);
+    wave_sync();
+    store_weights((lds_f32*)vroom, sc, lane);  // (the values are done with)
+    landed();
+    add_seen_rows<kBF16, DT>(acc, (const lds_f32*)vroom, kt, lane, [&](int r) { return key0 + r <= limit; });
+    landed();
   }
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-    if (lane + 64 * x < a.D) args.dq[row * a.D + lane + 64 * x] = round16<kBF16>(dq[x] * args.scale);
 }
 
 // dq: as the forward pass, 32 packed rows a wave (a lane's column), tiles of 64
@@ -326,11 +323,10 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
   // (with a NaN for delta or lse all of the row is, from its own keys)
   const bool bad = inside && half_sum(fine ? 0.0f : 1.0f) != 0.0f && lse == lse && delta == delta;
   if (inside && !bad) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale * exp2f(-shift), a.D, half);
-  uint64_t todo = __ballot(bad && half == 0);
-  while (todo) {
-    const int src = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    redo_dq<kBF16>(args, s, hk, __shfl(tok, src), __shfl(head, src), __shfl(limit, src));
+  if (__builtin_expect(__ballot(bad) != 0, 0)) {
+    uint8_t* const room = wave == 0 ? g_back_a0<DT> : wave == 1 ? g_back_a1<DT> : wave == 2 ? g_back_b0<DT> : g_back_b1<DT>;
+    exact_dq<kBF16, DT>(acc, a, s, hk, q, g, lse, delta, limit, (wave_end + 31) / 32, room, late_lane());
+    if (bad) store_rows<kBF16, DT>(args.dq + row * a.D, acc, args.scale, a.D, half);
   }
 }
 
@@ -388,60 +384,63 @@ __device__ __forceinline__ u32x4 units() {
   return kBF16 ? u32x4{0x3F803F80u, 0x3F80u, 0, 0} : u32x4{0x4C007800u, 0x04002000u, 0, 0};
 }
 
-// A key's gradients again, over the rows that see it only (as redo_dq): tiles
-// [first, last) of 64 rows, a row's weight and ds in a lane, then channels lane
-// and lane + 64.
-template <bool kBF16>
-__device__ __forceinline__ void redo_dkv(const BackArgs& args, const Seq& s, int hk, int key, int t0, int nt, int first,
-                                         int last, int split) {
+// A wave's 32 keys' dv, or dk, again where the products of tiles are not finite
+// (as exact_dq): tiles first .. last - 1 of 64 query rows, 32 at a time through
+// the wave's halves of the tiles' buffers, the rows' weights in another half.
+template <bool kBF16, int DT, bool kKeyGrad>
+__device__ __forceinline__ void exact_dkv(f32x16 (&sums)[DT / 32], const BackArgs& args, const Seq& s, int hk,
+                                          const u32x4 (&kf)[DT / 16], int kw, bool bad, int t0, int nt, int first, int last,
+                                          const lds_u8* vt, uint8_t* qroom, uint8_t* groom, int lane) {
+  constexpr int CH = DT / 8, RPI = 64 / CH;
   const AttnArgs& a = args.f;
-  const int lane = threadIdx.x & 63, G = static_cast<int>(a.G.d);
-  const uint16_t* k = a.k.p + static_cast<int64_t>(s.k0 + key) * a.k.st + hk * a.k.sh;
-  const uint16_t* v = a.v.p + static_cast<int64_t>(s.k0 + key) * a.v.st + hk * a.v.sh;
-  float dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
-  for (int x = first; x < last; ++x) {
-    const int head = hk * G + x / nt, tok0 = (t0 + nt - 1 - x % nt) * kBackRows, tok = tok0 + lane;
-    const uint16_t* q = a.q.p + s.q0 * a.q.st + head * a.q.sh;
-    const uint16_t* g = args.g.p + s.q0 * args.g.st + head * args.g.sh;
-    const bool sees = tok < s.Lq && last_key(a, s, tok) >= key;
-    float p = 0.0f, ds = 0.0f;
-    if (sees) {
-      float sc = 0.0f, dp = 0.0f;
-      for (int d = 0; d < a.D; ++d) {
-        sc = fmaf(value16<kBF16>(q[tok * a.q.st + d]), value16<kBF16>(k[d]), sc);
-        dp = fmaf(value16<kBF16>(g[tok * args.g.st + d]), value16<kBF16>(v[d]), dp);
-      }
-      const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
-      p = exp2f(fmaf(sc, a.c, -a.lse[row]));
-      ds = p * (dp - args.delta[row]);
-    }
-    uint64_t todo = __ballot(sees);
-    while (todo) {
-      const int t = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      const float wp = __shfl(p, t), wd = __shfl(ds, t);
+  const int half = lane >> 5, G = static_cast<int>(a.G.d), key = kw + (lane & 31), off = s.Lk - s.Lq;
+  const lds_u8 *qt = (const lds_u8*)qroom, *gt = (const lds_u8*)groom;
+  lds_f32* weights = (lds_f32*)(qroom + 32 * DT * 2);
+  const LaneAt<DT> where = lane_at<DT>(lane, 0);
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const int d = lane + 64 * y;
-        if (d >= a.D) continue;
-        dv[y] = fmaf(wp, value16<kBF16>(g[(tok0 + t) * args.g.st + d]), dv[y]);
-        dk[y] = fmaf(wd, value16<kBF16>(q[(tok0 + t) * a.q.st + d]), dk[y]);
-      }
-    }
-  }
-  const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
-  const int64_t all = static_cast<int64_t>(a.S) * a.Hk * a.D;
+  for (int db = 0; db < DT / 32; ++db) sums[db] = zero16();
+#pragma unroll 1
+  for (int x = 2 * first; x < 2 * last; ++x) {
+    const int head = hk * G + x / 2 / nt, r0 = (t0 + nt - 1 - x / 2 % nt) * kBackRows + 32 * (x & 1);
+    if (r0 >= s.Lq || last_key(a, s, r0 + 31 < s.Lq ? r0 + 31 : s.Lq - 1) < kw) continue;
+    const uint16_t* qp = a.q.p + s.q0 * a.q.st + head * a.q.sh;
+    const uint16_t* gp = args.g.p + s.q0 * args.g.st + head * args.g.sh;
 #pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    const int d = lane + 64 * y;
-    if (d >= a.D) continue;
-    if (args.splits > 1) {
-      args.part[2 * split * all + row + d] = dk[y] * args.scale;
-      args.part[(2 * split + 1) * all + row + d] = dv[y];
-    } else {
-      args.dk[row + d] = round16<kBF16>(dk[y] * args.scale);
-      args.dv[row + d] = round16<kBF16>(dv[y]);
+    for (int y = 0; y < 32 / RPI; ++y) {
+      const int i = y * RPI + lane / CH;
+      const int64_t tok = r0 + i;
+      const int ch = (lane % CH) ^ row_slot<DT>(i);
+      const bool in = tok < s.Lq && ch * 8 < a.D;
+      copy16_to_lds(in ? static_cast<const void*>(qp + tok * a.q.st + ch * 8) : g_attn_zeros, qroom + y * 1024);
+      copy16_to_lds(in ? static_cast<const void*>(gp + tok * args.g.st + ch * 8) : g_attn_zeros, groom + y * 1024);
     }
+    const int tok = r0 + (lane & 31) < s.Lq ? r0 + (lane & 31) : s.Lq - 1;
+    const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
+    const float lse = a.lse[row], delta = args.delta[row];
+    landed();
+    f32x16 w = zero16();
+#pragma unroll
+    for (int d = 0; d < DT / 16; ++d) w = mma32<kBF16>(row_operand<DT>(qt, 0, d, where), kf[d], w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = seen_weight(w[i], a.c, __shfl(lse, acc_row(i, half)));
+    if constexpr (kKeyGrad) {
+      f32x16 dp = zero16();
+#pragma unroll
+      for (int d = 0; d < DT / 16; ++d) dp = mma32<kBF16>(row_operand<DT>(gt, 0, d, where), row_operand<DT>(vt, 0, d, where), dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] *= dp[i] - __shfl(delta, acc_row(i, half));
+    }
+    store_weights(weights, w, lane);
+    landed();
+    const int seen = a.causal ? key - off - r0 : 0, rows = s.Lq - r0;
+    add_seen_rows<kBF16, DT>(sums, weights, kKeyGrad ? qt : gt, lane, [&](int r) { return r >= seen && r < rows; });
+    landed();
+    bool open = false;
+#pragma unroll
+    for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) open = open || sums[db][i] == sums[db][i];
+    if (__ballot(bad && open) == 0) break;  // (all NaN, whatever follows)
   }
 }
 
@@ -618,32 +617,36 @@ __global__ __launch_bounds__(256, 2) void attn_dkv_kernel(BackArgs args) {
       dv[db][i] += sum_v[(16 * db + i) * 64 + lane];
     }
   const int64_t row = (static_cast<int64_t>(s.k0 + key) * a.Hk + hk) * a.D;
-  const float rk = args.scale * exp2f(-shift), rv = exp2f(kBF16 ? 0.0f : -kWeightShift);
   const bool fine = all_finite<DT>(dk) && all_finite<DT>(dv);
   const bool bad = inside && half_sum(fine ? 0.0f : 1.0f) != 0.0f;
-  uint64_t todo = __ballot(bad && half == 0);
-  while (todo) {
-    const int src = __builtin_ctzll(todo);
-    todo &= todo - 1;
-    redo_dkv<kBF16>(args, s, hk, kw + src, t0, nt, first, last, split);
-  }
-  if (!inside || bad) return;
-  if (args.splits == 1) {
-    store_rows<kBF16, DT>(args.dk + row, dk, rk, a.D, half);
-    store_rows<kBF16, DT>(args.dv + row, dv, rv, a.D, half);
-    return;
-  }
   const int64_t all = static_cast<int64_t>(a.S) * a.Hk * a.D;
   float* part = args.part + 2 * split * all + row;
-#pragma unroll
-  for (int db = 0; db < DT / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int d = 32 * db + acc_row(i, half);
-      if (d >= a.D) continue;
-      *reinterpret_cast<f32x4*>(part + d) = f32x4{dk[db][i], dk[db][i + 1], dk[db][i + 2], dk[db][i + 3]} * rk;
-      *reinterpret_cast<f32x4*>(part + all + d) = f32x4{dv[db][i], dv[db][i + 1], dv[db][i + 2], dv[db][i + 3]} * rv;
+  auto store = [&](const f32x16 (&x)[DT / 32], float* to_part, uint16_t* to, float r) {
+    if (args.splits == 1) {
+      store_rows<kBF16, DT>(to + row, x, r, a.D, half);
+      return;
     }
+#pragma unroll
+    for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * db + acc_row(i, half);
+        if (d < a.D) *reinterpret_cast<f32x4*>(to_part + d) = f32x4{x[db][i], x[db][i + 1], x[db][i + 2], x[db][i + 3]} * r;
+      }
+  };
+  if (inside && !bad) {
+    store(dk, part, args.dk, args.scale * exp2f(-shift));
+    store(dv, part + all, args.dv, exp2f(kBF16 ? 0.0f : -kWeightShift));
+  }
+  if (__builtin_expect(__ballot(bad) == 0, 1)) return;
+  // (the other wave of these keys is done, and this one with its sums)
+  landed();
+  const lds_u8* vt = (const lds_u8*)&g_dkv_v<DT>[0] + 32 * (wave & 1) * (DT * 2);
+  uint8_t *const qroom = (wave & 1) ? g_dkv_q1<DT> : g_dkv_q0<DT>, *const groom = (wave & 1) ? g_dkv_g1<DT> : g_dkv_g0<DT>;
+  exact_dkv<kBF16, DT, false>(dv, args, s, hk, kf, kw, bad, t0, nt, first, last, vt, qroom, groom, late_lane());
+  if (bad) store(dv, part + all, args.dv, 1.0f);
+  exact_dkv<kBF16, DT, true>(dk, args, s, hk, kf, kw, bad, t0, nt, first, last, vt, qroom, groom, late_lane());
+  if (bad) store(dk, part, args.dk, args.scale);
 }
 
 // The splits' sums of dk and dv, 4 values a thread.

@@ -21,6 +21,7 @@ namespace {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) float lds_f32;
@@ -154,6 +155,55 @@ __device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, in
   for (int j = 0; j < 2; ++j)
     v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + at.col[db][j] + row0 * (DT * 2)));
   return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// The lane for a path taken seldom: what follows from it is computed there, and
+// not kept in registers until then.
+__device__ __forceinline__ int late_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// One wave's own copies into LDS have landed, and its reads of LDS are done.
+__device__ __forceinline__ void landed() {
+  wait_vm<0>();
+  wait_lgkm<0>();
+  wave_sync();
+}
+
+// sums += weights x rows of a tile of 32 rows, row by row and only those that
+// the lane's column sees: a product of the tile multiplies the zero weights of
+// the others with what they hold, and zero times an infinity is no term of a
+// sum.  weights: 32 floats for each row, in LDS.
+template <bool kBF16, int DT, class Sees>
+__device__ __forceinline__ void add_seen_rows(f32x16 (&sums)[DT / 32], const lds_f32* weights, const lds_u8* tile, int lane,
+                                              Sees&& sees) {
+  const int half = lane >> 5;
+#pragma unroll 1
+  for (int r = 0; r < 32; ++r) {
+    const float w = weights[r * 32 + (lane & 31)];
+    const bool in = sees(r);
+#pragma unroll
+    for (int db = 0; db < DT / 32; ++db) {
+      __builtin_amdgcn_sched_barrier(0);  // (all values at once would take as many registers as the sums)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const u32x2 x = *(const lds_u32x2*)(tile + r * (DT * 2) + (((4 * db + j) ^ row_slot<DT>(r)) << 4) + 8 * half);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float sum = sums[db][4 * j + e];
+          const float y = fmaf(w, value16<kBF16>(static_cast<uint16_t>(x[e / 2] >> (16 * (e % 2)))), sum);
+          sums[db][4 * j + e] = in ? y : sum;
+        }
+      }
+    }
+  }
+}
+// a column's 16 values of a lane as such weights
+__device__ __forceinline__ void store_weights(lds_f32* weights, const f32x16& w, int lane) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) weights[acc_row(i, lane >> 5) * 32 + (lane & 31)] = w[i];
 }
 
 // The order of a run of N pairs of an LDS read and an MFMA (two pairs of them at

@@ -61,3 +61,92 @@ def test_values_near_the_largest_over_a_cache(new, L):
     out = A().paged_attention(q[:new], kc.view(pages, page, Hk, D), vc.view(pages, page, Hk, D), table,
                               torch.tensor([L], device="cuda"), cu)
     check(out, one(q[:new], k, v)["out"])
+
+
+def microseconds(f):
+    f()
+    times = []
+    for _ in range(5):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return sorted(times)[2]
+
+
+def step(L, H, Hk, D, dtype):
+    g = torch.Generator(device="cuda").manual_seed(5)
+    return [torch.randn(L, h, D, generator=g, device="cuda").to(dtype) for h in (H, Hk, Hk, H)]
+
+
+def train(q, k, v, grad):
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    return torch.autograd.grad(A().attention(q, k, v), (q, k, v), grad)
+
+
+def nan(x):
+    return torch.full_like(x, math.nan)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_step_of_nan_takes_no_longer(dtype):
+    """All NaN, as after an overflow: within 10 times the time of a finite step
+    (making every row again, one by one, took 200 to 500 times)."""
+    q, k, v, grad = step(2048, 16, 8, 128, dtype)
+    usual = microseconds(lambda: train(q, k, v, grad))
+    for x in ((nan(q), k, v, grad), (q, nan(k), v, grad), (nan(q), nan(k), nan(v), nan(grad)), (q, k, v, nan(grad))):
+        assert microseconds(lambda: train(*x)) <= 10 * usual
+        assert all(bool(y.isnan().all()) for y in train(*x)[:2])
+    with torch.no_grad():
+        usual = microseconds(lambda: A().attention(q, k, v))
+        assert microseconds(lambda: A().attention(nan(q), k, v)) <= 10 * usual
+        kc, vc = (x.view(128, 16, 8, 128) for x in (k, v))
+        args = (kc, vc, torch.arange(128, device="cuda", dtype=torch.int32)[None], torch.tensor([2048], device="cuda"))
+        usual = microseconds(lambda: A().paged_attention(q[:1], *args))
+        assert microseconds(lambda: A().paged_attention(nan(q[:1]), *args)) <= 10 * usual
+        assert bool(A().paged_attention(nan(q[:1]), *args).isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_infinite_values_take_bounded_time(dtype):
+    """Sums with an infinity are made again row by row: within 60 times the time
+    of a finite step (one row or key after the other took 500 times)."""
+    q, k, v, grad = step(2048, 16, 8, 128, dtype)
+    usual = microseconds(lambda: train(q, k, v, grad))
+    for i in (2, 3):
+        x = [q, k, v, grad]
+        x[i] = x[i].clone()
+        x[i][0 if i == 2 else 2047, :, 3] = math.inf
+        assert microseconds(lambda: train(*x)) <= 60 * usual
+    with torch.no_grad():
+        usual = microseconds(lambda: A().attention(q, k, v))
+        v2 = v.clone()
+        v2[0, 0, 3] = math.inf
+        assert microseconds(lambda: A().attention(q, k, v2)) <= 60 * usual
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("L,H,Hk,D", [(70, 4, 2, 64), (300, 8, 2, 128), (961, 64, 64, 40)])
+def test_gradient_of_an_infinite_gradient(L, H, Hk, D, dtype):
+    """One infinity in the last row of dL/do, channel 3 of head 1: infinities of
+    the formula's signs where sums have them as terms, NaN where two meet, every
+    other sum as without it."""
+    q, k, v, grad = step(L, H, Hk, D, dtype)
+    clean = one(q, k, v, grad)
+    head, kv = 1, 1 // (H // Hk)
+    g2 = grad.clone()
+    g2[L - 1, head, 3] = math.inf
+    dq, dk, dv = train(q, k, v, g2)
+    # (delta and g v of that row are infinite)
+    o3, v3 = clean["out"][0][L - 1, head, 3], v[:, kv, 3].double()
+    ds = torch.where(v3.sign() == o3.sign(), math.nan, v3.sign() * math.inf)
+    want = {"dq": (dq, clean["dq"][0].clone()), "dk": (dk, clean["dk"][0].clone()), "dv": (dv, clean["dv"][0].clone())}
+    want["dq"][1][L - 1, head] = math.nan
+    want["dk"][1][:, kv] = ds[:, None] * q[L - 1, head].double()
+    want["dv"][1][:, kv, 3] = math.inf
+    for name, (got, ref) in want.items():
+        fine = ref.isfinite()
+        assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.double()[ref.isinf()], ref[ref.isinf()]), name
+        check(got[fine], (ref[fine], clean[name][1][fine]))
