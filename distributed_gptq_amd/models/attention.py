@@ -200,6 +200,8 @@ class PagedKVCache:
                  dtype: torch.dtype = torch.float16, device="cuda"):
         if pages < 1 or page_size < 1 or layers < 1:
             raise ValueError(f"a cache of {layers} layers, {pages} pages of {page_size} tokens")
+        if pages * page_size > 1 << 31:
+            raise ValueError(f"{pages} pages of {page_size} tokens: a cache has at most 2^31 places, which slots can name")
         shape = (layers, pages, page_size, kv_heads, head_dim)
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)

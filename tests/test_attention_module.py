@@ -82,3 +82,11 @@ def test_positions_past_the_table_raise(monkeypatch):
         # offsets or positions of the caller's are on the GPU: the operator clamps
         assert m(torch.zeros(21, 8), positions=torch.zeros(21, dtype=torch.int32)).shape == (21, 32)
         assert m(torch.zeros(21, 8), torch.tensor([0, 11, 21])).shape == (21, 32)
+
+
+def test_a_cache_of_more_places_than_slots_count_raises():
+    """Slots are 32-bit: places from 2^31 on could not be named (extend failed
+    there, after it had given the pages away)."""
+    A.PagedKVCache(1024, 2 ** 21, 1, 8, device="meta")
+    with pytest.raises(ValueError, match="2\\^31"):
+        A.PagedKVCache(1025, 2 ** 21, 1, 8, device="meta")
