@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from distributed_gptq_amd import _lib
 from distributed_gptq_amd.models import attention as A
@@ -149,3 +150,24 @@ def test_a_table_that_requires_a_gradient_raises(stand_ins):
         want = A.rotary(q, k, table, pos)
         A.rotary_append(q, k, v, table, pos, cache, cache.clone(), pos)
     assert torch.equal(A.rotary(q, k, table.detach(), pos)[0], want[0])
+
+
+TRACES = {"make_fx": lambda f, x: make_fx(f)(*x), "jit": lambda f, x: torch.jit.trace(f, x, check_trace=False)}
+
+
+@pytest.mark.parametrize("trace,gradient", [("make_fx", False), ("make_fx", True), ("jit", False)])
+def test_traces_hold_the_operators(stand_ins, trace, gradient):
+    """A trace of rotary and attention, with the gradient too, computes other
+    inputs' results."""
+    table, pos = table_and_positions()
+
+    def step(q, k, v, g):
+        if not gradient:
+            return (A.attention(*A.rotary(q, k, table, pos), v),)
+        q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+        out = A.attention(*A.rotary(q, k, table, pos), v)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), g))
+    x = (*heads(), torch.ones(T, H, D))
+    other = [torch.flip(y, (0,)) * 0.5 for y in x]
+    for got, want in zip(TRACES[trace](step, x)(*other), step(*other)):
+        assert torch.equal(got, want)
