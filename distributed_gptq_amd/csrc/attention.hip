@@ -211,15 +211,17 @@ __device__ __forceinline__ bool finite_column(const Column<DT>& col) {
 // values pass through two LDS buffers, the next one's copies in flight while
 // one is used.
 //
-// Bound by the issue of MFMAs and vector instructions together: a tile of 64 keys
-// and 32 rows of 128 takes 32 MFMAs (1024 cycles) and about 155 vector
-// instructions, 32 of them exponentials of 16 cycles, and the two waves of a SIMD
-// overlap these to 2/3 of their sum.  Measured (us; TFLOP/s of the products that
-// the mask leaves): 8192 tokens in four prompts, 32 over 8 heads of 128, 214-221
-// (850-870); 16 x 2048 tokens, 12 heads of 64, 163-166 (630); 512 tokens over
-// 16384 cached ones, 32 over 8 heads, 159-166 (840-880).  Tiles of 32 keys with 3
-// workgroups a CU: 3% faster on the prompts, 8% slower with gradients, 50% over a
-// cache.
+// Bound by the waits between a wave's steps: its scores, maximum, exponentials
+// and weighted values of a tile follow from one another, and all waves meet at
+// every tile's barrier.  The MFMAs are busy 46% of the cycles (37% with heads of
+// 64), where the issue of the instructions alone would allow 79%: so busy are they
+// in a loop of 8 MFMAs (32 cycles each), 40 multiply-adds and 8 exponentials (8
+// cycles each), a tile's mix, that do not depend on each other, in one or two waves
+// a SIMD.  Measured (us; TFLOP/s of the products that the mask leaves): 8192 tokens
+// in four prompts, 32 over 8 heads of 128, 209-224 (840-900); 16 x 2048 tokens, 12
+// heads of 64, 158-166 (620-650); 512 tokens over 16384 cached ones, 32 over 8
+// heads, 157-170 (820-890).  Tiles of 32 keys with 3 workgroups a CU: 3% faster on
+// the prompts, 8% slower with gradients, 50% over a cache.
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_rows_k0[kKeys * DT * 2];
 template <int DT>

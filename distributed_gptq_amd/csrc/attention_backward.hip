@@ -200,7 +200,7 @@ __device__ __forceinline__ void exact_dq(f32x16 (&acc)[DT / 32], const AttnArgs&
 // the error of dq against 64 bits is 1.45 times that of its own rounding for 2048
 // tokens and heads of 128, 1.50 for 3400 and heads of 64, and grows on.
 //
-// Bound by the MFMAs (busy 50% of the cycles) beside the vector instructions: 152
+// Bound by the waits between a wave's steps (MFMAs busy 50% of the cycles): 152-159
 // us for 2 x 2048 tokens, 32 over 8 heads of 128, of which the rests take 29 and
 // delta 8 (bf16; a kernel of its own took 17 with its launch).
 template <bool kBF16, int DT>
@@ -341,8 +341,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(BackArgs args, int slot
 // each, as 16 further channels of q and g (their parts, below) and of k and v
 // (the parts' units).
 //
-// 175 us and 13 of the join for 2 x 2048 tokens, 32 over 8 heads of 128 (MFMAs
-// busy 44% of the cycles, no LDS conflicts); one workgroup of 8 waves a CU, lse
+// 175-182 us and 13 of the join for 2 x 2048 tokens, 32 over 8 heads of 128 (MFMAs
+// busy 43% of the cycles, no LDS conflicts); one workgroup of 8 waves a CU, lse
 // and delta in registers: 218.
 constexpr int kBackRows = 64;
 template <int DT>

@@ -260,9 +260,12 @@ bool attention_sizes(int64_t B, int64_t T, int64_t S, int64_t H, int64_t Hk, int
 }  // namespace
 
 // Few rows: two workgroups of 4 waves run on each of the 256 CUs, so 512 for one
-// sequence, whose parts are equal; twice that for several, whose lengths differ.
-// Measured (us with the join, 512 / 1024 wanted): 24 sequences of up to 8192
-// tokens 78.2 / 70.1, one of 131072 102.8 / 104.9.  A part has at least a tile of
+// sequence, whose parts are equal; twice that for several, whose lengths (on the
+// GPU, not looked at) may differ.  One case each was measured (us with the join,
+// 512 / 1024 wanted): 24 sequences of 1 to 8192 tokens 78.2 / 70.1, one of 131072
+// 102.8 / 104.9.  The kernel is chosen by the rows of a sequence on average: of a
+// chunk beside many single tokens, one of both is on the other's kernel, which is
+// right and slower than a batch of its own.  A part has at least a tile of
 // 32 keys for each wave.  More rows than 32 go to the kernel of 128, though neither
 // is ahead throughout (us, that kernel / tiles of 32, heads 32 over 8 of 128: 16 new
 // tokens over 8192 26.0 / 21.5, 16 for each of 8 sequences over 4096 35.8 / 42.3, 32

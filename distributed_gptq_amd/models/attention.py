@@ -10,11 +10,13 @@ projection's output (any strides, the last dimension contiguous): nothing is
 copied then.  ``cu_seqlens`` holds the B + 1 offsets of the sequences (int32
 on the GPU, the first 0); tokens past the last one give zeros.  A cache is
 (pages, page_size, kv_heads, head_dim); a sequence's block table row names its
-pages in order.
+pages in order.  Offsets, positions, slots, lengths and page numbers may be int64
+too, which takes two small launches more.
 
 The functions run on the current stream, allocate from torch's caching
-allocator, do not wait for the GPU, and can be captured in a graph.  There is
-no CPU path.
+allocator, do not wait for the GPU, and can be captured in a graph
+(``PagedKVCache.extend`` waits, and can not).  There is no CPU path.  Forward-mode
+derivatives raise, as do gradients of what has none.
 """
 from __future__ import annotations
 
@@ -152,7 +154,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
     query sees the last key, the one before it one key less, and so on; a query
     without a key gives zeros, and gradients of zero.  ``scale``: 1 / sqrt(head_dim)
     by default, else within [1e-7, 1e7].  Infinities and NaN reach only the rows
-    and gradients whose sums they are terms of."""
+    and gradients whose sums they are terms of; sums that are infinite are made
+    a second time, at up to 20 times a finite call's time."""
     return _op("attention", q, k, v, cu_seqlens, cu_seqlens_k, causal, _scale(q, scale))
 
 
@@ -229,7 +232,11 @@ class PagedKVCache:
     def extend(self, seqs: Sequence, new: Sequence[int]) -> PagedBatch:
         """Places for ``new[b]`` more tokens of sequence ``seqs[b]`` (unknown ones
         begin here), and the step's tensors.  Raises MemoryError, and changes
-        nothing, when the pages do not suffice."""
+        nothing, when the pages do not suffice.
+
+        The host makes all sequences' whole block tables on each call (0.3-0.6 ms
+        for one of 8192 pages, 0.9-1.7 ms for 48 of 512) and copies them from pageable
+        memory, which waits for what the current stream has been given."""
         seqs, new = list(seqs), [int(n) for n in new]
         if not seqs or len(seqs) != len(new) or len(set(seqs)) != len(seqs) or min(new) < 1:
             raise ValueError("extend: one count of new tokens, at least 1, for each of some different sequences")
