@@ -150,3 +150,61 @@ def test_gradient_of_an_infinite_gradient(L, H, Hk, D, dtype):
         fine = ref.isfinite()
         assert torch.equal(got.isnan(), ref.isnan()) and torch.equal(got.double()[ref.isinf()], ref[ref.isinf()]), name
         check(got[fine], (ref[fine], clean[name][1][fine]))
+
+
+def spoil(v, seed, n=6):
+    """v with infinities of both signs and NaN in some places, and v with zeros there."""
+    g = torch.Generator().manual_seed(seed)
+    bad, clean = v.clone(), v.clone()
+    for i in range(n):
+        at = tuple(int(torch.randint(0, s, (1,), generator=g)) for s in v.shape)
+        bad[at] = (math.inf, -math.inf, math.nan)[i % 3]
+        clean[at] = 0
+    return bad, clean
+
+
+def follows(out, q, k, bad, clean):
+    """out: infinite or NaN where the formula is (of what a row sees), within the
+    bounds elsewhere; later queries see all earlier keys and their own."""
+    L, S, G = q.shape[0], k.shape[0], q.shape[1] // k.shape[1]
+    ref, bound = one(q, k, clean)["out"]
+    sees = (torch.arange(S, device="cuda")[None] <= torch.arange(L, device="cuda")[:, None] + S - L).float()
+
+    def count(x):  # of such values that each row sees: (L, heads, channels)
+        return torch.einsum("ls,shd->lhd", sees, x.float()).repeat_interleave(G, 1) > 0
+    up, down, nan = count(bad == math.inf), count(bad == -math.inf), count(bad.isnan())
+    nan = nan | (up & down)
+    assert torch.equal(out.isnan(), nan)
+    assert torch.equal(out == math.inf, up & ~nan) and torch.equal(out == -math.inf, down & ~nan)
+    fine = ~(up | down | nan)
+    check(out[fine], (ref[fine], bound[fine]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("L,H,Hk,D", [(70, 7, 1, 40), (200, 6, 2, 96), (333, 4, 4, 64), (150, 8, 2, 128)])
+def test_not_finite_values_as_the_formula(L, H, Hk, D, dtype):
+    q, k, v, _ = step(L, H, Hk, D, dtype)
+    for seed in range(4):
+        bad, clean = spoil(v, seed)
+        with torch.no_grad():
+            follows(A().attention(q, k, bad), q, k, bad, clean)
+        follows(A().attention(q.clone().requires_grad_(True), k, bad).detach(), q, k, bad, clean)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,Hk,D,page", [(7, 1, 40, 7), (6, 2, 96, 16), (8, 4, 64, 24), (8, 2, 128, 64)])
+@pytest.mark.parametrize("new,S", [(1, 50), (1, 3000), (5, 700), (130, 1300)])
+def test_not_finite_cached_values_as_the_formula(new, S, H, Hk, D, page, dtype):
+    """Few and many rows, one part and many, pages that end inside a tile."""
+    _, k, v, _ = step(S, H, Hk, D, dtype)
+    q = step(new, H, Hk, D, dtype)[0]
+    pages = -(-S // page)
+    table = torch.randperm(pages, device="cuda").int()
+    place = table.long()[torch.arange(S, device="cuda") // page] * page + torch.arange(S, device="cuda") % page
+    for seed in range(3):
+        bad, clean = spoil(v, seed)
+        kc, vc = (torch.full((pages * page, Hk, D), math.nan, device="cuda", dtype=dtype) for _ in range(2))
+        kc[place], vc[place] = k, bad
+        out = A().paged_attention(q, kc.view(pages, page, Hk, D), vc.view(pages, page, Hk, D), table[None],
+                                  torch.tensor([S], device="cuda"), torch.tensor([0, new], device="cuda"))
+        follows(out, q, k, bad, clean)
