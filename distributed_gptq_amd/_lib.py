@@ -24,6 +24,8 @@ TORCH_OPS_PATH = os.path.join(HERE, "libgptq_torch.so")  # the native torch oper
 OK, ERR_ARG, ERR_SHAPE, ERR_DTYPE, ERR_WORKSPACE, ERR_LAUNCH, ERR_DEVICE = range(7)
 # dtypes (gptq_dtype)
 F32, F16, BF16 = 0, 1, 2
+# what a paged cache holds (gptq_code)
+CODE_NONE, CODE_I8, CODE_E4M3 = 0, 1, 2
 # factor modes / sweep flags
 FACTOR_FULL_INVERSE, FACTOR_UPPER_CHOL_INV = 0, 1
 SWEEP_TRAILING, SWEEP_REF_QUANTIZER, SWEEP_GROUPS_FROM_W0, PARAMS_SYM = 1, 2, 4, 8
@@ -80,6 +82,17 @@ SIGNATURES = {
     "gptq_paged_attention_workspace_size": (_sz, [_i64] * 6),
     "gptq_paged_attention": (_i, [_p, _p, _p, _i] + [_i64] * 8 + [_p] + [_i64] * 4 + [_p, _p] + [_i64] * 5
                              + [_f, _i64, _p, _p, _sz, _p]),
+    "gptq_norm_rotary": (_i, [_p, _p, _i] + [_i64] * 4 + [_p, _p, _i, _f, _p, _i64, _i64, _p, _i] + [_i64] * 4
+                         + [_p, _p, _p]),
+    "gptq_norm_rotary_backward_workspace_size": (_sz, [_i64] * 4),
+    "gptq_norm_rotary_backward": (_i, [_p] * 4 + [_i] + [_i64] * 8 + [_p, _p, _i, _f, _p, _i64, _i64, _p, _i]
+                                  + [_i64] * 4 + [_p] * 5 + [_sz, _p]),
+    "gptq_norm_rotary_append": (_i, [_p, _p, _p, _i] + [_i64] * 6 + [_p, _p, _i, _f, _p, _i64, _i64, _p, _i, _p]
+                                + [_i64] * 6 + [_p, _i] + ([_p] + [_i64] * 3) * 4 + [_p]),
+    "gptq_cached_rows": (_i, [_i] + ([_p] + [_i64] * 3) * 4 + [_p] + [_i64] * 4 + [_p, _p] + [_i64] * 4
+                         + [_p, _p, _i, _p]),
+    "gptq_code_attention": (_i, [_p, _i, _i64, _i64, _i] + ([_p] + [_i64] * 3) * 4 + [_p] + [_i64] * 4 + [_p, _p]
+                            + [_i64] * 5 + [_f, _i64, _p, _p, _sz, _p]),
     "gptq_stream_read": (_i, [_p, _sz, _i, _i, _p, _p]),
 }
 

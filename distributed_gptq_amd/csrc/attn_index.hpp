@@ -155,6 +155,31 @@ GPTQ_INDEX KvAt kv_at(const AttnArgs& a, const Seq& s, int key) {
     return KvAt{0, s.k0 + key};
   }
 }
+// The sequence of packed row t of B sequences by their offsets, each thread's own
+// row: the last whose offset is not past it, or B for rows behind the last one.
+// Offsets that do not ascend give some sequence.
+GPTQ_INDEX int sequence_of(const int32_t* cu, int B, int t) {
+  if (t >= cu[B]) return B;
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if (cu[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+// Which cached token packed row t is, when a sequence's rows are its last ones:
+// -1 where it has none.
+GPTQ_INDEX int cached_token(const int32_t* cu, const int32_t* context, int B, int most, int t, int* b) {
+  *b = sequence_of(cu, B, t);
+  if (*b >= B) return -1;
+  const int have = clamp_int(context[*b], 0, most);
+  const int64_t key = static_cast<int64_t>(have) - cu[*b + 1] + t;
+  return key >= 0 && key < have ? static_cast<int>(key) : -1;
+}
+
 template <bool kPaged>
 GPTQ_INDEX const uint16_t* kv_row(const Rows16& r, int64_t page_stride, int hk, KvAt k) {
   const uint16_t* p = r.p + hk * r.sh + k.at * r.st;

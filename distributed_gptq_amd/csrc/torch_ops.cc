@@ -300,6 +300,227 @@ at::Tensor rotary_append(const at::Tensor& q_, const at::Tensor& k_, const at::T
   return qo;
 }
 
+// ------------------------------------------- normed heads, a cache of codes ----
+
+// t (16 bits or 32) with 16-byte aligned rows of whole 8s of values: itself
+// wherever it has them already
+at::Tensor vector_rows(const at::Tensor& t) {
+  if (rows_aligned(t)) return t;
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
+void check_weights(const char* fn, const at::Tensor& q, const at::Tensor& q_weight, const at::Tensor& k_weight) {
+  TORCH_CHECK_VALUE(q_weight.device() == q.device() && k_weight.device() == q.device(), fn,
+                    ": expected GPU tensors on one device");
+  TORCH_CHECK_TYPE(q_weight.scalar_type() == k_weight.scalar_type(), fn, ": the weights have different types");
+  TORCH_CHECK_VALUE(q_weight.dim() == 1 && k_weight.dim() == 1 && q_weight.size(0) == q.size(-1) &&
+                        k_weight.size(0) == q.size(-1),
+                    fn, ": weights ", q_weight.sizes(), " and ", k_weight.sizes(), " for heads of ", q.size(-1));
+}
+
+// a table and positions as the kernels take them (undefined: nothing turns)
+struct Angles {
+  at::Tensor table, positions;
+  Angles(const char* fn, const at::Tensor& q, const std::optional<at::Tensor>& table_,
+         const std::optional<at::Tensor>& positions_) {
+    check_table(fn, q, table_, positions_);
+    if (!table_) return;
+    table = vector_rows(table_->contiguous());
+    positions = int32_of(*positions_, q, "positions");
+  }
+  const float* at() const { return table.defined() ? table.const_data_ptr<float>() : nullptr; }
+  int64_t rows() const { return table.defined() ? table.size(0) : 0; }
+  int64_t dim() const { return table.defined() ? 2 * table.size(2) : 0; }
+  const int32_t* where() const { return positions.defined() ? positions.const_data_ptr<int32_t>() : nullptr; }
+};
+
+// q and k normed, weighted and turned
+std::tuple<at::Tensor, at::Tensor> norm_rotary(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& q_weight,
+                                               const at::Tensor& k_weight, const std::optional<at::Tensor>& table,
+                                               const std::optional<at::Tensor>& positions, bool interleaved, double eps) {
+  check_heads("gptq::norm_rotary", q_, k_, k_, 3);
+  TORCH_CHECK_VALUE(k_.size(0) == q_.size(0), "gptq::norm_rotary: ", q_.size(0), " queries and ", k_.size(0), " keys");
+  check_weights("gptq::norm_rotary", q_, q_weight, k_weight);
+  const c10::DeviceGuard guard(q_.device());
+  const Angles angles("gptq::norm_rotary", q_, table, positions);
+  const at::Tensor q = vector_rows(q_), k = vector_rows(k_), wq = vector_rows(q_weight), wk = vector_rows(k_weight);
+  at::Tensor qo = at::empty(q.sizes(), q.options()), ko = at::empty(k.sizes(), k.options());
+  GPTQ_CALL(gptq_norm_rotary, q.const_data_ptr(), k.const_data_ptr(), dtype_code(q.scalar_type()), stride_of(q, 0),
+            stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), wq.const_data_ptr(), wk.const_data_ptr(),
+            dtype_code(wq.scalar_type()), static_cast<float>(eps), angles.at(), angles.rows(), angles.dim(), angles.where(),
+            interleaved, q.size(0), q.size(1), k.size(1), q.size(2), qo.mutable_data_ptr(), ko.mutable_data_ptr(),
+            stream_of(q));
+  return {qo, ko};
+}
+
+// (dq, dk, dq_weight, dk_weight); the weights' undefined where they are not wanted
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> norm_rotary_backward(
+    const at::Tensor& grad_q_, const at::Tensor& grad_k_, const at::Tensor& q_, const at::Tensor& k_,
+    const at::Tensor& q_weight, const at::Tensor& k_weight, const std::optional<at::Tensor>& table,
+    const std::optional<at::Tensor>& positions, bool interleaved, double eps, bool weights) {
+  const char* fn = "gptq::norm_rotary_backward";
+  check_heads(fn, q_, k_, k_, 3);
+  check_weights(fn, q_, q_weight, k_weight);
+  TORCH_CHECK_VALUE(k_.size(0) == q_.size(0) && grad_q_.sizes() == q_.sizes() && grad_k_.sizes() == k_.sizes() &&
+                        grad_q_.device() == q_.device() && grad_k_.device() == q_.device(),
+                    fn, ": the gradients do not match the heads");
+  TORCH_CHECK_TYPE(grad_q_.scalar_type() == q_.scalar_type() && grad_k_.scalar_type() == q_.scalar_type(), fn,
+                   ": the gradients have another type");
+  const c10::DeviceGuard guard(q_.device());
+  const Angles angles(fn, q_, table, positions);
+  const at::Tensor q = vector_rows(q_), k = vector_rows(k_), wq = vector_rows(q_weight), wk = vector_rows(k_weight);
+  const at::Tensor gq = vector_rows(grad_q_), gk = vector_rows(grad_k_);
+  at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dwq, dwk, ws;
+  size_t bytes = 0;
+  if (weights) {
+    dwq = at::empty(wq.sizes(), wq.options()), dwk = at::empty(wk.sizes(), wk.options());
+    bytes = gptq_norm_rotary_backward_workspace_size(q.size(0), q.size(1), k.size(1), q.size(2));
+    ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+  }
+  GPTQ_CALL(gptq_norm_rotary_backward, gq.const_data_ptr(), gk.const_data_ptr(), q.const_data_ptr(), k.const_data_ptr(),
+            dtype_code(q.scalar_type()), stride_of(gq, 0), stride_of(gq, 1), stride_of(gk, 0), stride_of(gk, 1),
+            stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), wq.const_data_ptr(), wk.const_data_ptr(),
+            dtype_code(wq.scalar_type()), static_cast<float>(eps), angles.at(), angles.rows(), angles.dim(), angles.where(),
+            interleaved, q.size(0), q.size(1), k.size(1), q.size(2), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
+            weights ? dwq.mutable_data_ptr() : nullptr, weights ? dwk.mutable_data_ptr() : nullptr,
+            weights ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(q));
+  return {dq, dk, dwq, dwk};
+}
+
+// what a cache holds: codes with scales, or values without
+int code_of(const char* fn, const at::Tensor& cache, const std::optional<at::Tensor>& k_scale,
+            const std::optional<at::Tensor>& v_scale) {
+  const auto t = cache.scalar_type();
+  const int code = t == at::kChar ? GPTQ_CODE_I8 : t == at::kFloat8_e4m3fn ? GPTQ_CODE_E4M3 : GPTQ_CODE_NONE;
+  TORCH_CHECK_VALUE(code != GPTQ_CODE_NONE ? k_scale && v_scale : !k_scale && !v_scale, fn, ": a cache of ", t,
+                    code != GPTQ_CODE_NONE ? " needs the scales of its keys and values" : " has no scales");
+  return code;
+}
+void check_cache(const char* fn, const at::Tensor& k_cache, const at::Tensor& v_cache, int code,
+                 const std::optional<at::Tensor>& k_scale, const std::optional<at::Tensor>& v_scale) {
+  TORCH_CHECK_VALUE(k_cache.is_cuda() && v_cache.device() == k_cache.device(), fn, ": expected GPU tensors on one device");
+  TORCH_CHECK_TYPE(v_cache.scalar_type() == k_cache.scalar_type(), fn, ": the caches of keys and of values have different types");
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(), fn, ": caches ", k_cache.sizes(), " and ",
+                    v_cache.sizes(), " are not two of (pages, page_size, kv_heads, head_dim)");
+  const int64_t unit = code == GPTQ_CODE_NONE ? 8 : 16;
+  for (const at::Tensor* c : {&k_cache, &v_cache}) {
+    bool ok = c->stride(-1) == 1 && reinterpret_cast<uintptr_t>(c->const_data_ptr()) % 16 == 0;
+    for (int64_t i = 0; i < 3; ++i) ok = ok && (c->stride(i) % unit == 0 || c->size(i) <= 1);
+    TORCH_CHECK_VALUE(ok, fn, ": the cache's heads have to be contiguous and 16-byte aligned");  // (it is never copied)
+  }
+  if (code == GPTQ_CODE_NONE) return;
+  for (const at::Tensor* c : {&*k_scale, &*v_scale}) {
+    TORCH_CHECK_TYPE(c->scalar_type() == at::kFloat, fn, ": the scales have to be float32");
+    TORCH_CHECK_VALUE(c->device() == k_cache.device() && c->sizes() == k_cache.sizes().slice(0, 3), fn, ": scales ",
+                      c->sizes(), " for a cache ", k_cache.sizes());
+  }
+}
+#define GPTQ_CACHE(t) (t).data_ptr(), stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)
+#define GPTQ_SCALE(t) (t) ? (t)->data_ptr<float>() : nullptr, (t) ? stride_of(*(t), 0) : 0, (t) ? stride_of(*(t), 1) : 0, (t) ? stride_of(*(t), 2) : 0
+
+// rotary_append with norms, into a cache of values or of codes
+at::Tensor norm_rotary_append(const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_,
+                              const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight,
+                              const std::optional<at::Tensor>& table, const std::optional<at::Tensor>& positions,
+                              at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots_,
+                              std::optional<at::Tensor> k_scale, std::optional<at::Tensor> v_scale, bool interleaved,
+                              double eps) {
+  const char* fn = "gptq::norm_rotary_append";
+  check_heads(fn, q_, k_, v_, 3);
+  const int code = code_of(fn, k_cache, k_scale, v_scale);
+  check_cache(fn, k_cache, v_cache, code, k_scale, v_scale);
+  TORCH_CHECK_TYPE(code != GPTQ_CODE_NONE || k_cache.scalar_type() == q_.scalar_type(), fn, ": heads of ", q_.scalar_type(),
+                   " into a cache of ", k_cache.scalar_type());
+  TORCH_CHECK_VALUE(k_cache.device() == q_.device() && k_.size(0) == q_.size(0) && k_cache.size(2) == k_.size(1) &&
+                        k_cache.size(3) == k_.size(2) && slots_.dim() == 1 && slots_.size(0) == q_.size(0),
+                    fn, ": queries ", q_.sizes(), ", keys ", k_.sizes(), ", slots ", slots_.sizes(), " and a cache ",
+                    k_cache.sizes(), " do not match");
+  TORCH_CHECK_VALUE(!q_weight == !k_weight, fn, ": the queries' weights without the keys', or these without those");
+  if (q_weight) check_weights(fn, q_, *q_weight, *k_weight);
+  const c10::DeviceGuard guard(q_.device());
+  const Angles angles(fn, q_, table, positions);
+  const at::Tensor q = vector_rows(q_), k = vector_rows(k_), v = vector_rows(v_);
+  at::Tensor wq, wk;
+  if (q_weight) wq = vector_rows(*q_weight), wk = vector_rows(*k_weight);
+  const at::Tensor slots = int32_of(slots_, q, "slots");
+  at::Tensor qo = at::empty(q.sizes(), q.options());
+  if (k_cache.numel() == 0) TORCH_CHECK_VALUE(k.numel() == 0, fn, ": the cache has no pages");
+  GPTQ_CALL(gptq_norm_rotary_append, q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(),
+            dtype_code(q.scalar_type()), stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0),
+            stride_of(v, 1), q_weight ? wq.const_data_ptr() : nullptr, q_weight ? wk.const_data_ptr() : nullptr,
+            q_weight ? dtype_code(wq.scalar_type()) : 0, static_cast<float>(eps), angles.at(), angles.rows(), angles.dim(),
+            angles.where(), interleaved, slots.const_data_ptr<int32_t>(), k_cache.size(1), k_cache.size(0), q.size(0),
+            q.size(1), k.size(1), q.size(2), qo.mutable_data_ptr(), code, GPTQ_CACHE(k_cache), GPTQ_CACHE(v_cache),
+            GPTQ_SCALE(k_scale), GPTQ_SCALE(v_scale), stream_of(q));
+  return qo;
+}
+
+// the last cached tokens of each sequence as packed rows
+std::tuple<at::Tensor, at::Tensor> cached_rows(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                               const at::Tensor& block_table, const at::Tensor& context,
+                                               const at::Tensor& cu_rows, int64_t tokens,
+                                               const std::optional<at::Tensor>& k_scale,
+                                               const std::optional<at::Tensor>& v_scale, at::ScalarType dtype) {
+  const char* fn = "gptq::cached_rows";
+  const int code = code_of(fn, k_cache, k_scale, v_scale);
+  check_cache(fn, k_cache, v_cache, code, k_scale, v_scale);
+  TORCH_CHECK_TYPE(code != GPTQ_CODE_NONE || k_cache.scalar_type() == dtype, fn, ": rows of ", dtype, " from a cache of ",
+                   k_cache.scalar_type());
+  const int out = dtype_code(dtype);
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && context.dim() == 1 && block_table.size(0) == context.size(0) &&
+                        cu_rows.dim() == 1 && cu_rows.numel() == context.size(0) + 1 && context.size(0) >= 1,
+                    fn, ": a block table ", block_table.sizes(), " and offsets ", cu_rows.sizes(), " for ", context.sizes(),
+                    " contexts");
+  TORCH_CHECK_VALUE(tokens >= 0, fn, ": ", tokens, " rows");
+  const c10::DeviceGuard guard(k_cache.device());
+  const at::Tensor table = int32_of(block_table, k_cache, "block_table"), ctx = int32_of(context, k_cache, "context_lens"),
+                   cu = int32_of(cu_rows, k_cache, "cu_seqlens");
+  const int64_t Hk = k_cache.size(2), D = k_cache.size(3);
+  at::Tensor k = at::empty({tokens, Hk, D}, k_cache.options().dtype(dtype)), v = at::empty_like(k);
+  GPTQ_CALL(gptq_cached_rows, code, GPTQ_CACHE(k_cache), GPTQ_CACHE(v_cache), GPTQ_SCALE(k_scale), GPTQ_SCALE(v_scale),
+            table.const_data_ptr<int32_t>(), table.size(1), table.size(1), k_cache.size(1), k_cache.size(0),
+            ctx.const_data_ptr<int32_t>(), cu.const_data_ptr<int32_t>(), context.size(0), tokens, Hk, D,
+            k.mutable_data_ptr(), v.mutable_data_ptr(), out, stream_of(k_cache));
+  return {k, v};
+}
+
+// paged_attention over a cache of codes
+at::Tensor code_attention(const at::Tensor& q_, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                          const at::Tensor& block_table, const at::Tensor& context, const std::optional<at::Tensor>& cu_q,
+                          const at::Tensor& k_scale, const at::Tensor& v_scale, double scale, int64_t max_context) {
+  const char* fn = "gptq::code_attention";
+  const std::optional<at::Tensor> ks(k_scale), vs(v_scale);
+  const int code = code_of(fn, k_cache, ks, vs);
+  check_cache(fn, k_cache, v_cache, code, ks, vs);
+  TORCH_CHECK_VALUE(q_.device() == k_cache.device() && q_.dim() == 3 && q_.size(2) == k_cache.size(3), fn, ": queries ",
+                    q_.sizes(), " and a cache ", k_cache.sizes(), " do not match");
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && context.dim() == 1 && block_table.size(0) == context.size(0), fn,
+                    ": a block table ", block_table.sizes(), " for ", context.sizes(), " contexts");
+  const int64_t B = context.size(0), T = q_.size(0), H = q_.size(1), D = q_.size(2);
+  TORCH_CHECK_VALUE(cu_q ? cu_q->dim() == 1 && cu_q->numel() == B + 1 : T == B, fn, ": ", T, " new tokens of ", B,
+                    " sequences ", cu_q ? "need B + 1 offsets" : "without their offsets");
+  const c10::DeviceGuard guard(q_.device());
+  const at::Tensor q = aligned_rows(q_);
+  at::Tensor out = at::empty({T, H, D}, q.options());
+  if (T == 0) return out;
+  const at::Tensor table = int32_of(block_table, q, "block_table"), ctx = int32_of(context, q, "context_lens");
+  at::Tensor cq;
+  if (cu_q) cq = int32_of(*cu_q, q, "cu_seqlens");
+  const int64_t Hk = k_cache.size(2);
+  const size_t bytes = gptq_paged_attention_workspace_size(B, T, H, Hk, D, max_context);
+  at::Tensor ws;
+  if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
+  GPTQ_CALL(gptq_code_attention, q.const_data_ptr(), dtype_code(q.scalar_type()), stride_of(q, 0), stride_of(q, 1), code,
+            GPTQ_CACHE(k_cache), GPTQ_CACHE(v_cache), GPTQ_SCALE(ks), GPTQ_SCALE(vs), table.const_data_ptr<int32_t>(),
+            table.size(1), table.size(1), k_cache.size(1), k_cache.size(0), ctx.const_data_ptr<int32_t>(),
+            cu_q ? cq.const_data_ptr<int32_t>() : nullptr, B, T, H, Hk, D, static_cast<float>(scale), max_context,
+            out.mutable_data_ptr(), bytes ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(q));
+  return out;
+}
+#undef GPTQ_CACHE
+#undef GPTQ_SCALE
+
 // -------------------------------------------------------------- gradients ----
 
 template <class F>
@@ -408,6 +629,54 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
   return op.call(q, k, table, positions, interleaved, inverse);
 }
 
+struct NormRotaryGrad : torch::autograd::Function<NormRotaryGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                               const at::Tensor& k_weight, const std::optional<at::Tensor>& table,
+                               const std::optional<at::Tensor>& positions, bool interleaved, double eps) {
+    static const auto op = typed_op<decltype(norm_rotary)>("gptq::norm_rotary");
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [qo, ko] = op.call(q, k, q_weight, k_weight, table, positions, interleaved, eps);
+    ctx->save_for_backward({q, k, q_weight, k_weight, or_none(table), or_none(positions)});
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["eps"] = eps;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = typed_op<decltype(norm_rotary_backward)>("gptq::norm_rotary_backward");
+    const auto s = ctx->get_saved_variables();
+    no_tangents("gptq::norm_rotary", {&grads[0], &grads[1], &s[0], &s[1], &s[2], &s[3]});
+    const bool weights = ctx->needs_input_grad(2) || ctx->needs_input_grad(3);
+    at::Tensor dq, dk, dwq, dwk;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      std::tie(dq, dk, dwq, dwk) =
+          op.call(grads[0], grads[1], s[0], s[1], s[2], s[3], or_null(s[4]), or_null(s[5]),
+                  ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(), weights);
+    }
+    variable_list want = {dq, dk};
+    if (weights) want.push_back(dwq), want.push_back(dwk);
+    variable_list got = once(std::move(want), {&grads[0], &grads[1], &s[0], &s[1], &s[2], &s[3]}, "gptq::norm_rotary");
+    got.resize(8);
+    return got;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> norm_rotary_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                                        const at::Tensor& k_weight, const std::optional<at::Tensor>& table,
+                                                        const std::optional<at::Tensor>& positions, bool interleaved,
+                                                        double eps) {
+  const at::Tensor angles = or_none(table);
+  no_tangents("gptq::norm_rotary", {&q, &k, &q_weight, &k_weight, &angles});
+  TORCH_CHECK(!follows({&angles}), "gptq::norm_rotary: the table gets no gradient: detach it");
+  if (follows({&q, &k, &q_weight, &k_weight})) {
+    const variable_list out = NormRotaryGrad::apply(q, k, q_weight, k_weight, table, positions, interleaved, eps);
+    return {out[0], out[1]};
+  }
+  static const auto op = typed_op<decltype(norm_rotary)>("gptq::norm_rotary");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, q_weight, k_weight, table, positions, interleaved, eps);
+}
+
 // Serving's operators have no gradient at all.
 void no_gradient(const char* name, std::initializer_list<const at::Tensor*> ts) {
   no_tangents(name, ts);
@@ -433,6 +702,43 @@ at::Tensor paged_attention_autograd(const at::Tensor& q, const at::Tensor& k_cac
   return op.call(q, k_cache, v_cache, block_table, context, cu_q, scale, max_context);
 }
 
+at::Tensor norm_rotary_append_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                       const std::optional<at::Tensor>& q_weight, const std::optional<at::Tensor>& k_weight,
+                                       const std::optional<at::Tensor>& table, const std::optional<at::Tensor>& positions,
+                                       at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots,
+                                       std::optional<at::Tensor> k_scale, std::optional<at::Tensor> v_scale,
+                                       bool interleaved, double eps) {
+  const at::Tensor angles = or_none(table), wq = or_none(q_weight), wk = or_none(k_weight), ks = or_none(k_scale),
+                   vs = or_none(v_scale);
+  no_gradient("gptq::norm_rotary_append", {&q, &k, &v, &wq, &wk, &angles, &k_cache, &v_cache, &ks, &vs});
+  static const auto op = typed_op<decltype(norm_rotary_append)>("gptq::norm_rotary_append");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, q_weight, k_weight, table, positions, std::move(k_cache), std::move(v_cache), slots,
+                 std::move(k_scale), std::move(v_scale), interleaved, eps);
+}
+
+std::tuple<at::Tensor, at::Tensor> cached_rows_autograd(const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                                        const at::Tensor& block_table, const at::Tensor& context,
+                                                        const at::Tensor& cu_rows, int64_t tokens,
+                                                        const std::optional<at::Tensor>& k_scale,
+                                                        const std::optional<at::Tensor>& v_scale, at::ScalarType dtype) {
+  const at::Tensor ks = or_none(k_scale), vs = or_none(v_scale);
+  no_gradient("gptq::cached_rows", {&k_cache, &v_cache, &ks, &vs});
+  static const auto op = typed_op<decltype(cached_rows)>("gptq::cached_rows");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(k_cache, v_cache, block_table, context, cu_rows, tokens, k_scale, v_scale, dtype);
+}
+
+at::Tensor code_attention_autograd(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                                   const at::Tensor& block_table, const at::Tensor& context,
+                                   const std::optional<at::Tensor>& cu_q, const at::Tensor& k_scale,
+                                   const at::Tensor& v_scale, double scale, int64_t max_context) {
+  no_gradient("gptq::code_attention", {&q, &k_cache, &v_cache, &k_scale, &v_scale});
+  static const auto op = typed_op<decltype(code_attention)>("gptq::code_attention");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k_cache, v_cache, block_table, context, cu_q, k_scale, v_scale, scale, max_context);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(gptq, m) {
@@ -450,6 +756,18 @@ TORCH_LIBRARY_FRAGMENT(gptq, m) {
         "Tensor(b!) v_cache, Tensor slots, bool interleaved) -> Tensor");
   m.def("paged_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, "
         "Tensor? cu_seqlens, float scale, int max_context) -> Tensor");
+  m.def("norm_rotary(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor? table, Tensor? positions, "
+        "bool interleaved, float eps) -> (Tensor, Tensor)");
+  m.def("norm_rotary_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, "
+        "Tensor? table, Tensor? positions, bool interleaved, float eps, bool weights) "
+        "-> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("norm_rotary_append(Tensor q, Tensor k, Tensor v, Tensor? q_weight, Tensor? k_weight, Tensor? table, "
+        "Tensor? positions, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor slots, Tensor(c!)? k_scale, "
+        "Tensor(d!)? v_scale, bool interleaved, float eps) -> Tensor");
+  m.def("cached_rows(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, Tensor cu_seqlens, "
+        "int tokens, Tensor? k_scale, Tensor? v_scale, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("code_attention(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor context_lens, "
+        "Tensor? cu_seqlens, Tensor k_scale, Tensor v_scale, float scale, int max_context) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(gptq, CUDA, m) {
@@ -460,6 +778,11 @@ TORCH_LIBRARY_IMPL(gptq, CUDA, m) {
   m.impl("paged_attention", paged_attention);
   m.impl("rotary", rotary);
   m.impl("rotary_append", rotary_append);
+  m.impl("norm_rotary", norm_rotary);
+  m.impl("norm_rotary_backward", norm_rotary_backward);
+  m.impl("norm_rotary_append", norm_rotary_append);
+  m.impl("cached_rows", cached_rows);
+  m.impl("code_attention", code_attention);
 }
 
 TORCH_LIBRARY_IMPL(gptq, Autograd, m) {
@@ -467,7 +790,12 @@ TORCH_LIBRARY_IMPL(gptq, Autograd, m) {
   m.impl("rotary", rotary_autograd);
   m.impl("rotary_append", rotary_append_autograd);
   m.impl("paged_attention", paged_attention_autograd);
-  // (parts of attention's own derivative)
+  m.impl("norm_rotary", norm_rotary_autograd);
+  m.impl("norm_rotary_append", norm_rotary_append_autograd);
+  m.impl("cached_rows", cached_rows_autograd);
+  m.impl("code_attention", code_attention_autograd);
+  // (parts of the operators' own derivatives)
+  m.impl("norm_rotary_backward", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_forward", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_backward", torch::autograd::autogradNotImplementedFallback());
 }

@@ -30,6 +30,8 @@ import torch.nn as nn
 
 from .. import _lib as L
 
+CODES = (torch.int8, torch.float8_e4m3fn)  # what a quantised cache holds, beside fp32 scales
+
 _ops: dict = {}  # name -> operator, once its library is loaded
 
 
@@ -127,18 +129,44 @@ def rotary(q: torch.Tensor, k: torch.Tensor, table: torch.Tensor, positions: tor
     return _op("rotary", q, k, table, positions, interleaved, False)
 
 
+def norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                table: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None,
+                interleaved: bool = False, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``rotary`` of normed heads in one pass: each head of q and k over its root
+    mean square, x (mean x^2 + eps)^-1/2, times ``q_weight`` or ``k_weight``
+    (head_dim values, the same for all heads; fp32, fp16 or bf16), then turned.
+    ``table`` None: only normed.  head_dim a multiple of 8 up to 256, the turned
+    channels of 4; ``eps`` within [1e-12, 1].  Computed in fp32 and rounded once;
+    differentiable in q, k and the weights (once), whose gradients are the same
+    bits from call to call."""
+    return _op("norm_rotary", q, k, q_weight, k_weight, table, positions, interleaved, eps)
+
+
 def rotary_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: Optional[torch.Tensor],
                   positions: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor,
-                  slots: torch.Tensor, interleaved: bool = False) -> torch.Tensor:
+                  slots: torch.Tensor, interleaved: bool = False, *, k_scale: Optional[torch.Tensor] = None,
+                  v_scale: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                  k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6) -> torch.Tensor:
     """``rotary`` for new tokens in one launch with the cache's update: returns
     the turned queries and writes the turned keys and the values of token t into
     place ``slots[t]`` (page * page_size + row) of the cache.  Tokens with a
     negative slot (padding) are not written.  ``table`` None: positions are not
     rotary, nothing is turned; positions outside it are turned by the angles of
-    its ends.  For serving: no gradient is recorded."""
+    its ends.  For serving: no gradient is recorded.
+
+    ``q_weight`` and ``k_weight``: the heads are normed first, as in
+    ``norm_rotary``.  A cache of int8 or float8_e4m3fn holds codes (head_dim a
+    multiple of 16, the turned channels of 8), and ``k_scale`` and ``v_scale``
+    (pages, page_size, kv_heads; float32) the scale of each token's head: its
+    largest value over 127 or 448.  Codes are of the fp32 values, rounded to the
+    nearest; heads up to 2^-120 read back as zeros, ones with values that are not
+    finite as NaN."""
     if _needs_grad(q, k, v):
         raise RuntimeError("rotary_append records no gradient: call it under torch.no_grad()")
-    return _op("rotary_append", q, k, v, table, positions, k_cache, v_cache, slots, interleaved)
+    if k_scale is None and v_scale is None and q_weight is None and k_weight is None and k_cache.dtype not in CODES:
+        return _op("rotary_append", q, k, v, table, positions, k_cache, v_cache, slots, interleaved)
+    return _op("norm_rotary_append", q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, k_scale,
+               v_scale, interleaved, eps)
 
 
 # --------------------------------------------------------------- attention --
@@ -161,7 +189,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
-                    scale: Optional[float] = None, max_context: Optional[int] = None) -> torch.Tensor:
+                    scale: Optional[float] = None, max_context: Optional[int] = None, *,
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of new tokens, q (T, heads, head_dim), over the cache,
     which holds their own keys and values already (``rotary_append``).
 
@@ -170,13 +199,39 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``block_table`` (B, pages): the sequence's pages, entries past its context
     unused.  ``cu_seqlens``: offsets of the sequences' new tokens (None: one
     token each).  ``max_context``: the longest context where it is known, for
-    the choice of kernel (by default what the block table could hold)."""
+    the choice of kernel (by default what the block table could hold).
+
+    ``k_scale`` and ``v_scale``: those of a cache of codes (``rotary_append``),
+    whose rows are code times scale; q is fp16 or bf16.  A row whose scale is NaN
+    reaches the queries that see it only."""
     if _needs_grad(q, k_cache, v_cache):
         raise RuntimeError("paged_attention records no gradient: call it under torch.no_grad()")
     if max_context is None:
         max_context = block_table.shape[-1] * k_cache.shape[1]
+    if k_cache.dtype in CODES or k_scale is not None or v_scale is not None:
+        if k_scale is None or v_scale is None or k_cache.dtype not in CODES:
+            raise ValueError(f"paged_attention: a cache of {k_cache.dtype} "
+                             + ("needs the scales of its keys and values" if k_cache.dtype in CODES else "has no scales"))
+        return _op("code_attention", q, k_cache, v_cache, block_table, context_lens, cu_seqlens, k_scale, v_scale,
+                   _scale(q, scale), max_context)
     return _op("paged_attention", q, k_cache, v_cache, block_table, context_lens, cu_seqlens, _scale(q, scale),
                max_context)
+
+
+def cached_rows(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+                cu_seqlens: torch.Tensor, tokens: int, dtype: Optional[torch.dtype] = None, *,
+                k_scale: Optional[torch.Tensor] = None,
+                v_scale: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values (tokens, kv_heads, head_dim) read back from the cache: of
+    sequence b the last cu_seqlens[b + 1] - cu_seqlens[b] of its
+    ``context_lens[b]`` cached tokens.  Rows that a sequence does not have, and
+    rows behind the last sequence, are zeros.  A cache of codes (``k_scale``,
+    ``v_scale``) is read as code times scale in fp32, rounded to ``dtype`` (fp16,
+    bf16 or fp32; bf16 by default); another cache has its own type.  No gradient
+    is recorded."""
+    if dtype is None:
+        dtype = torch.bfloat16 if k_cache.dtype in CODES else k_cache.dtype
+    return _op("cached_rows", k_cache, v_cache, block_table, context_lens, cu_seqlens, tokens, k_scale, v_scale, dtype)
 
 
 # ------------------------------------------------------------------- cache --
@@ -197,7 +252,13 @@ class PagedKVCache:
     """Keys and values of ``layers`` layers in pages of ``page_size`` tokens,
     (pages, page_size, kv_heads, head_dim) each, and which page belongs to which
     sequence (on the host).  All layers share the pages' numbers.  Places that
-    no token was written to are never read."""
+    no token was written to are never read.
+
+    ``dtype`` int8 or float8_e4m3fn: a quantised cache of codes, with ``k_scale``
+    and ``v_scale`` (layers, pages, page_size, kv_heads), None of another cache;
+    head_dim is a multiple of 16.  A head's rows of a page lie next to each other
+    then: 2 KB at a time for pages of 16 tokens and heads of 128, where a token's
+    heads side by side would leave 128 bytes."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, layers: int = 1,
                  dtype: torch.dtype = torch.float16, device="cuda"):
@@ -205,9 +266,18 @@ class PagedKVCache:
             raise ValueError(f"a cache of {layers} layers, {pages} pages of {page_size} tokens")
         if pages * page_size > 1 << 31:
             raise ValueError(f"{pages} pages of {page_size} tokens: a cache has at most 2^31 places, which slots can name")
-        shape = (layers, pages, page_size, kv_heads, head_dim)
-        self.k = torch.empty(shape, dtype=dtype, device=device)
-        self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.k_scale: Optional[torch.Tensor] = None
+        self.v_scale: Optional[torch.Tensor] = None
+        if dtype in CODES:
+            if head_dim % 16:
+                raise ValueError(f"a quantised cache of heads of {head_dim} values (multiples of 16 are supported)")
+            rows = (layers, pages, kv_heads, page_size)
+            self.k, self.v = (torch.empty(*rows, head_dim, dtype=dtype, device=device).transpose(2, 3) for _ in "kv")
+            self.k_scale, self.v_scale = (torch.empty(rows, device=device).transpose(2, 3) for _ in "kv")
+        else:
+            shape = (layers, pages, page_size, kv_heads, head_dim)
+            self.k = torch.empty(shape, dtype=dtype, device=device)
+            self.v = torch.empty(shape, dtype=dtype, device=device)
         self.page_size = page_size
         self._free: List[int] = list(range(pages - 1, -1, -1))
         self._pages: Dict[object, List[int]] = {}
@@ -223,6 +293,31 @@ class PagedKVCache:
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def scales(self, layer: int = 0) -> Dict[str, torch.Tensor]:
+        """``k_scale`` and ``v_scale`` of a layer as the functions' arguments (none
+        of a cache that has none)."""
+        if self.k_scale is None:
+            return {}
+        return {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer]}
+
+    def rows(self, seqs: Sequence, layer: int = 0,
+             dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """All cached keys and values of some sequences as packed rows
+        (``cached_rows``), and the sequences' offsets.  Waits for the GPU as
+        ``extend`` does."""
+        seqs = list(seqs)
+        if not seqs or not all(s in self._lens for s in seqs):
+            raise ValueError("rows: some sequences of the cache")
+        lens = [self._lens[s] for s in seqs]
+        width = max(len(self._pages[s]) for s in seqs)
+        table = [p for s in seqs for p in self._pages[s] + [0] * (width - len(self._pages[s]))]
+        parts = [table, lens, [0, *itertools.accumulate(lens)]]
+        t = torch.tensor(list(itertools.chain(*parts)), dtype=torch.int32).to(self.k.device)
+        b, c, o = t.split([len(x) for x in parts])
+        k, v = cached_rows(self.k[layer], self.v[layer], b.view(len(seqs), width), c, o, sum(lens), dtype,
+                           **self.scales(layer))
+        return k, v, o
 
     def free(self, seq) -> None:
         """Forget a sequence; its pages can be given to others."""
@@ -275,23 +370,34 @@ class QuantizedAttention(nn.Module):
     """A decoder layer's attention over quantized projections: ``qkv`` gives
     queries, keys and values of packed tokens (a ``FusedQuantizedLinear`` of the
     three), ``o`` takes the heads' outputs.  ``table`` (``rotary_table``) None:
-    positions are not rotary.
+    positions are not rotary.  ``q_norm`` and ``k_norm`` (head_dim weights each, or
+    neither): the heads are normed before they are turned (``norm_rotary``); they
+    become parameters.
 
     ``forward`` runs whole packed sequences, for prompts, calibration and
-    training; ``step`` runs new tokens over a ``PagedKVCache``.  Both raise
+    training; ``step`` runs new tokens over a ``PagedKVCache``, a quantised one
+    too.  Both raise
     ValueError where the host knows that a position is past the table: one
     sequence longer than it, a step whose longest context is.  Sequences by
     ``cu_seqlens`` and given positions are not looked at; positions past the
     table are turned by its last angles."""
 
     def __init__(self, qkv: nn.Module, o: nn.Module, heads: int, kv_heads: int, head_dim: int,
-                 table: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None):
+                 table: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None,
+                 q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6):
         super().__init__()
+        if (q_norm is None) != (k_norm is None):
+            raise ValueError("QuantizedAttention: the queries' norm without the keys', or these without those")
+        for w in (q_norm, k_norm):
+            if w is not None and tuple(w.shape) != (head_dim,):
+                raise ValueError(f"QuantizedAttention: a norm of {tuple(w.shape)} weights for heads of {head_dim}")
         if heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise ValueError(f"{heads} query heads over {kv_heads} key heads")
         self.qkv, self.o = qkv, o
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
-        self.interleaved, self.scale = interleaved, scale
+        self.interleaved, self.scale, self.eps = interleaved, scale, eps
+        self.q_norm = None if q_norm is None else nn.Parameter(q_norm.detach().clone())
+        self.k_norm = None if k_norm is None else nn.Parameter(k_norm.detach().clone())
         self.register_buffer("table", table, persistent=False)
 
     def _apply(self, fn, recurse=True):
@@ -322,6 +428,10 @@ class QuantizedAttention(nn.Module):
             if positions is None:
                 positions = (torch.arange(x.shape[0], device=x.device, dtype=torch.int32) if cu_seqlens is None
                              else packed_positions(cu_seqlens, x.shape[0]))
+        if self.q_norm is not None:
+            q, k = norm_rotary(q, k, self.q_norm, self.k_norm, self.table, positions if self.table is not None else None,
+                               self.interleaved, self.eps)
+        elif self.table is not None:
             q, k = rotary(q, k, self.table, positions, self.interleaved)
         y = attention(q, k, v, cu_seqlens, scale=self.scale)
         return self.o(y.flatten(-2))
@@ -333,7 +443,9 @@ class QuantizedAttention(nn.Module):
         self._check_length(batch.max_context)
         q, k, v = self._heads(x)
         kc, vc = cache.k[layer], cache.v[layer]
-        q = rotary_append(q, k, v, self.table, batch.positions, kc, vc, batch.slots, self.interleaved)
+        scales = cache.scales(layer)
+        norms = {} if self.q_norm is None else {"q_weight": self.q_norm, "k_weight": self.k_norm, "eps": self.eps}
+        q = rotary_append(q, k, v, self.table, batch.positions, kc, vc, batch.slots, self.interleaved, **scales, **norms)
         y = paged_attention(q, kc, vc, batch.block_table, batch.context_lens, batch.cu_seqlens, self.scale,
-                            batch.max_context)
+                            batch.max_context, **scales)
         return self.o(y.flatten(-2))

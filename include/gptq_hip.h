@@ -37,6 +37,14 @@ typedef enum {
 
 typedef enum { GPTQ_F32 = 0, GPTQ_F16 = 1, GPTQ_BF16 = 2 } gptq_dtype;
 
+/* What a paged cache holds: values, or codes of 8 bits and a fp32 scale for each
+ * row of one token and key head. */
+typedef enum {
+  GPTQ_CODE_NONE = 0,
+  GPTQ_CODE_I8 = 1,  /* whole numbers -127 .. 127                            */
+  GPTQ_CODE_E4M3 = 2 /* 4 exponent and 3 mantissa bits, up to 448 (no infinity) */
+} gptq_code;
+
 /* Message describing the last error returned on this thread ("" if none). */
 const char* gptq_last_error(void);
 /* ABI version of this header (bumped on incompatible change). */
@@ -451,6 +459,105 @@ int gptq_rotary_append(const void* q, const void* k, const void* v, int dtype,
                        int64_t k_page, int64_t kc_token, int64_t kc_head,
                        void* v_cache, int64_t v_page, int64_t vc_token,
                        int64_t vc_head, gptq_stream_t stream);
+
+/* ------------------------------------------------- norms with the rotation --
+ * y = R(positions[t]) (w x r), r = (mean x^2 + eps)^-1/2, for each head x of a
+ * token: its values over their root mean square, times the head's weights w
+ * (one weight a value, the same for all heads of the queries, or of the keys),
+ * then turned as gptq_rotary turns (table NULL: not turned).  fp32, fp16 or bf16,
+ * computed in fp32 and rounded once; weights of any of these types.  eps: within
+ * [1e-12, 1].  D a multiple of 8 up to 256, rotary_dim of 4; rows, weights and
+ * the table 16-byte aligned, strides multiples of 8.  q_out and k_out contiguous,
+ * not overlapping the inputs.  No counterpart in the reference. */
+int gptq_norm_rotary(const void* q, const void* k, int dtype, int64_t q_token,
+                     int64_t q_head, int64_t k_token, int64_t k_head,
+                     const void* q_weight, const void* k_weight,
+                     int weight_dtype, float eps, const float* table,
+                     int64_t table_rows, int64_t rotary_dim,
+                     const int32_t* positions, int interleaved, int64_t T,
+                     int64_t H, int64_t Hk, int64_t D, void* q_out,
+                     void* k_out, gptq_stream_t stream);
+
+/* Its gradients from those of the outputs: dq and dk contiguous; dq_weight and
+ * dk_weight (both or neither) in weight_dtype, fp32 sums over all tokens and
+ * heads in an order that depends on the sizes only, zeros for T = 0.  The
+ * workspace is for the weights' sums. */
+size_t gptq_norm_rotary_backward_workspace_size(int64_t T, int64_t H,
+                                                int64_t Hk, int64_t D);
+int gptq_norm_rotary_backward(
+    const void* grad_q, const void* grad_k, const void* q, const void* k,
+    int dtype, int64_t gq_token, int64_t gq_head, int64_t gk_token,
+    int64_t gk_head, int64_t q_token, int64_t q_head, int64_t k_token,
+    int64_t k_head, const void* q_weight, const void* k_weight,
+    int weight_dtype, float eps, const float* table, int64_t table_rows,
+    int64_t rotary_dim, const int32_t* positions, int interleaved, int64_t T,
+    int64_t H, int64_t Hk, int64_t D, void* dq, void* dk, void* dq_weight,
+    void* dk_weight, void* workspace, size_t workspace_bytes,
+    gptq_stream_t stream);
+
+/* gptq_rotary_append with the norms (weights NULL: none), into a cache of the
+ * inputs' type or of codes.  A row x of a token's key or value head is quantised
+ * from its fp32 values: scale = max|x| / top (at most the largest that gives a
+ * number for the last code), code = x (top / max|x|) rounded to the
+ * nearest (ties to even), top 127 or 448; a row whose largest value is not above
+ * 2^-120 has scale and codes 0, one with a value that is not finite has the scale
+ * NaN and codes 0.  Codes and scales have the strides (elements) of a page, a
+ * token and a head; those of codes are multiples of 16, D too, rotary_dim of 8. */
+int gptq_norm_rotary_append(
+    const void* q, const void* k, const void* v, int dtype, int64_t q_token,
+    int64_t q_head, int64_t k_token, int64_t k_head, int64_t v_token,
+    int64_t v_head, const void* q_weight, const void* k_weight,
+    int weight_dtype, float eps, const float* table, int64_t table_rows,
+    int64_t rotary_dim, const int32_t* positions, int interleaved,
+    const int32_t* slots, int64_t page_size, int64_t pages, int64_t T,
+    int64_t H, int64_t Hk, int64_t D, void* q_out, int code, void* k_cache,
+    int64_t k_page, int64_t kc_token, int64_t kc_head, void* v_cache,
+    int64_t v_page, int64_t vc_token, int64_t vc_head, float* k_scale,
+    int64_t ks_page, int64_t ks_token, int64_t ks_head, float* v_scale,
+    int64_t vs_page, int64_t vs_token, int64_t vs_head, gptq_stream_t stream);
+
+/* --------------------------------------------------------- rows of a cache --
+ * The last cu_rows[b + 1] - cu_rows[b] cached tokens of each sequence as packed
+ * rows k_out and v_out (T, Hk, D), contiguous: copied (code NONE; out_dtype is
+ * the cache's type), or code * scale in fp32, rounded once to out_dtype.  Rows
+ * that a sequence does not have, and rows behind the last sequence, are zeros.
+ * Rows of the cache are whole 16s of bytes, 16-byte aligned.  Device arrays out
+ * of range are clamped as in gptq_paged_attention.  No counterpart in the
+ * reference. */
+int gptq_cached_rows(int code, const void* k_cache, int64_t k_page,
+                     int64_t k_token, int64_t k_head, const void* v_cache,
+                     int64_t v_page, int64_t v_token, int64_t v_head,
+                     const float* k_scale, int64_t ks_page, int64_t ks_token,
+                     int64_t ks_head, const float* v_scale, int64_t vs_page,
+                     int64_t vs_token, int64_t vs_head,
+                     const int32_t* block_table, int64_t table_stride,
+                     int64_t width, int64_t page_size, int64_t pages,
+                     const int32_t* context, const int32_t* cu_rows, int64_t B,
+                     int64_t T, int64_t Hk, int64_t D, void* k_out,
+                     void* v_out, int out_dtype, gptq_stream_t stream);
+
+/* gptq_paged_attention over a cache of codes: key j stands for ks_j kc_j and its
+ * value for vs_j vc_j.  D a multiple of 16; strides of codes too.  Products are of
+ * the codes as they are and of the queries; a weight times its value's scale is
+ * rounded to the queries' type (for few rows to twice its bits) relative to the
+ * largest scale so far.  Codes are numbers (not e4m3's NaN); a row that is not
+ * finite has a scale that is NaN, which reaches only the queries that see it.
+ * Workspace: as for gptq_paged_attention. */
+int gptq_code_attention(const void* q, int dtype, int64_t q_token,
+                        int64_t q_head, int code, const void* k_cache,
+                        int64_t k_page, int64_t k_token, int64_t k_head,
+                        const void* v_cache, int64_t v_page, int64_t v_token,
+                        int64_t v_head, const float* k_scale, int64_t ks_page,
+                        int64_t ks_token, int64_t ks_head,
+                        const float* v_scale, int64_t vs_page,
+                        int64_t vs_token, int64_t vs_head,
+                        const int32_t* block_table, int64_t table_stride,
+                        int64_t width, int64_t page_size, int64_t pages,
+                        const int32_t* context, const int32_t* cu_q, int64_t B,
+                        int64_t T, int64_t H, int64_t Hk, int64_t D,
+                        float scale, int64_t max_context, void* out,
+                        void* workspace, size_t workspace_bytes,
+                        gptq_stream_t stream);
 
 /* ------------------------------------------------------- measurement aid --
  * No counterpart in the reference: a read-only streaming kernel for the
