@@ -91,6 +91,7 @@ SIGNATURES = {
                                 + [_i64] * 6 + [_p, _i] + ([_p] + [_i64] * 3) * 4 + [_p]),
     "gptq_cached_rows": (_i, [_i] + ([_p] + [_i64] * 3) * 4 + [_p] + [_i64] * 4 + [_p, _p] + [_i64] * 4
                          + [_p, _p, _i, _p]),
+    "gptq_code_attention_workspace_size": (_sz, [_i64] * 6),
     "gptq_code_attention": (_i, [_p, _i, _i64, _i64, _i] + ([_p] + [_i64] * 3) * 4 + [_p] + [_i64] * 4 + [_p, _p]
                             + [_i64] * 5 + [_f, _i64, _p, _p, _sz, _p]),
     "gptq_stream_read": (_i, [_p, _sz, _i, _i, _p, _p]),

@@ -36,51 +36,42 @@ constexpr float kBias = kBF16 ? 0.0f : 7.0f;
 template <bool kBF16>
 constexpr int kScaleRoom = kBF16 ? 24 : 0;
 
-template <int DT>
-struct CodeColumn {
-  float m, l;       // the running maximum, and this lane's part of the sum of weights
-  f32x16 o[DT / 32];
-  float down, cap;  // 2^-e, and the largest scale that it allows (the same in the wave's lanes)
+// A wave's e: 2^-e, and the largest scale that it allows.
+struct ScaleRoom {
+  float down = 1.0f, cap = -1.0f;
 };
-
-template <int DT>
-__device__ __forceinline__ void start_column(CodeColumn<DT>& col) {
-  col.m = kLowest;
-  col.l = 0.0f;
-  col.down = 1.0f;
-  col.cap = -1.0f;
-#pragma unroll
-  for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
-}
-
-// Raises e where a tile's scales pass what it allows.  `vs`: a scale of each
-// lane's (0 for none); those that are not finite are no reason.
-template <bool kBF16, int DT>
-__device__ __forceinline__ void allow_scales(CodeColumn<DT>& col, float vs) {
-  if (__builtin_expect(__ballot(vs > col.cap && vs < INFINITY) == 0, 1)) return;
+// `vs`: a scale of each lane's (0 for none); those that are not finite are no
+// reason for another e.
+__device__ __forceinline__ bool lacks_room(const ScaleRoom& r, float vs) { return __ballot(vs > r.cap && vs < INFINITY) != 0; }
+// Raises e; what the sums are multiplied with then.
+template <bool kBF16>
+__device__ __forceinline__ float make_room(ScaleRoom& r, float vs) {
   float top = vs > 0.0f && vs < INFINITY ? vs : 0.0f;
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-  if (top == 0.0f) return;  // (scales of 0 need no e)
-  int e = ilogbf(top) + 1;
-  e = clamp_int(e, -100, 126);
+  if (top == 0.0f) return 1.0f;  // (scales of 0 need no e)
+  const int e = clamp_int(ilogbf(top) + 1, -100, 126);
   const float down = ldexpf(1.0f, -e);
-  const float less = down / col.down;
-  col.down = down;
-  col.cap = ldexpf(1.0f, clamp_int(e + kScaleRoom<kBF16>, -126, 127));
-  if (less == 1.0f) return;
-#pragma unroll
-  for (int db = 0; db < DT / 32; ++db)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
+  const float less = down / r.down;
+  r.down = down;
+  r.cap = ldexpf(1.0f, clamp_int(e + kScaleRoom<kBF16>, -126, 127));
+  return less;
 }
 
-// Adds NK x 32 keys with scores s (scaled, -infinity where not seen) and scales
-// vs (0 where not seen) of their values to the column's sums.  `value` gives the
+template <int DT>
+struct CodeColumn {
+  float m, l;  // the running maximum, and this lane's part of the sum of weights
+  f32x16 o[DT / 32];
+};
+
+// Adds NK x 32 keys with scores s (scaled, -infinity where not seen) to the
+// column's sums.  `scale` gives the scales of the values of keys 32 kt + 8 g + 4
+// (lane / 32) .. + 3; `drop` clears what belongs to keys that the column does not
+// see, where the tile has any (a scale there may be NaN).  `value` gives the
 // operand of value rows 16 ks .. of the tile, channels 32 db ..  kRest: what the
 // rounding of the weights left is multiplied too.
-template <bool kBF16, int DT, int NK, bool kRest, class Value>
-__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], const f32x16 (&vs)[NK], Value&& value) {
+template <bool kBF16, int DT, int NK, bool kRest, class Scale, class Drop, class Value>
+__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float down, Scale&& scale, Drop&& drop, Value&& value) {
   float t = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
@@ -101,12 +92,17 @@ __device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], 
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float p = __builtin_amdgcn_exp2f(s[kt][i] - col.m);
-      sum += p;
-      s[kt][i] = p * vs[kt][i];
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 vs = scale(kt, g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(s[kt][4 * g + e] - col.m);
+        sum += p;
+        s[kt][4 * g + e] = p * (vs[e] * down);
+      }
     }
   col.l += sum;
+  drop(s);
 #pragma unroll
   for (int ks = 0; ks < 2 * NK; ++ks) {
     const u32x4 p = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
@@ -131,8 +127,8 @@ __device__ __forceinline__ void widen16(const u32x4& w, u32x4& lo, u32x4& hi) {
   hi = u32x4{x[4], x[5], x[6], x[7]};
 }
 
-// The row's statistics as a part's: the maximum, and a sum of weights of 1
-// beside values that are divided by theirs already.  A sum that is NaN stays one.
+// A part's statistics of a row, whose sums are divided already: a weight of 1 at
+// the maximum m + log2 l.  Of a sum that is NaN the weight is NaN.
 __device__ __forceinline__ void store_part_stats(const AttnArgs& a, float m, float l, int64_t row, bool none, int split) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.H;
   float* mm = a.part + a.splits * rows * a.D;
@@ -142,56 +138,75 @@ __device__ __forceinline__ void store_part_stats(const AttnArgs& a, float m, flo
 }
 
 // -------------------------------------------------------------- few rows ----
-// A workgroup has up to 32 packed rows (query token and head of one key head) and
-// its 4 waves share the keys, every wave tiles of 32 of its own (t0 + wave, + 4,
-// ...), whose sums are joined at the end.  A lane loads 16-byte pieces of one
-// row: of a key they are operands as they come (the contraction's order is free,
-// the queries are loaded in the same one), a value's go through LDS to be read
-// transposed.  The next tile's loads are in flight while one is used.
+// A workgroup has up to 16 NQ packed rows (query token and head of one key head)
+// and its 4 waves share the keys, every wave tiles of 32 of its own (t0 + wave, +
+// 4, ...), whose sums are joined at the end.  The products are 16 x 16: of a row of
+// 16 keys a lane ends with keys 4 (lane / 16) + i of query lane % 16, and the
+// weights of a tile's two such rows are the next product's operand as they are.
+//
+// A lane loads 16-byte pieces of rows lane % 16 of a tile's halves: of keys they
+// are operands as they come (the contraction's order is free, the queries are
+// loaded in the same one), values go through LDS to be read transposed.  The next
+// tile's loads are in flight while one is used.
 constexpr int kFew = 32;
 
+// 16-byte chunk c of a row of values is at slot c ^ this in LDS: the writes of 16
+// rows' chunks, and the transposing reads of 8 rows by 16 lanes, 32 lanes at a
+// time, meet each bank once.
 template <int DT>
-__device__ __forceinline__ int code_slot(int row) {  // 16-byte chunk c of a row of codes is at slot c ^ this
+__device__ __forceinline__ int code_slot(int row) {
+  const int high = ((row >> 3) ^ (row >> 4)) & 1;
   if constexpr (DT == 128)
-    return ((row >> 3) & 1) << 2 | ((row >> 1) & 1) << 1 | ((row >> 2) & 1);
+    return ((row >> 1) & 3) | high << 2;
   else
-    return (row >> 2) & 3;
+    return ((row >> 2) & 1) | high << 1;
 }
 
-template <int DT>
-struct FewTile {
-  u32x4 k[DT / 32], v[DT / 32];  // chunks 2 j + lane / 32 of row lane % 32
-  float scale;                   // of that row's key (lanes below 32) or value
-};
-
-template <int DT>
-__device__ __forceinline__ void load_few(FewTile<DT>& x, const CodeArgs& c, const Seq& s, int hk, KvAt at, int key0, int lane) {
-  const int half = lane >> 5;
-  const bool in = key0 + (lane & 31) < s.Lk;
-  const uint8_t* kp = c.k.p + at.page * c.k.page + at.at * c.k.token + hk * c.k.head + 16 * half;
-  const uint8_t* vp = c.v.p + at.page * c.v.page + at.at * c.v.token + hk * c.v.head + 16 * half;
-#pragma unroll
-  for (int j = 0; j < DT / 32; ++j) {
-    x.k[j] = x.v[j] = u32x4{0, 0, 0, 0};
-    if (in && 32 * j + 16 * half < c.a.D) {
-      x.k[j] = *reinterpret_cast<const u32x4*>(kp + 32 * j);
-      x.v[j] = *reinterpret_cast<const u32x4*>(vp + 32 * j);
-    }
-  }
-  const CodeRows& r = half ? c.v : c.k;
-  x.scale = in ? r.scale[at.page * r.s_page + at.at * r.s_token + hk * r.s_head] : 0.0f;
+template <bool kBF16>
+__device__ __forceinline__ f32x4 mma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  if constexpr (kBF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// over a column's four lanes, l % 16 alike: in all of them
+__device__ __forceinline__ void both_rows(float v, float& even, float& odd) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  even = __uint_as_float(r[0]);
+  odd = __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float quarter_max(float v) {
+  float a, b;
+  both_rows(v, a, b);
+  return half_max(__builtin_elementwise_maximum(a, b));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  float a, b;
+  both_rows(v, a, b);
+  return half_sum(a + b);
 }
 
-template <int DT>
-__shared__ __attribute__((aligned(1024))) uint8_t g_code_few[4 * DT * 32 * 4];  // the join's, and before it the waves' tiles
+// what tiles past the last one read
+__device__ __attribute__((aligned(16))) const uint32_t g_no_codes[4] = {};
 
-template <bool kBF16, int DT, int kCode>
-__global__ __launch_bounds__(256, 2) void code_few_kernel(CodeArgs c, int slots) {
-  constexpr int R = 32;
+typedef __attribute__((address_space(1))) const u32x4 gbl_u32x4;
+typedef __attribute__((address_space(1))) const float gbl_f32;
+typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
+typedef __attribute__((address_space(3))) const f32x4 lds_cf32x4;
+
+// the join's sums, and before it the waves' tiles of values
+template <int DT, int R>
+__shared__ __attribute__((aligned(1024))) uint8_t g_code_few[4 * DT * R * 4];
+
+// kWhole: pages hold whole 16s of tokens, so that each half of a tile is in one
+// page and its addresses are scalar.
+template <bool kBF16, int DT, int kCode, int NQ, bool kWhole>
+__global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs c, int slots) {
+  constexpr int R = 16 * NQ, NX = DT / 64, NB = DT / 16;
   const AttnArgs& a = c.a;
   __shared__ float stats[3][4][R];
   __shared__ __attribute__((aligned(16))) float scales[4][64];
-  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int hk = blockIdx.x % a.Hk;
   const int rest = blockIdx.x / a.Hk;
@@ -203,12 +218,34 @@ __global__ __launch_bounds__(256, 2) void code_few_kernel(CodeArgs c, int slots)
   const int rows = s.Lq * G;
   if (tile * R >= rows) return;
 
-  const int r = tile * R + (lane & 31);
-  const bool inside = r < rows;
-  const int tok = div_by(inside ? r : rows - 1, a.G);
-  const int head = hk * G + ((inside ? r : rows - 1) - tok * G);
-  const int limit = last_key(a, s, tok);
-  const int full = last_key(a, s, div_by(tile * R, a.G));
+  // this lane's columns: their queries (in LDS where the registers do not suffice)
+  // and the last key that they see
+  constexpr bool kHeld = NQ == 1 || DT == 64;
+  __shared__ __attribute__((aligned(16))) u32x4 queries[kHeld ? 1 : NQ * 2 * NX][64];
+  int limit[NQ];
+  u32x4 q[NQ][2 * NX];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int r = tile * R + 16 * n + row;
+    const bool inside = r < rows;
+    const int tok = div_by(inside ? r : rows - 1, a.G);
+    const int head = hk * G + ((inside ? r : rows - 1) - tok * G);
+    limit[n] = last_key(a, s, tok);
+    const uint16_t* qrow = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh;
+#pragma unroll
+    for (int x = 0; x < 2 * NX; ++x) {
+      const int d = 64 * (x / 2) + 16 * quarter + 8 * (x % 2);
+      q[n][x] = inside && d < a.D ? *reinterpret_cast<const u32x4*>(qrow + d) : u32x4{0, 0, 0, 0};
+      if constexpr (!kHeld)
+        if (wave == x % 4) queries[2 * NX * n + x][lane] = q[n][x];  // (the waves' are the same)
+    }
+  }
+  if constexpr (!kHeld) __syncthreads();
+  auto query = [&](int n, int x) {
+    if constexpr (kHeld) return q[n][x];
+    return queries[2 * NX * n + x][lane];
+  };
+  const int full = last_key(a, s, div_by(tile * R, a.G));  // keys that all rows see
   const int last_r = (tile + 1) * R < rows ? (tile + 1) * R - 1 : rows - 1;
   const int last = last_key(a, s, div_by(last_r, a.G));
   const int end = last < 0 ? 0 : last + 1;
@@ -217,144 +254,284 @@ __global__ __launch_bounds__(256, 2) void code_few_kernel(CodeArgs c, int slots)
   per = per < 4 ? 4 : per;  // (a tile for each wave)
   const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
-  // channels 32 j + 16 half + 8 e .. + 7: the order of a key's pieces
-  u32x4 q[DT / 16];
-  const uint16_t* qrow = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh;
+  float m[NQ], l[NQ];
+  f32x4 o[NQ][NB];
+  ScaleRoom room;
 #pragma unroll
-  for (int j = 0; j < DT / 16; ++j) {
-    const int d = 32 * (j / 2) + 16 * half + 8 * (j % 2);
-    q[j] = inside && d < a.D ? *reinterpret_cast<const u32x4*>(qrow + d) : u32x4{0, 0, 0, 0};
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = kLowest, l[n] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < NB; ++x) o[n][x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  CodeColumn<DT> col;
-  start_column(col);
-
-  uint8_t* const vroom = &g_code_few<DT>[wave * (kFew * DT)];
-  lds_u8* const vt = (lds_u8*)vroom;
+  lds_u8* const vt = (lds_u8*)&g_code_few<DT, R>[wave * (kFew * DT)];
   lds_f32* const sc_lds = (lds_f32*)&scales[wave][0];
-  int put[DT / 32], get[DT / 32];
+  // where a lane's chunks are in a row (one past the head: its first chunk, which
+  // meets zeros of the queries and channels that are not stored), and where they
+  // go; of a row 16 further the slot's high bit is turned
+  uint32_t chunk[NX];
+  int put[NX];
 #pragma unroll
-  for (int j = 0; j < DT / 32; ++j) {
-    const int row = lane & 31;
-    put[j] = row * DT + (((2 * j + half) ^ code_slot<DT>(row)) << 4);
-    // a transposing read takes from 16 lanes the addresses of 8 rows x 16 codes,
-    // 8 codes a lane, and gives lane i the 8 rows' code i: here the rows 8 (i / 8)
-    // + 4 half + (i / 2) % 4 (+ 16 ks, which leaves their slots)
-    const int i = lane & 15;
-    const int from = 8 * (i >> 3) + 4 * half + ((i >> 1) & 3);
-    get[j] = from * DT + (((2 * j + ((lane >> 4) & 1)) ^ code_slot<DT>(from)) << 4) + ((i & 1) << 3);
+  for (int x = 0; x < NX; ++x) {
+    chunk[x] = 64 * x + 16 * quarter;
+    if (chunk[x] >= static_cast<uint32_t>(a.D)) chunk[x] = 0;
+    put[x] = row * DT + (((4 * x + quarter) ^ code_slot<DT>(row)) << 4);
   }
+  constexpr int kTurn = DT == 128 ? 64 : 32;
+  // A transposing read takes from 16 lanes the addresses of 8 rows x 16 codes, 8
+  // codes a lane, and gives lane i the 8 rows' code i: the rows 16 (i / 8) + 4
+  // quarter + (i / 2) % 4 here, chunk 0; chunk c is at the address ^ 16 c.
+  const int from = 16 * (row >> 3) + 4 * quarter + ((row >> 1) & 3);
+  const int get = from * DT + (code_slot<DT>(from) << 4) + ((row & 1) << 3);
 
-  FewTile<DT> now;
-  KvAt at = kv_at_clamped<true>(a, s, (t0 + wave) * kFew + (lane & 31));
-  if (t0 + wave < t1) load_few(now, c, s, hk, at, (t0 + wave) * kFew, lane);
-  at = kv_at_clamped<true>(a, s, (t0 + wave + 4) * kFew + (lane & 31));
-  for (int t = t0 + wave; t < t1; t += 4) {
-    FewTile<DT> next = now;
-    if (t + 4 < t1) {
-      load_few(next, c, s, hk, at, (t + 4) * kFew, lane);
-      at = kv_at_clamped<true>(a, s, (t + 8) * kFew + (lane & 31));
+  // The block table's entries of a tile: of its halves, or of the lane's two rows.
+  // They are loaded a tile before the rows are, and before the rows of the tile
+  // between: loads return in order, so that a wait for an entry does not wait for
+  // rows.
+  auto key_of = [&](int t, int n) {  // a half's first key, or the lane's: one of the sequence in any case
+    if constexpr (kWhole) return clamp_int(t * kFew + 16 * n, 0, (s.Lk - 1) & ~15);
+    return clamp_int(t * kFew + 16 * n + row, 0, s.Lk - 1);
+  };
+  auto page_of = [&](int t, int n) {
+    return a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, n), a.paged.page)];
+  };
+  // A tile's rows.  Every lane loads in any case, of tiles past the last one the
+  // same few bytes: with loads under a branch the compiler waits for all of them
+  // where it could wait for the older ones.
+  auto load = [&](u32x4 (&k)[2][NX], u32x4 (&v)[2][NX], float& scale, int t, const int (&pages)[2]) {
+    const bool some = t < t1;
+    const uint32_t keep = some ? ~0u : 0u;
+    const uint64_t none = reinterpret_cast<uint64_t>(&g_no_codes[0]);
+    int page[2], at[2];
+    uint64_t kp[2], vp[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      const int key = key_of(t, n);
+      at[n] = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+      page[n] = clamp_int(kWhole ? uniform_int(pages[n]) : pages[n], 0, a.paged.pages - 1);
+      kp[n] = reinterpret_cast<uint64_t>(c.k.p) + page[n] * c.k.page + at[n] * c.k.token + hk * c.k.head;
+      vp[n] = reinterpret_cast<uint64_t>(c.v.p) + page[n] * c.v.page + at[n] * c.v.token + hk * c.v.head;
+      kp[n] = some ? kp[n] : none;
+      vp[n] = some ? vp[n] : none;
+      if constexpr (kWhole) kp[n] = uniform_u64(kp[n]), vp[n] = uniform_u64(vp[n]);
     }
+    const uint32_t krow = kWhole ? row * static_cast<uint32_t>(c.k.token) : 0u;
+    const uint32_t vrow = kWhole ? row * static_cast<uint32_t>(c.v.token) : 0u;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int x = 0; x < NX; ++x) k[n][x] = *(gbl_u32x4*)(kp[n] + ((krow + chunk[x]) & keep));
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int x = 0; x < NX; ++x) v[n][x] = *(gbl_u32x4*)(vp[n] + ((vrow + chunk[x]) & keep));
+    // quarters 0 and 1: the keys' scales of the two halves, 2 and 3: the values'
+    const int pg = quarter & 1 ? page[1] : page[0];
+    const int to = (quarter & 1 ? at[1] : at[0]) + (kWhole ? row : 0);
+    const bool values = quarter >= 2;
+    const int64_t i = pg * (values ? c.v.s_page : c.k.s_page) + to * (values ? c.v.s_token : c.k.s_token) +
+                      hk * (values ? c.v.s_head : c.k.s_head);
+    const uint64_t sp = reinterpret_cast<uint64_t>(values ? c.v.scale : c.k.scale) + 4 * i;
+    scale = *(gbl_f32*)(some ? sp : none);
+  };
+  // Uses a tile's rows, and has the next one's loaded into their registers as soon
+  // as these are free: the loads are in flight for the larger part of a tile's time.
+  u32x4 k[2][NX], v[2][NX];
+  float scale;
+  auto use = [&](int t, const int (&next)[2]) {
     const int key0 = t * kFew;
+    if (key0 + kFew > s.Lk) {  // rows past the end hold anything
 #pragma unroll
-    for (int j = 0; j < DT / 32; ++j) *(lds_u32x4*)(vt + put[j]) = now.v[j];
-    sc_lds[lane] = half ? now.scale : now.scale * a.c;
-    allow_scales<kBF16>(col, half ? now.scale : 0.0f);
+      for (int n = 0; n < 2; ++n)
+        if (key0 + 16 * n + row >= s.Lk)
+#pragma unroll
+          for (int x = 0; x < NX; ++x) v[n][x] = u32x4{0, 0, 0, 0};
+      if (key0 + 16 * (quarter & 1) + row >= s.Lk) scale = 0.0f;
+    }
+#pragma unroll
+    for (int x = 0; x < NX; ++x) {
+      *(lds_u32x4*)(vt + put[x]) = v[0][x];
+      *(lds_u32x4*)(vt + (put[x] ^ kTurn) + 16 * DT) = v[1][x];
+    }
+    sc_lds[lane] = quarter >= 2 ? scale : scale * a.c;
+    const float vs = quarter >= 2 ? scale : 0.0f;
+    if (__builtin_expect(lacks_room(room, vs), 0)) {
+      const float less = make_room<kBF16>(room, vs);
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][x][e] *= less;
+    }
 
-    f32x16 sc[1] = {zero16()};
+    f32x4 sc[NQ][2];
 #pragma unroll
-    for (int j = 0; j < DT / 32; ++j) {
-      u32x4 lo, hi;
-      widen16<kBF16, kCode>(now.k[j], lo, hi);
-      sc[0] = mma32<kBF16>(lo, q[2 * j], sc[0]);
-      sc[0] = mma32<kBF16>(hi, q[2 * j + 1], sc[0]);
-    }
-    wave_sync();
-    f32x16 vs[1];
+    for (int n = 0; n < NQ; ++n) sc[n][0] = sc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 ks4 = *(const __attribute__((address_space(3))) f32x4*)(sc_lds + 8 * g + 4 * half);
-      const f32x4 vs4 = *(const __attribute__((address_space(3))) f32x4*)(sc_lds + 32 + 8 * g + 4 * half);
+    for (int x = 0; x < NX; ++x)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[0][4 * g + e] *= ks4[e];
-        vs[0][4 * g + e] = vs4[e] * col.down;
+      for (int y = 0; y < 2; ++y) {
+        u32x4 lo, hi;
+        widen16<kBF16, kCode>(k[y][x], lo, hi);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          sc[n][y] = mma16<kBF16>(lo, query(n, 2 * x), sc[n][y]);
+          sc[n][y] = mma16<kBF16>(hi, query(n, 2 * x + 1), sc[n][y]);
+        }
       }
-    }
-    if (key0 + kFew - 1 > full) {
+    __builtin_amdgcn_sched_barrier(0);
+    load(k, v, scale, t + 4, next);
+    __builtin_amdgcn_sched_barrier(0);
+    wave_sync();
+    f32x4 ks[2], vs4[2];
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (key0 + acc_row(i, half) > limit) sc[0][i] = -INFINITY, vs[0][i] = 0.0f;
+    for (int y = 0; y < 2; ++y) {
+      ks[y] = *(lds_cf32x4*)(sc_lds + 16 * y + 4 * quarter);
+      vs4[y] = *(lds_cf32x4*)(sc_lds + 32 + 16 * y + 4 * quarter);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vs4[y][e] *= room.down;
     }
-    code_step<kBF16, DT, 1, true>(col, sc, vs, [&](int ks, int db) {
+    const bool cut = key0 + kFew - 1 > full;
+    u32x4 p[NQ], pr[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[n][y][e] *= ks[y][e];
+          if (cut && key0 + 16 * y + 4 * quarter + e > limit[n]) sc[n][y][e] = -INFINITY;
+          top = __builtin_elementwise_maximum(top, sc[n][y][e]);
+        }
+      top = quarter_max(top) - kBias<kBF16>;
+      if (__builtin_expect(__ballot(top > m[n] + kSlack) != 0, 0)) {
+        const float now = fmaxf(m[n], top);
+        const float alpha = __builtin_amdgcn_exp2f(m[n] - now);
+        m[n] = now;
+        l[n] *= alpha;
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][x][e] *= alpha;
+      }
+      float w[2][4], left[2][4];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __builtin_amdgcn_exp2f(sc[n][y][e] - m[n]);
+          l[n] += x;
+          w[y][e] = x * vs4[y][e];
+          // (a scale there may be NaN)
+          if (cut && key0 + 16 * y + 4 * quarter + e > limit[n]) w[y][e] = 0.0f;
+        }
+      p[n] = u32x4{pack16<kBF16>(w[0][0], w[0][1]), pack16<kBF16>(w[0][2], w[0][3]), pack16<kBF16>(w[1][0], w[1][1]),
+                   pack16<kBF16>(w[1][2], w[1][3])};
+      // what the rounding of the weights left is multiplied too: the cache's bytes
+      // take longer than both products
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          left[y][e] = w[y][e] - value16<kBF16>(static_cast<uint16_t>(p[n][2 * y + e / 2] >> (16 * (e % 2))));
+      pr[n] = u32x4{pack16<kBF16>(left[0][0], left[0][1]), pack16<kBF16>(left[0][2], left[0][3]),
+                    pack16<kBF16>(left[1][0], left[1][1]), pack16<kBF16>(left[1][2], left[1][3])};
+    }
+#pragma unroll
+    for (int x = 0; x < NB; ++x) {
       typedef int i32x2 __attribute__((ext_vector_type(2)));
       typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
-      const i32x2 w = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(vt + get[db] + 16 * ks * DT));
-      u32x4 v;
-      uint32_t x[4];
-      widen4<kBF16, kCode>(static_cast<uint32_t>(w[0]), x[0], x[1]);
-      widen4<kBF16, kCode>(static_cast<uint32_t>(w[1]), x[2], x[3]);
-      v = u32x4{x[0], x[1], x[2], x[3]};
-      return v;
-    });
+      const i32x2 z = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2*)(vt + (get ^ (x << 4))));
+      uint32_t y[4];
+      widen4<kBF16, kCode>(static_cast<uint32_t>(z[0]), y[0], y[1]);
+      widen4<kBF16, kCode>(static_cast<uint32_t>(z[1]), y[2], y[3]);
+      const u32x4 value = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        o[n][x] = mma16<kBF16>(value, p[n], o[n][x]);
+        o[n][x] = mma16<kBF16>(value, pr[n], o[n][x]);
+      }
+    }
     wait_lgkm<0>();  // (this tile's reads, before the next one's writes)
     wave_sync();
-    now = next;
+  };
+  const int first = t0 + wave;
+  if (first < t1) {
+    int p0[2] = {page_of(first, 0), page_of(first, 1)}, p1[2] = {page_of(first + 4, 0), page_of(first + 4, 1)};
+    load(k, v, scale, first, p0);
+    for (int t = first; t < t1; t += 4) {
+      p0[0] = p1[0], p0[1] = p1[1];
+      p1[0] = page_of(t + 8, 0), p1[1] = page_of(t + 8, 1);
+      use(t, p0);
+    }
   }
-  const float l1 = half_sum(col.l);
-  if (half == 0) {
-    stats[0][wave][lane] = col.m;
-    stats[1][wave][lane] = l1;
-    stats[2][wave][lane] = col.down;
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    l[n] = quarter_sum(l[n]);
+    if (quarter == 0) {
+      stats[0][wave][16 * n + row] = m[n];
+      stats[1][wave][16 * n + row] = l[n];
+      stats[2][wave][16 * n + row] = room.down;
+    }
   }
   __syncthreads();
 
   // joined: the waves' sums at the largest maximum and the smallest 2^-e.  Wave
-  // w's channels d .. d + 3 of column x are at chunk (d / 4) ^ (x % (DT / 4)) of row
-  // (w, x), so that neither side's accesses meet in a bank.
-  const int x = lane & 31;
-  float m = stats[0][0][x], down = stats[2][0][x];
+  // w's channels 4 d .. 4 d + 3 of column x are at chunk d ^ (x % (DT / 4)) of row
+  // (w, x): neither side's accesses meet in a bank.
+  lds_u8* const sums = (lds_u8*)&g_code_few<DT, R>[0];
+  auto sum_at = [&](int w, int x, int d) { return ((w * R + x) * (DT / 4) + (d ^ (x & (DT / 4 - 1)))) * 16; };
+  auto joined = [&](int x, float& top, float& down) {
+    top = stats[0][0][x], down = stats[2][0][x];
 #pragma unroll
-  for (int w = 1; w < 4; ++w) m = fmaxf(m, stats[0][w][x]), down = fminf(down, stats[2][w][x]);
-  float l = 0.0f;
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, stats[0][w][x]), down = fminf(down, stats[2][w][x]);
+  };
 #pragma unroll
-  for (int w = 0; w < 4; ++w) l += stats[1][w][x] * exp2f(stats[0][w][x] - m);
-  lds_u8* const sums = (lds_u8*)&g_code_few<DT>[0];
-  auto chunk = [&](int w, int d4) { return ((w * 32 + x) * (DT / 4) + (d4 ^ (x & (DT / 4 - 1)))) * 16; };
-  typedef __attribute__((address_space(3))) f32x4 lds_f32x4;
-  if (inside) {
-    const float scale = exp2f(col.m - m) * (down / col.down);
+  for (int n = 0; n < NQ; ++n) {
+    const int x = 16 * n + row;
+    if (tile * R + x >= rows) continue;
+    float top, down;
+    joined(x, top, down);
+    const float f = exp2f(m[n] - top) * (down / room.down);
 #pragma unroll
-    for (int db = 0; db < DT / 32; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; i += 4)
-        *(lds_f32x4*)(sums + chunk(wave, (32 * db + acc_row(i, half)) / 4)) =
-            f32x4{col.o[db][i] * scale, col.o[db][i + 1] * scale, col.o[db][i + 2] * scale, col.o[db][i + 3] * scale};
+    for (int d = 0; d < NB; ++d)
+      *(lds_f32x4*)(sums + sum_at(wave, x, 4 * d + quarter)) =
+          f32x4{o[n][d][0] * f, o[n][d][1] * f, o[n][d][2] * f, o[n][d][3] * f};
   }
   __syncthreads();
-  if (!inside) return;
 
+  const int x = threadIdx.x % R;
+  const int r = tile * R + x;
+  if (r >= rows) return;
+  const int tok = div_by(r, a.G);
+  float top, down, sum = 0.0f;
+  joined(x, top, down);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) sum += stats[1][w][x] * exp2f(stats[0][w][x] - top);
+  const int seen = last_key(a, s, tok) + 1;
   const int k0 = t0 * kFew;
-  const int k1 = t1 * kFew < limit + 1 ? t1 * kFew : limit + 1;
+  const int k1 = t1 * kFew < seen ? t1 * kFew : seen;
   const bool none = k1 <= k0;
-  const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
-  constexpr int N = DT / 8;  // channels of a thread
-  const int d0 = (threadIdx.x >> 5) * N;
-  if (threadIdx.x < R && a.splits > 1) store_part_stats(a, m, l, row, none, split);
-  const float rl = none ? 0.0f : 1.0f / l;
+  const int64_t out_row = static_cast<int64_t>(s.q0 + tok) * a.H + hk * G + (r - tok * G);
+  constexpr int N = DT * R / 256;  // channels of a thread
+  const int d0 = (threadIdx.x / R) * N;
+  if (threadIdx.x < R && a.splits > 1) store_part_stats(a, top, sum, out_row, none, split);
+  const float inv = none ? 0.0f : 1.0f / sum;
   const float up = 1.0f / down;
 #pragma unroll
   for (int d = 0; d < N; d += 4) {
     if (d0 + d >= a.D) break;
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) y += *(const lds_f32x4*)(sums + chunk(w, (d0 + d) / 4));
+    for (int w = 0; w < 4; ++w) y += *(lds_cf32x4*)(sums + sum_at(w, x, (d0 + d) / 4));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : y[e] * rl * up;
+    for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : y[e] * inv * up;
     if (a.splits > 1)
-      *reinterpret_cast<f32x4*>(a.part + (split * (static_cast<int64_t>(a.T) * a.H) + row) * a.D + d0 + d) = y;
+      *reinterpret_cast<f32x4*>(a.part + (split * (static_cast<int64_t>(a.T) * a.H) + out_row) * a.D + d0 + d) = y;
     else
-      *reinterpret_cast<u32x2*>(a.out + row * a.D + d0 + d) = u32x2{pack16<kBF16>(y[0], y[1]), pack16<kBF16>(y[2], y[3])};
+      *reinterpret_cast<u32x2*>(a.out + out_row * a.D + d0 + d) = u32x2{pack16<kBF16>(y[0], y[1]), pack16<kBF16>(y[2], y[3])};
   }
 }
 
@@ -417,7 +594,11 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   }
 
   CodeColumn<DT> col;
-  start_column(col);
+  ScaleRoom room;
+  col.m = kLowest;
+  col.l = 0.0f;
+#pragma unroll
+  for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
 
   // this thread's chunk of rows row0, row0 + RPI, ..; and one of the tile's scales
   const int ch = threadIdx.x % Tile::CH, row0 = threadIdx.x / Tile::CH;
@@ -468,8 +649,14 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     if (key0 >= wave_end) return;
     const lds_u8 *kt = (const lds_u8*)&g_code_k<DT>[buf][0], *vt = (const lds_u8*)&g_code_v<DT>[buf][0];
     const lds_f32* sl = (const lds_f32*)&scales[buf][0];
-    allow_scales<kBF16>(col, sl[kKeys + lane]);
-    f32x16 sc[2] = {zero16(), zero16()}, vs[2];
+    if (__builtin_expect(lacks_room(room, sl[kKeys + lane]), 0)) {
+      const float less = make_room<kBF16>(room, sl[kKeys + lane]);
+#pragma unroll
+      for (int db = 0; db < DT / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
+    }
+    f32x16 sc[2] = {zero16(), zero16()};
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
@@ -478,23 +665,25 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        typedef __attribute__((address_space(3))) const f32x4 lds_cf32x4;
         const f32x4 ks4 = *(lds_cf32x4*)(sl + 32 * n + 8 * g + 4 * half);
-        const f32x4 vs4 = *(lds_cf32x4*)(sl + kKeys + 32 * n + 8 * g + 4 * half);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[n][4 * g + e] *= ks4[e];
-          vs[n][4 * g + e] = vs4[e] * col.down;
-        }
+        for (int e = 0; e < 4; ++e) sc[n][4 * g + e] *= ks4[e];
       }
-    if (key0 + kKeys - 1 > full) {
+    const bool cut = key0 + kKeys - 1 > full;
+    auto mask = [&](float with) {
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = -INFINITY, vs[n][i] = 0.0f;
-    }
-    code_step<kBF16, DT, 2, false>(col, sc, vs, [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
+          if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = with;
+    };
+    if (cut) mask(-INFINITY);
+    code_step<kBF16, DT, 2, false>(
+        col, sc, room.down, [&](int kt, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt + 8 * g + 4 * half); },
+        [&](f32x16 (&)[2]) {
+          if (cut) mask(0.0f);
+        },
+        [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
   };
 
   if (t0 < t1) {
@@ -520,7 +709,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   if (!inside) return;
   if (half == 0 && a.splits > 1) store_part_stats(a, col.m, l, row, none, split);
   const float rl = none ? 0.0f : 1.0f / l;
-  const float up = 1.0f / col.down;
+  const float up = 1.0f / room.down;
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
@@ -537,15 +726,24 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     }
 }
 
+template <bool kBF16, int DT, int kCode, int NQ>
+void launch_few(const CodeArgs& c, uint32_t grid, int slots, hipStream_t st) {
+  if (c.a.paged.whole)
+    code_few_kernel<kBF16, DT, kCode, NQ, true><<<grid, 256, 0, st>>>(c, slots);
+  else
+    code_few_kernel<kBF16, DT, kCode, NQ, false><<<grid, 256, 0, st>>>(c, slots);
+}
 template <bool kBF16, int DT, int kCode>
-int launch(const CodeArgs& c, bool few, hipStream_t st) {
+int launch(const CodeArgs& c, int R, hipStream_t st) {
   const AttnArgs& a = c.a;
-  const int64_t slots = slots_of(a.cu_q, a.B, a.T, a.G.d, few ? 32 : 128);
+  const int64_t slots = slots_of(a.cu_q, a.B, a.T, a.G.d, R);
   const int64_t grid = slots * a.Hk * a.splits;
   GPTQ_REQUIRE(grid < (int64_t{1} << 31), GPTQ_ERR_SHAPE, "attention: too many rows (%lld workgroups)",
                static_cast<long long>(grid));
-  if (few)
-    code_few_kernel<kBF16, DT, kCode><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
+  if (R == 16)
+    launch_few<kBF16, DT, kCode, 1>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
+  else if (R == 32)
+    launch_few<kBF16, DT, kCode, 2>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
   else
     code_rows_kernel<kBF16, DT, kCode><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
   const int rc = check_launch("attention");
@@ -553,14 +751,19 @@ int launch(const CodeArgs& c, bool few, hipStream_t st) {
   return launch_join<kBF16>(a, st);
 }
 template <bool kBF16, int DT>
-int launch_code(const CodeArgs& c, int code, bool few, hipStream_t st) {
-  return code == GPTQ_CODE_I8 ? launch<kBF16, DT, GPTQ_CODE_I8>(c, few, st) : launch<kBF16, DT, GPTQ_CODE_E4M3>(c, few, st);
+int launch_code(const CodeArgs& c, int code, int R, hipStream_t st) {
+  return code == GPTQ_CODE_I8 ? launch<kBF16, DT, GPTQ_CODE_I8>(c, R, st) : launch<kBF16, DT, GPTQ_CODE_E4M3>(c, R, st);
 }
 
 }  // namespace
 }  // namespace gptq
 
 using namespace gptq;
+
+extern "C" size_t gptq_code_attention_workspace_size(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
+                                                     int64_t max_context) {
+  return plan::code_workspace(B, T, H, Hk, D, max_context);
+}
 
 extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, int64_t q_head, int code, const void* k_cache,
                                    int64_t k_page, int64_t k_token, int64_t k_head, const void* v_cache, int64_t v_page,
@@ -591,8 +794,11 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   for (int64_t x : code_strides)
     GPTQ_REQUIRE(x >= 0 && x % 16 == 0, GPTQ_ERR_SHAPE, "%s: strides of codes have to be multiples of 16 (got %lld)", fn,
                  static_cast<long long>(x));
-  const plan::PagedPlan p = plan::paged_plan(B, T, H, Hk, max_context);
-  const size_t need = plan::paged_workspace(B, T, H, Hk, D, max_context);
+  for (int64_t x : {k_token, v_token})  // (16 tokens' offsets are 32 bits)
+    GPTQ_REQUIRE(x < (int64_t{1} << 27), GPTQ_ERR_SHAPE, "%s: tokens of codes have to be less than 2^27 apart (got %lld)", fn,
+                 static_cast<long long>(x));
+  const plan::CodePlan p = plan::code_plan(B, T, H, Hk, max_context);
+  const size_t need = plan::code_workspace(B, T, H, Hk, D, max_context);
   GPTQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), GPTQ_ERR_WORKSPACE,
                "%s: workspace of %zu bytes, needs %zu", fn, workspace_bytes, need);
   CodeArgs c{};
@@ -606,6 +812,7 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   a.paged.most = static_cast<int>(plan::cached_most(width, page_size));
   a.paged.pages = static_cast<int>(pages);
   a.paged.page = fast_div(static_cast<uint32_t>(page_size));
+  a.paged.whole = page_size % 16 == 0;
   a.cu_q = cu_q;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T);
   a.H = static_cast<int>(H), a.Hk = static_cast<int>(Hk), a.D = static_cast<int>(D);
@@ -618,6 +825,6 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   const hipStream_t st = as_hip(stream);
   const bool wide = D > 64;
   if (dtype == GPTQ_BF16)
-    return wide ? launch_code<true, 128>(c, code, p.few, st) : launch_code<true, 64>(c, code, p.few, st);
-  return wide ? launch_code<false, 128>(c, code, p.few, st) : launch_code<false, 64>(c, code, p.few, st);
+    return wide ? launch_code<true, 128>(c, code, p.rows, st) : launch_code<true, 64>(c, code, p.rows, st);
+  return wide ? launch_code<false, 128>(c, code, p.rows, st) : launch_code<false, 64>(c, code, p.rows, st);
 }

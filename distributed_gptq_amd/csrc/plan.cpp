@@ -289,6 +289,25 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
   return mul_sat(mul_sat(static_cast<size_t>(T * H), static_cast<size_t>(D + 2)), 4 * static_cast<size_t>(p.splits));
 }
 
+CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context) {
+  CodePlan p;
+  if (T == 0 || !attention_sizes(B, T, 0, H, Hk, 8)) return p;
+  const int64_t rows = ceil_div(T * (H / Hk), B);  // of a sequence and key head, on average
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+  const int64_t groups = ceil_div(rows, p.rows) * B * Hk;
+  const int64_t want = p.rows == 128 ? 512 : B == 1 ? 512 : 1024;  // workgroups
+  const int64_t most = ceil_div(std::max<int64_t>(max_context, 1), p.rows == 128 ? 512 : 128);
+  p.splits = static_cast<int>(std::min<int64_t>({ceil_div(want, groups), most, 128}));
+  return p;
+}
+
+size_t code_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context) {
+  if (!attention_sizes(B, T, 0, H, Hk, D)) return 0;
+  const CodePlan p = code_plan(B, T, H, Hk, max_context);
+  if (p.splits == 1) return 0;
+  return mul_sat(mul_sat(static_cast<size_t>(T * H), static_cast<size_t>(D + 2)), 4 * static_cast<size_t>(p.splits));
+}
+
 // Workgroups of 64 keys, two to a CU: fewer than 1024 are cut until there are as
 // many, because those of the first keys run twice as long as the average and
 // hold up the end.  Measured (2 x 2048 tokens, 8 key heads, 528 workgroups, us of

@@ -508,7 +508,7 @@ at::Tensor code_attention(const at::Tensor& q_, const at::Tensor& k_cache, const
   at::Tensor cq;
   if (cu_q) cq = int32_of(*cu_q, q, "cu_seqlens");
   const int64_t Hk = k_cache.size(2);
-  const size_t bytes = gptq_paged_attention_workspace_size(B, T, H, Hk, D, max_context);
+  const size_t bytes = gptq_code_attention_workspace_size(B, T, H, Hk, D, max_context);
   at::Tensor ws;
   if (bytes) ws = at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte));
   GPTQ_CALL(gptq_code_attention, q.const_data_ptr(), dtype_code(q.scalar_type()), stride_of(q, 0), stride_of(q, 1), code,

@@ -542,7 +542,10 @@ int gptq_cached_rows(int code, const void* k_cache, int64_t k_page,
  * rounded to the queries' type (for few rows to twice its bits) relative to the
  * largest scale so far.  Codes are numbers (not e4m3's NaN); a row that is not
  * finite has a scale that is NaN, which reaches only the queries that see it.
- * Workspace: as for gptq_paged_attention. */
+ * Tokens of codes are less than 2^27 bytes apart. */
+size_t gptq_code_attention_workspace_size(int64_t B, int64_t T, int64_t H,
+                                          int64_t Hk, int64_t D,
+                                          int64_t max_context);
 int gptq_code_attention(const void* q, int dtype, int64_t q_token,
                         int64_t q_head, int code, const void* k_cache,
                         int64_t k_page, int64_t k_token, int64_t k_head,

@@ -417,7 +417,7 @@ def test_nothing_outside_is_touched(H, Hk, D, page, code):
         _lib.call("gptq_cached_rows", code, ptr(kc), *cs, ptr(vc), *cs, ptr(ks), *ss, ptr(vs), *ss, ptr(table), width, width,
                   page, pages, ptr(ctx), ptr(cu), 2, T, Hk, D, ptr(ko), ptr(vo), 1, stream)
         if code:
-            n = _lib.lib().gptq_paged_attention_workspace_size(2, T, H, Hk, D, longest)
+            n = _lib.lib().gptq_code_attention_workspace_size(2, T, H, Hk, D, longest)
             ws = room.empty(max(n, 1), dtype=torch.uint8).zero_()
             _lib.call("gptq_code_attention", ptr(q), 1, *strides(q), code, ptr(kc), *cs, ptr(vc), *cs, ptr(ks), *ss, ptr(vs), *ss,
                       ptr(table), width, width, page, pages, ptr(ctx), ptr(cu), 2, T, H, Hk, D, 0.1, longest, ptr(out),
