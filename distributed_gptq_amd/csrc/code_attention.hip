@@ -7,8 +7,9 @@
 // into the weights.  The weights times scales are rounded to the queries' type;
 // their unrounded sum divides.
 //
-// The scales are taken relative to 2^e, with e a wave's own: the sums of values
-// of any size then stay inside fp32, and fp16 weights inside their 16 bits.
+// Both sums are kept 2^-e as large, with e a wave's own that follows the scales: it
+// is added to m, and leaves the quotient.  The sums of values of any size then stay
+// inside fp32, and fp16 weights inside their 16 bits.
 #include "attn_join.hpp"
 #include "attn_tile.hpp"
 #include "codes.hpp"
@@ -32,52 +33,56 @@ struct CodeArgs {
 constexpr float kSlack = 8.0f;
 template <bool kBF16>
 constexpr float kBias = kBF16 ? 0.0f : 7.0f;
-// how far a scale may pass 2^e before e is raised
+// how far a scale may pass 2^e before e is raised, and the largest e: fp32 ends at
+// 2^-126, and 2^-26 of the largest weight is still above it (in fp16, whose outputs
+// end at 2^16, scales of more than 2^100 need not be exact)
 template <bool kBF16>
 constexpr int kScaleRoom = kBF16 ? 24 : 0;
+template <bool kBF16>
+constexpr int kMostE = kBF16 ? 100 : 120;
+constexpr int kLeastE = -80;  // (2^31 weights of 2^(kSlack + 7 + 80) are inside fp32)
 
-// A wave's e: 2^-e, and the largest scale that it allows.
+// A wave's e, and the largest scale that it allows.
 struct ScaleRoom {
-  float down = 1.0f, cap = -1.0f;
+  float e = 0.0f, cap = -1.0f;
 };
 // `vs`: a scale of each lane's (0 for none); those that are not finite are no
 // reason for another e.
 __device__ __forceinline__ bool lacks_room(const ScaleRoom& r, float vs) { return __ballot(vs > r.cap && vs < INFINITY) != 0; }
-// Raises e; what the sums are multiplied with then.
+// Raises e, by how much it returns.
 template <bool kBF16>
 __device__ __forceinline__ float make_room(ScaleRoom& r, float vs) {
   float top = vs > 0.0f && vs < INFINITY ? vs : 0.0f;
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-  if (top == 0.0f) return 1.0f;  // (scales of 0 need no e)
-  const int e = clamp_int(ilogbf(top) + 1, -100, 126);
-  const float down = ldexpf(1.0f, -e);
-  const float less = down / r.down;
-  r.down = down;
-  r.cap = ldexpf(1.0f, clamp_int(e + kScaleRoom<kBF16>, -126, 127));
-  return less;
+  if (top == 0.0f) return 0.0f;  // (scales of 0 need no e)
+  const int e = clamp_int(ilogbf(top) + 1, kLeastE, kMostE<kBF16>);
+  const float more = static_cast<float>(e) - r.e;
+  r.e = static_cast<float>(e);
+  r.cap = e == kMostE<kBF16> ? INFINITY : ldexpf(1.0f, e + kScaleRoom<kBF16>);
+  return more;
 }
 
 template <int DT>
 struct CodeColumn {
-  float m, l;  // the running maximum, and this lane's part of the sum of weights
+  float m, l;  // the running maximum and e, and this lane's part of the sum of weights
   f32x16 o[DT / 32];
 };
 
 // Adds NK x 32 keys with scores s (scaled, -infinity where not seen) to the
-// column's sums.  `scale` gives the scales of the values of keys 32 kt + 8 g + 4
+// column's sums; `ahead` is e less kBias.  `scale` gives the scales of the values of keys 32 kt + 8 g + 4
 // (lane / 32) .. + 3; `drop` clears what belongs to keys that the column does not
 // see, where the tile has any (a scale there may be NaN).  `value` gives the
 // operand of value rows 16 ks .. of the tile, channels 32 db ..  kRest: what the
 // rounding of the weights left is multiplied too.
 template <bool kBF16, int DT, int NK, bool kRest, class Scale, class Drop, class Value>
-__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float down, Scale&& scale, Drop&& drop, Value&& value) {
+__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, Scale&& scale, Drop&& drop, Value&& value) {
   float t = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);
-  t = half_max(t) - kBias<kBF16>;
+  t = half_max(t) + ahead;
   if (__builtin_expect(__ballot(t > col.m + kSlack) != 0, 0)) {
     const float m = fmaxf(col.m, t);
     const float alpha = __builtin_amdgcn_exp2f(col.m - m);
@@ -98,7 +103,7 @@ __device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], 
       for (int e = 0; e < 4; ++e) {
         const float p = __builtin_amdgcn_exp2f(s[kt][4 * g + e] - col.m);
         sum += p;
-        s[kt][4 * g + e] = p * (vs[e] * down);
+        s[kt][4 * g + e] = p * vs[e];
       }
     }
   col.l += sum;
@@ -204,7 +209,7 @@ template <bool kBF16, int DT, int kCode, int NQ, bool kWhole>
 __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs c, int slots) {
   constexpr int R = 16 * NQ, NX = DT / 64, NB = DT / 16;
   const AttnArgs& a = c.a;
-  __shared__ float stats[3][4][R];
+  __shared__ float stats[4][R];
   __shared__ __attribute__((aligned(16))) float scales[4][64];
   const int lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -356,13 +361,16 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     sc_lds[lane] = quarter >= 2 ? scale : scale * a.c;
     const float vs = quarter >= 2 ? scale : 0.0f;
     if (__builtin_expect(lacks_room(room, vs), 0)) {
-      const float less = make_room<kBF16>(room, vs);
+      const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
 #pragma unroll
-      for (int n = 0; n < NQ; ++n)
+      for (int n = 0; n < NQ; ++n) {
+        m[n] += more;
+        l[n] *= less;
 #pragma unroll
         for (int x = 0; x < NB; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[n][x][e] *= less;
+      }
     }
 
     f32x4 sc[NQ][2];
@@ -389,8 +397,6 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     for (int y = 0; y < 2; ++y) {
       ks[y] = *(lds_cf32x4*)(sc_lds + 16 * y + 4 * quarter);
       vs4[y] = *(lds_cf32x4*)(sc_lds + 32 + 16 * y + 4 * quarter);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) vs4[y][e] *= room.down;
     }
     const bool cut = key0 + kFew - 1 > full;
     u32x4 p[NQ], pr[NQ];
@@ -400,12 +406,25 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[n][y][e] *= ks[y][e];
-          if (cut && key0 + 16 * y + 4 * quarter + e > limit[n]) sc[n][y][e] = -INFINITY;
-          top = __builtin_elementwise_maximum(top, sc[n][y][e]);
-        }
-      top = quarter_max(top) - kBias<kBF16>;
+        for (int e = 0; e < 4; ++e) sc[n][y][e] *= ks[y][e];
+      auto mask = [&](float (&x)[2][4], float with) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + 16 * y + 4 * quarter + e > limit[n]) x[y][e] = with;
+      };
+      float w[2][4], left[2][4];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[y][e] = sc[n][y][e];
+      if (cut) mask(w, -INFINITY);
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, w[y][e]);
+      top = quarter_max(top) + (room.e - kBias<kBF16>);
       if (__builtin_expect(__ballot(top > m[n] + kSlack) != 0, 0)) {
         const float now = fmaxf(m[n], top);
         const float alpha = __builtin_amdgcn_exp2f(m[n] - now);
@@ -416,17 +435,15 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[n][x][e] *= alpha;
       }
-      float w[2][4], left[2][4];
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x = __builtin_amdgcn_exp2f(sc[n][y][e] - m[n]);
+          const float x = __builtin_amdgcn_exp2f(w[y][e] - m[n]);
           l[n] += x;
           w[y][e] = x * vs4[y][e];
-          // (a scale there may be NaN)
-          if (cut && key0 + 16 * y + 4 * quarter + e > limit[n]) w[y][e] = 0.0f;
         }
+      if (cut) mask(w, 0.0f);  // (a scale there may be NaN)
       p[n] = u32x4{pack16<kBF16>(w[0][0], w[0][1]), pack16<kBF16>(w[0][2], w[0][3]), pack16<kBF16>(w[1][0], w[1][1]),
                    pack16<kBF16>(w[1][2], w[1][3])};
       // what the rounding of the weights left is multiplied too: the cache's bytes
@@ -467,34 +484,31 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
       use(t, p0);
     }
   }
+  // a column's sums of this wave as a weighted mean, and the log2 of its weights
+  float lse[NQ];
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     l[n] = quarter_sum(l[n]);
-    if (quarter == 0) {
-      stats[0][wave][16 * n + row] = m[n];
-      stats[1][wave][16 * n + row] = l[n];
-      stats[2][wave][16 * n + row] = room.down;
-    }
+    lse[n] = l[n] == 0.0f ? -INFINITY : m[n] + log2f(l[n]);
+    if (quarter == 0) stats[wave][16 * n + row] = lse[n];
   }
   __syncthreads();
 
-  // joined: the waves' sums at the largest maximum and the smallest 2^-e.  Wave
-  // w's channels 4 d .. 4 d + 3 of column x are at chunk d ^ (x % (DT / 4)) of row
-  // (w, x): neither side's accesses meet in a bank.
+  // The waves' means are joined.  Wave w's channels 4 d .. 4 d + 3 of column x are at
+  // chunk d ^ (x % (DT / 4)) of row (w, x): neither side's accesses meet in a bank.
   lds_u8* const sums = (lds_u8*)&g_code_few<DT, R>[0];
   auto sum_at = [&](int w, int x, int d) { return ((w * R + x) * (DT / 4) + (d ^ (x & (DT / 4 - 1)))) * 16; };
-  auto joined = [&](int x, float& top, float& down) {
-    top = stats[0][0][x], down = stats[2][0][x];
+  auto top_of = [&](int x) {
+    float top = stats[0][x];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, stats[0][w][x]), down = fminf(down, stats[2][w][x]);
+    for (int w = 1; w < 4; ++w) top = __builtin_elementwise_maximum(top, stats[w][x]);
+    return top == -INFINITY ? 0.0f : top;  // (no wave has a key)
   };
 #pragma unroll
   for (int n = 0; n < NQ; ++n) {
     const int x = 16 * n + row;
     if (tile * R + x >= rows) continue;
-    float top, down;
-    joined(x, top, down);
-    const float f = exp2f(m[n] - top) * (down / room.down);
+    const float f = l[n] == 0.0f ? 0.0f : exp2f(lse[n] - top_of(x)) / l[n];
 #pragma unroll
     for (int d = 0; d < NB; ++d)
       *(lds_f32x4*)(sums + sum_at(wave, x, 4 * d + quarter)) =
@@ -506,10 +520,10 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
   const int r = tile * R + x;
   if (r >= rows) return;
   const int tok = div_by(r, a.G);
-  float top, down, sum = 0.0f;
-  joined(x, top, down);
+  const float top = top_of(x);
+  float sum = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) sum += stats[1][w][x] * exp2f(stats[0][w][x] - top);
+  for (int w = 0; w < 4; ++w) sum += exp2f(stats[w][x] - top);
   const int seen = last_key(a, s, tok) + 1;
   const int k0 = t0 * kFew;
   const int k1 = t1 * kFew < seen ? t1 * kFew : seen;
@@ -519,7 +533,6 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
   const int d0 = (threadIdx.x / R) * N;
   if (threadIdx.x < R && a.splits > 1) store_part_stats(a, top, sum, out_row, none, split);
   const float inv = none ? 0.0f : 1.0f / sum;
-  const float up = 1.0f / down;
 #pragma unroll
   for (int d = 0; d < N; d += 4) {
     if (d0 + d >= a.D) break;
@@ -527,7 +540,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 #pragma unroll
     for (int w = 0; w < 4; ++w) y += *(lds_cf32x4*)(sums + sum_at(w, x, (d0 + d) / 4));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : y[e] * inv * up;
+    for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : y[e] * inv;
     if (a.splits > 1)
       *reinterpret_cast<f32x4*>(a.part + (split * (static_cast<int64_t>(a.T) * a.H) + out_row) * a.D + d0 + d) = y;
     else
@@ -545,17 +558,18 @@ __shared__ __attribute__((aligned(1024))) uint8_t g_code_k[2][kKeys * DT * 2];
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_code_v[2][kKeys * DT * 2];
 
-template <int DT>
+// A thread's share of a tile: chunks of NX rows, RPI apart.
+template <int DT, int NW>
 struct ManyTile {
-  static constexpr int CH = DT / 16, RPI = 256 / CH, NX = kKeys / RPI;  // chunks of a row, rows at a time
+  static constexpr int CH = DT / 16, RPI = 64 * NW / CH, NX = RPI < kKeys ? kKeys / RPI : 1;
   u32x4 k[NX], v[NX];
-  float scale;
+  float scale[NX];  // of the row's key (chunk 0) or value (chunk 1)
 };
 
-template <bool kBF16, int DT, int kCode>
-__global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots) {
-  constexpr int R = 128;
-  using Tile = ManyTile<DT>;
+template <bool kBF16, int DT, int kCode, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int slots) {
+  constexpr int R = 32 * NW;
+  using Tile = ManyTile<DT, NW>;
   const AttnArgs& a = c.a;
   __shared__ __attribute__((aligned(16))) float scales[2][2 * kKeys];  // keys', times c; then values'
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -600,29 +614,28 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
 
-  // this thread's chunk of rows row0, row0 + RPI, ..; and one of the tile's scales
+  // this thread's chunk of rows row0, row0 + RPI, ..
   const int ch = threadIdx.x % Tile::CH, row0 = threadIdx.x / Tile::CH;
-  const int srow = threadIdx.x & 63;
-  KvAt at[Tile::NX], sat;
+  KvAt at[Tile::NX];
   auto find = [&](int t) {
 #pragma unroll
     for (int x = 0; x < Tile::NX; ++x) at[x] = kv_at_clamped<true>(a, s, t * kKeys + row0 + x * Tile::RPI);
-    sat = kv_at_clamped<true>(a, s, t * kKeys + srow);
   };
   Tile next;
   auto load = [&](int t) {
 #pragma unroll
     for (int x = 0; x < Tile::NX; ++x) {
       next.k[x] = next.v[x] = u32x4{0, 0, 0, 0};
-      if (t * kKeys + row0 + x * Tile::RPI < s.Lk && 16 * ch < a.D) {
+      next.scale[x] = 0.0f;
+      const bool in = row0 + x * Tile::RPI < kKeys && t * kKeys + row0 + x * Tile::RPI < s.Lk;
+      if (in && 16 * ch < a.D) {
         next.k[x] = *reinterpret_cast<const u32x4*>(c.k.p + at[x].page * c.k.page + at[x].at * c.k.token + hk * c.k.head + 16 * ch);
         next.v[x] = *reinterpret_cast<const u32x4*>(c.v.p + at[x].page * c.v.page + at[x].at * c.v.token + hk * c.v.head + 16 * ch);
       }
-    }
-    next.scale = 0.0f;
-    if (threadIdx.x < 2 * kKeys && t * kKeys + srow < s.Lk) {
-      const CodeRows& rr = wave == 0 ? c.k : c.v;
-      next.scale = rr.scale[sat.page * rr.s_page + sat.at * rr.s_token + hk * rr.s_head];
+      if (in && ch < 2) {
+        const CodeRows& r = ch == 0 ? c.k : c.v;
+        next.scale[x] = r.scale[at[x].page * r.s_page + at[x].at * r.s_token + hk * r.s_head];
+      }
     }
     find(t + 1);
   };
@@ -630,6 +643,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
 #pragma unroll
     for (int x = 0; x < Tile::NX; ++x) {
       const int row = row0 + x * Tile::RPI;
+      if (Tile::RPI > kKeys && row >= kKeys) break;  // (threads without a row)
       u32x4 lo, hi;
       const int o0 = row * (DT * 2) + (((2 * ch) ^ row_slot<DT>(row)) << 4);
       const int o1 = row * (DT * 2) + (((2 * ch + 1) ^ row_slot<DT>(row)) << 4);
@@ -639,8 +653,8 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
       widen16<kBF16, kCode>(next.v[x], lo, hi);
       *(lds_u32x4*)((lds_u8*)&g_code_v<DT>[buf][0] + o0) = lo;
       *(lds_u32x4*)((lds_u8*)&g_code_v<DT>[buf][0] + o1) = hi;
+      if (ch < 2) scales[buf][ch * kKeys + row] = ch == 0 ? next.scale[x] * a.c : next.scale[x];
     }
-    if (threadIdx.x < 2 * kKeys) scales[buf][threadIdx.x] = wave == 0 ? next.scale * a.c : next.scale;
   };
 
   const LaneAt<DT> where = lane_at<DT>(lane, 0);
@@ -650,7 +664,9 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     const lds_u8 *kt = (const lds_u8*)&g_code_k<DT>[buf][0], *vt = (const lds_u8*)&g_code_v<DT>[buf][0];
     const lds_f32* sl = (const lds_f32*)&scales[buf][0];
     if (__builtin_expect(lacks_room(room, sl[kKeys + lane]), 0)) {
-      const float less = make_room<kBF16>(room, sl[kKeys + lane]);
+      const float more = make_room<kBF16>(room, sl[kKeys + lane]), less = __builtin_amdgcn_exp2f(-more);
+      col.m += more;
+      col.l *= less;
 #pragma unroll
       for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
@@ -679,7 +695,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     };
     if (cut) mask(-INFINITY);
     code_step<kBF16, DT, 2, false>(
-        col, sc, room.down, [&](int kt, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt + 8 * g + 4 * half); },
+        col, sc, room.e - kBias<kBF16>, [&](int kt, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt + 8 * g + 4 * half); },
         [&](f32x16 (&)[2]) {
           if (cut) mask(0.0f);
         },
@@ -709,7 +725,6 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   if (!inside) return;
   if (half == 0 && a.splits > 1) store_part_stats(a, col.m, l, row, none, split);
   const float rl = none ? 0.0f : 1.0f / l;
-  const float up = 1.0f / room.down;
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
@@ -718,7 +733,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
       if (d >= a.D) continue;
       f32x4 y;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : col.o[db][i + e] * rl * up;
+      for (int e = 0; e < 4; ++e) y[e] = none ? 0.0f : col.o[db][i + e] * rl;
       if (a.splits > 1)
         *reinterpret_cast<f32x4*>(a.part + (split * (static_cast<int64_t>(a.T) * a.H) + row) * a.D + d) = y;
       else
@@ -744,8 +759,10 @@ int launch(const CodeArgs& c, int R, hipStream_t st) {
     launch_few<kBF16, DT, kCode, 1>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
   else if (R == 32)
     launch_few<kBF16, DT, kCode, 2>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
+  else if (R == 128)
+    code_rows_kernel<kBF16, DT, kCode, 4><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
   else
-    code_rows_kernel<kBF16, DT, kCode><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
+    code_rows_kernel<kBF16, DT, kCode, 8><<<static_cast<uint32_t>(grid), 512, 0, st>>>(c, static_cast<int>(slots));
   const int rc = check_launch("attention");
   if (rc != GPTQ_OK || a.splits == 1) return rc;
   return launch_join<kBF16>(a, st);
