@@ -81,17 +81,6 @@ __device__ __forceinline__ void softmax_step(Column<DT>& col, f32x16 (&s)[NK], f
   }
 }
 
-// The lane's query row as an operand over its channels: zeros past D and for
-// rows outside the tile.
-template <int DT>
-__device__ __forceinline__ void load_query(u32x4 (&q)[DT / 16], const uint16_t* row, bool inside, int D, int half) {
-#pragma unroll
-  for (int s = 0; s < DT / 16; ++s) {
-    const int d = 16 * s + 8 * half;
-    q[s] = inside && d < D ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
-  }
-}
-
 // Writes a column's result: the output (and lse), or this split's sums.  kExact:
 // of sums that may hold infinities (whose rounding leaves nothing).
 template <bool kBF16, int DT, bool kTrain, bool kExact>

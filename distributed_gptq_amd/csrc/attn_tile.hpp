@@ -157,6 +157,17 @@ __device__ __forceinline__ u32x4 column_operand(const lds_u8* tile, int row0, in
   return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The lane's query row as an operand over its channels: zeros past D and for
+// rows outside the tile.
+template <int DT>
+__device__ __forceinline__ void load_query(u32x4 (&q)[DT / 16], const uint16_t* row, bool inside, int D, int half) {
+#pragma unroll
+  for (int s = 0; s < DT / 16; ++s) {
+    const int d = 16 * s + 8 * half;
+    q[s] = inside && d < D ? *reinterpret_cast<const u32x4*>(row + d) : u32x4{0, 0, 0, 0};
+  }
+}
+
 // The lane for a path taken seldom: what follows from it is computed there, and
 // not kept in registers until then.
 __device__ __forceinline__ int late_lane() {

@@ -70,13 +70,13 @@ struct CodeColumn {
 };
 
 // Adds NK x 32 keys with scores s (scaled, -infinity where not seen) to the
-// column's sums; `ahead` is e less kBias.  `scale` gives the scales of the values of keys 32 kt + 8 g + 4
-// (lane / 32) .. + 3; `drop` clears what belongs to keys that the column does not
-// see, where the tile has any (a scale there may be NaN).  `value` gives the
-// operand of value rows 16 ks .. of the tile, channels 32 db ..  kRest: what the
-// rounding of the weights left is multiplied too.
-template <bool kBF16, int DT, int NK, bool kRest, class Scale, class Drop, class Value>
-__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, Scale&& scale, Drop&& drop, Value&& value) {
+// column's sums; `ahead` is e less kBias.  `scale` gives the scales of the values of
+// keys 32 kt + 8 g + 4 (lane / 32) .. + 3; `drop` clears what belongs to keys that
+// the column does not see, where the tile has any.  `value` gives the operand of
+// value rows 16 ks .. of the tile, channels 32 db ...
+template <bool kBF16, int DT, int NK, class Scale, class Drop, class Value>
+__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, Scale&& scale, Drop&& drop,
+                                          Value&& value) {
   float t = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
@@ -107,18 +107,12 @@ __device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], 
       }
     }
   col.l += sum;
-  drop(s);
+  drop();
 #pragma unroll
   for (int ks = 0; ks < 2 * NK; ++ks) {
     const u32x4 p = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
-    u32x4 rest;
-    if constexpr (kRest) rest = operand_rest<kBF16>(s[ks / 2], 8 * (ks % 2), p);
 #pragma unroll
-    for (int db = 0; db < DT / 32; ++db) {
-      const u32x4 v = value(ks, db);
-      col.o[db] = mma32<kBF16>(v, p, col.o[db]);
-      if constexpr (kRest) col.o[db] = mma32<kBF16>(v, rest, col.o[db]);
-    }
+    for (int db = 0; db < DT / 32; ++db) col.o[db] = mma32<kBF16>(value(ks, db), p, col.o[db]);
   }
 }
 
@@ -155,16 +149,15 @@ __device__ __forceinline__ void store_part_stats(const AttnArgs& a, float m, flo
 // tile's loads are in flight while one is used.
 constexpr int kFew = 32;
 
-// 16-byte chunk c of a row of values is at slot c ^ this in LDS: the writes of 16
-// rows' chunks, and the transposing reads of 8 rows by 16 lanes, 32 lanes at a
-// time, meet each bank once.
+// 16-byte chunk c of a row of values is at slot c ^ this in LDS: the writes of 8
+// neighbouring rows' chunks (128 bytes at a time), and the transposing reads of 16
+// rows by 32 lanes (256 bytes), meet each bank once.
 template <int DT>
 __device__ __forceinline__ int code_slot(int row) {
-  const int high = ((row >> 3) ^ (row >> 4)) & 1;
   if constexpr (DT == 128)
-    return ((row >> 1) & 3) | high << 2;
+    return ((row >> 1) & 3) | (((row >> 4) ^ row) & 1) << 2;
   else
-    return ((row >> 2) & 1) | high << 1;
+    return ((row >> 2) & 1) | (((row >> 4) ^ (row >> 1)) & 1) << 1;
 }
 
 template <bool kBF16>
@@ -550,26 +543,23 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 
 // ------------------------------------------------------------- many rows ----
 // A workgroup of 4 waves has 128 packed rows, 32 a wave.  Tiles of 64 keys are
-// loaded as codes by all threads, widened once and left in LDS as 16-bit rows,
-// in one of two buffers while the other one is used.
+// loaded as codes by all threads, widened once and left in LDS as 16-bit values, in
+// one of two buffers while the other one is used.
+//
+// A tile's 16-byte chunk c (8 channels) of row r is at c kChunk + 16 r: one address
+// and constants reach all operands of a lane.  kChunk is 64 bytes past a multiple of
+// all banks' 256, so that the transposing reads of 4 rows x 4 chunks by 32 lanes,
+// the reads of 16 rows, and the writes of 4 rows x 2 chunks by 8 lanes (128 bytes)
+// meet each bank once.
 constexpr int kKeys = 64;
+constexpr int kChunk = kKeys * 16 + 64;
 template <int DT>
-__shared__ __attribute__((aligned(1024))) uint8_t g_code_k[2][kKeys * DT * 2];
-template <int DT>
-__shared__ __attribute__((aligned(1024))) uint8_t g_code_v[2][kKeys * DT * 2];
+__shared__ __attribute__((aligned(1024))) uint8_t g_code_tiles[2][2][DT / 8 * kChunk];  // buffer; keys, values
 
-// A thread's share of a tile: chunks of NX rows, RPI apart.
-template <int DT, int NW>
-struct ManyTile {
-  static constexpr int CH = DT / 16, RPI = 64 * NW / CH, NX = RPI < kKeys ? kKeys / RPI : 1;
-  u32x4 k[NX], v[NX];
-  float scale[NX];  // of the row's key (chunk 0) or value (chunk 1)
-};
-
-template <bool kBF16, int DT, int kCode, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int slots) {
-  constexpr int R = 32 * NW;
-  using Tile = ManyTile<DT, NW>;
+template <bool kBF16, int DT, int kCode, bool kWhole>
+__global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots) {
+  constexpr int R = 128;
+  constexpr int CH = DT / 16, RPI = 256 / CH, NX = kKeys / RPI;  // chunks of a row of codes, rows at a time
   const AttnArgs& a = c.a;
   __shared__ __attribute__((aligned(16))) float scales[2][2 * kKeys];  // keys', times c; then values'
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -601,11 +591,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
 
   u32x4 q[DT / 16];
-#pragma unroll
-  for (int d = 0; d < DT / 16; ++d) {
-    const int at = 16 * d + 8 * half;
-    q[d] = inside && at < a.D ? *reinterpret_cast<const u32x4*>(qrow + at) : u32x4{0, 0, 0, 0};
-  }
+  load_query<DT>(q, qrow, inside, a.D, half);
 
   CodeColumn<DT> col;
   ScaleRoom room;
@@ -614,57 +600,84 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
 
-  // this thread's chunk of rows row0, row0 + RPI, ..
-  const int ch = threadIdx.x % Tile::CH, row0 = threadIdx.x / Tile::CH;
-  KvAt at[Tile::NX];
-  auto find = [&](int t) {
-#pragma unroll
-    for (int x = 0; x < Tile::NX; ++x) at[x] = kv_at_clamped<true>(a, s, t * kKeys + row0 + x * Tile::RPI);
+  // This thread's chunk of rows row0 + RPI x of a tile.  Rows past the sequence's
+  // end are its last one again, which the mask drops; chunks past the head are its
+  // first one, which meets zeros of the queries and channels that are not stored.
+  // 8 neighbouring lanes have 2 chunks of 4 rows.
+  const int ch = (lane & 1) | ((lane >> 3) & (CH / 2 - 1)) << 1;
+  const int own_row = ((lane >> 1) & 3) | (lane >> (CH == 8 ? 5 : 4)) << 2;
+  const int wave_row = wave * (64 / CH);  // (of 16 or fewer, of which all are in one page)
+  const int row0 = wave_row + own_row;
+  auto key_of = [&](int t, int x) {
+    if constexpr (kWhole) return clamp_int(t * kKeys + RPI * x + wave_row, 0, s.Lk - 1);
+    return clamp_int(t * kKeys + RPI * x + row0, 0, s.Lk - 1);
   };
-  Tile next;
-  auto load = [&](int t) {
+  auto page_of = [&](int t, int x) {
+    return a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, x), a.paged.page)];
+  };
+  const uint32_t chunk = 16 * ch < a.D ? 16 * ch : 0;
+  u32x4 nk[NX], nv[NX];
+  float nks[NX], nvs[NX];
+  auto load = [&](int t, const int (&pages)[NX]) {
 #pragma unroll
-    for (int x = 0; x < Tile::NX; ++x) {
-      next.k[x] = next.v[x] = u32x4{0, 0, 0, 0};
-      next.scale[x] = 0.0f;
-      const bool in = row0 + x * Tile::RPI < kKeys && t * kKeys + row0 + x * Tile::RPI < s.Lk;
-      if (in && 16 * ch < a.D) {
-        next.k[x] = *reinterpret_cast<const u32x4*>(c.k.p + at[x].page * c.k.page + at[x].at * c.k.token + hk * c.k.head + 16 * ch);
-        next.v[x] = *reinterpret_cast<const u32x4*>(c.v.p + at[x].page * c.v.page + at[x].at * c.v.token + hk * c.v.head + 16 * ch);
-      }
-      if (in && ch < 2) {
-        const CodeRows& r = ch == 0 ? c.k : c.v;
-        next.scale[x] = r.scale[at[x].page * r.s_page + at[x].at * r.s_token + hk * r.s_head];
+    for (int x = 0; x < NX; ++x) {
+      const int key = key_of(t, x);
+      const int at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+      const int page = clamp_int(kWhole ? uniform_int(pages[x]) : pages[x], 0, a.paged.pages - 1);
+      // (of rows past the end the last one's)
+      int own = own_row;
+      if constexpr (kWhole) own = own < s.Lk - 1 - key ? own : s.Lk - 1 - key;
+      const uint8_t* kp = c.k.p + page * c.k.page + at * c.k.token + hk * c.k.head;
+      const uint8_t* vp = c.v.p + page * c.v.page + at * c.v.token + hk * c.v.head;
+      const float* ks = c.k.scale + page * c.k.s_page + at * c.k.s_token + hk * c.k.s_head;
+      const float* vs = c.v.scale + page * c.v.s_page + at * c.v.s_token + hk * c.v.s_head;
+      const uint32_t ko = (kWhole ? own * static_cast<uint32_t>(c.k.token) : 0u) + chunk;
+      const uint32_t vo = (kWhole ? own * static_cast<uint32_t>(c.v.token) : 0u) + chunk;
+      nk[x] = *reinterpret_cast<const u32x4*>(kp + ko);
+      nv[x] = *reinterpret_cast<const u32x4*>(vp + vo);
+      if (ch == 0) {
+        nks[x] = kWhole ? ks[own * c.k.s_token] : *ks;
+        nvs[x] = kWhole ? vs[own * c.v.s_token] : *vs;
       }
     }
-    find(t + 1);
   };
+  // (the order of a thread's two chunks takes turns: two lanes' first ones would meet)
+  const bool turn = ch & 1;
+  const int put0 = (2 * ch + (turn ? 1 : 0)) * kChunk + 16 * row0;
+  const int put1 = (2 * ch + (turn ? 0 : 1)) * kChunk + 16 * row0;
   auto put = [&](int buf) {
+    lds_u8 *const kt = (lds_u8*)&g_code_tiles<DT>[buf][0][0], *const vt = (lds_u8*)&g_code_tiles<DT>[buf][1][0];
+    auto turned = [&](const u32x4& w) { return turn ? u32x4{w[2], w[3], w[0], w[1]} : w; };
 #pragma unroll
-    for (int x = 0; x < Tile::NX; ++x) {
-      const int row = row0 + x * Tile::RPI;
-      if (Tile::RPI > kKeys && row >= kKeys) break;  // (threads without a row)
+    for (int x = 0; x < NX; ++x) {
       u32x4 lo, hi;
-      const int o0 = row * (DT * 2) + (((2 * ch) ^ row_slot<DT>(row)) << 4);
-      const int o1 = row * (DT * 2) + (((2 * ch + 1) ^ row_slot<DT>(row)) << 4);
-      widen16<kBF16, kCode>(next.k[x], lo, hi);
-      *(lds_u32x4*)((lds_u8*)&g_code_k<DT>[buf][0] + o0) = lo;
-      *(lds_u32x4*)((lds_u8*)&g_code_k<DT>[buf][0] + o1) = hi;
-      widen16<kBF16, kCode>(next.v[x], lo, hi);
-      *(lds_u32x4*)((lds_u8*)&g_code_v<DT>[buf][0] + o0) = lo;
-      *(lds_u32x4*)((lds_u8*)&g_code_v<DT>[buf][0] + o1) = hi;
-      if (ch < 2) scales[buf][ch * kKeys + row] = ch == 0 ? next.scale[x] * a.c : next.scale[x];
+      widen16<kBF16, kCode>(turned(nk[x]), lo, hi);
+      *(lds_u32x4*)(kt + put0 + 16 * RPI * x) = lo;
+      *(lds_u32x4*)(kt + put1 + 16 * RPI * x) = hi;
+      widen16<kBF16, kCode>(turned(nv[x]), lo, hi);
+      *(lds_u32x4*)(vt + put0 + 16 * RPI * x) = lo;
+      *(lds_u32x4*)(vt + put1 + 16 * RPI * x) = hi;
+      if (ch == 0) {
+        scales[buf][row0 + RPI * x] = nks[x] * a.c;
+        scales[buf][kKeys + row0 + RPI * x] = nvs[x];
+      }
     }
   };
 
-  const LaneAt<DT> where = lane_at<DT>(lane, 0);
+  // where a lane reads: row lane % 32, channels 8 (lane / 32) .. of a product over
+  // channels; for one over rows, by 16 lanes, 4 rows x 16 channels (attn_tile.hpp)
+  int krow = half * kChunk + 16 * (lane & 31);
+  int vrow = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * kChunk + 16 * (4 * half + ((lane & 15) >> 2)) + 8 * (lane & 1);
+  asm volatile("" : "+v"(krow), "+v"(vrow));  // (so that the constant parts go into the instructions)
   auto use = [&](int t, int buf) {
     const int key0 = t * kKeys;
     if (key0 >= wave_end) return;
-    const lds_u8 *kt = (const lds_u8*)&g_code_k<DT>[buf][0], *vt = (const lds_u8*)&g_code_v<DT>[buf][0];
-    const lds_f32* sl = (const lds_f32*)&scales[buf][0];
-    if (__builtin_expect(lacks_room(room, sl[kKeys + lane]), 0)) {
-      const float more = make_room<kBF16>(room, sl[kKeys + lane]), less = __builtin_amdgcn_exp2f(-more);
+    const lds_u8* const kt = (const lds_u8*)&g_code_tiles<DT>[buf][0][0] + krow;
+    const lds_u8* const vt = (const lds_u8*)&g_code_tiles<DT>[buf][1][0] + vrow;
+    const lds_f32* const sl = (const lds_f32*)&scales[buf][0];
+    const float vs = sl[kKeys + lane];
+    if (__builtin_expect(lacks_room(room, vs), 0)) {
+      const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
       col.m += more;
       col.l *= less;
 #pragma unroll
@@ -676,7 +689,11 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) sc[n] = mma32<kBF16>(row_operand<DT>(kt, 32 * n, d, where), q[d], sc[n]);
+      for (int n = 0; n < 2; ++n) {
+        const u32x4 k = *(const lds_u32x4*)(kt + 2 * d * kChunk + 512 * n);
+        sc[n] = mma32<kBF16>(k, q[d], sc[n]);
+      }
+    reads_ahead<DT / 8, 8>();
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -694,24 +711,38 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
           if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = with;
     };
     if (cut) mask(-INFINITY);
-    code_step<kBF16, DT, 2, false>(
-        col, sc, room.e - kBias<kBF16>, [&](int kt, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt + 8 * g + 4 * half); },
-        [&](f32x16 (&)[2]) {
-          if (cut) mask(0.0f);
+    code_step<kBF16, DT, 2>(
+        col, sc, room.e - kBias<kBF16>, [&](int kt2, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt2 + 8 * g + 4 * half); },
+        [&]() {
+          if (cut) mask(0.0f);  // (a scale there may be NaN)
         },
-        [&](int ks, int db) { return column_operand<DT>(vt, 16 * ks, db, where); });
+        [&](int ks, int db) {
+          s16x4 v[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + 4 * db * kChunk + 256 * ks + 128 * j));
+          return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        });
   };
 
+  // A tile's entries of the block table are loaded before the rows of the tile
+  // before it: loads return in order.
   if (t0 < t1) {
-    find(t0);
-    load(t0);
+    int p0[NX], p1[NX];
+#pragma unroll
+    for (int x = 0; x < NX; ++x) p0[x] = page_of(t0, x), p1[x] = page_of(t0 + 1, x);
+    load(t0, p0);
     put(0);
-    if (t0 + 1 < t1) load(t0 + 1);
+#pragma unroll
+    for (int x = 0; x < NX; ++x) p0[x] = page_of(t0 + 2, x);
+    load(t0 + 1, p1);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
-      if (t + 1 < t1) put(buf ^ 1);
-      if (t + 2 < t1) load(t + 2);
+      put(buf ^ 1);
+#pragma unroll
+      for (int x = 0; x < NX; ++x) p1[x] = p0[x], p0[x] = page_of(t + 3, x);
+      load(t + 2, p1);
       use(t, buf);
       __syncthreads();
     }
@@ -759,10 +790,10 @@ int launch(const CodeArgs& c, int R, hipStream_t st) {
     launch_few<kBF16, DT, kCode, 1>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
   else if (R == 32)
     launch_few<kBF16, DT, kCode, 2>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
-  else if (R == 128)
-    code_rows_kernel<kBF16, DT, kCode, 4><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
+  else if (a.paged.whole)
+    code_rows_kernel<kBF16, DT, kCode, true><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
   else
-    code_rows_kernel<kBF16, DT, kCode, 8><<<static_cast<uint32_t>(grid), 512, 0, st>>>(c, static_cast<int>(slots));
+    code_rows_kernel<kBF16, DT, kCode, false><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
   const int rc = check_launch("attention");
   if (rc != GPTQ_OK || a.splits == 1) return rc;
   return launch_join<kBF16>(a, st);
