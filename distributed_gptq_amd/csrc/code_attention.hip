@@ -635,10 +635,8 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
       const uint32_t vo = (kWhole ? own * static_cast<uint32_t>(c.v.token) : 0u) + chunk;
       nk[x] = *reinterpret_cast<const u32x4*>(kp + ko);
       nv[x] = *reinterpret_cast<const u32x4*>(vp + vo);
-      if (ch == 0) {
-        nks[x] = kWhole ? ks[own * c.k.s_token] : *ks;
-        nvs[x] = kWhole ? vs[own * c.v.s_token] : *vs;
-      }
+      nks[x] = kWhole ? ks[own * c.k.s_token] : *ks;  // (the same for all of a row's threads)
+      nvs[x] = kWhole ? vs[own * c.v.s_token] : *vs;
     }
   };
   // (the order of a thread's two chunks takes turns: two lanes' first ones would meet)
@@ -657,10 +655,8 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
       widen16<kBF16, kCode>(turned(nv[x]), lo, hi);
       *(lds_u32x4*)(vt + put0 + 16 * RPI * x) = lo;
       *(lds_u32x4*)(vt + put1 + 16 * RPI * x) = hi;
-      if (ch == 0) {
-        scales[buf][row0 + RPI * x] = nks[x] * a.c;
-        scales[buf][kKeys + row0 + RPI * x] = nvs[x];
-      }
+      scales[buf][row0 + RPI * x] = nks[x] * a.c;
+      scales[buf][kKeys + row0 + RPI * x] = nvs[x];
     }
   };
 
@@ -669,9 +665,8 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   int krow = half * kChunk + 16 * (lane & 31);
   int vrow = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * kChunk + 16 * (4 * half + ((lane & 15) >> 2)) + 8 * (lane & 1);
   asm volatile("" : "+v"(krow), "+v"(vrow));  // (so that the constant parts go into the instructions)
-  auto use = [&](int t, int buf) {
+  auto use = [&](int t, int buf, auto&& meanwhile) {
     const int key0 = t * kKeys;
-    if (key0 >= wave_end) return;
     const lds_u8* const kt = (const lds_u8*)&g_code_tiles<DT>[buf][0][0] + krow;
     const lds_u8* const vt = (const lds_u8*)&g_code_tiles<DT>[buf][1][0] + vrow;
     const lds_f32* const sl = (const lds_f32*)&scales[buf][0];
@@ -685,6 +680,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
 #pragma unroll
         for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
     }
+    meanwhile();
     f32x16 sc[2] = {zero16(), zero16()};
 #pragma unroll
     for (int d = 0; d < DT / 16; ++d)
@@ -739,11 +735,12 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
-      put(buf ^ 1);
+      use(t, buf, [&]() {
+        put(buf ^ 1);
 #pragma unroll
-      for (int x = 0; x < NX; ++x) p1[x] = p0[x], p0[x] = page_of(t + 3, x);
-      load(t + 2, p1);
-      use(t, buf);
+        for (int x = 0; x < NX; ++x) p1[x] = p0[x], p0[x] = page_of(t + 3, x);
+        load(t + 2, p1);
+      });
       __syncthreads();
     }
   }
