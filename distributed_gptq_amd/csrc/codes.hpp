@@ -19,18 +19,17 @@ constexpr float kLeast = 0x1p-120f;
 template <int kCode>
 constexpr float kMostScale = kCode == GPTQ_CODE_I8 ? 0x1.020406p+121f : 0x1.249248p+119f;
 
-// Four values, each times inv and rounded to the nearest code (ties to even);
-// the clamp takes what the rounding of inv put past the last code.
+// Four values, each times inv and rounded to the nearest code (ties to even).  inv
+// is the top code over the largest of them, so that no product is more than two
+// roundings past the top: both types round that back to it.
 template <int kCode>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
-  constexpr float top = kTop<kCode>;
-  auto in = [&](float x) { return fminf(fmaxf(x * inv, -top), top); };
   if constexpr (kCode == GPTQ_CODE_I8) {
-    auto code = [&](float x) { return static_cast<uint32_t>(static_cast<int>(rintf(in(x)))) & 0xFFu; };
+    auto code = [&](float x) { return static_cast<uint32_t>(static_cast<int>(rintf(x * inv))) & 0xFFu; };
     return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
   } else {
-    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
-    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), low, true));
+    const int low = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, low, true));
   }
 }
 

@@ -47,5 +47,28 @@ __device__ __forceinline__ void store_values(void* p, int64_t at, const float (&
   }
 }
 
+// store_values by the conversions of a pair at a time (a NaN stays one, with other
+// bits than store_values gives it)
+template <int N, int kType>
+__device__ __forceinline__ void store_pairs(void* p, int64_t at, const float (&x)[N]) {
+  if constexpr (kType == GPTQ_F32) {
+    store_values<N, kType>(p, at, x);
+  } else {
+    constexpr int kWide = N / 2 < 4 ? N / 2 : 4;
+    typedef uint32_t vec __attribute__((ext_vector_type(kWide)));
+    vec* to = reinterpret_cast<vec*>(static_cast<uint16_t*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < N / 2; i += kWide) {
+      vec w;
+#pragma unroll
+      for (int e = 0; e < kWide; ++e) {
+        const float lo = x[2 * (i + e)], hi = x[2 * (i + e) + 1];
+        w[e] = kType == GPTQ_BF16 ? pack_bf16(lo, hi) : pack_f16(lo, hi);
+      }
+      to[i / kWide] = w;
+    }
+  }
+}
+
 }  // namespace
 }  // namespace gptq
