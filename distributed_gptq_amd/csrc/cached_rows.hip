@@ -51,7 +51,7 @@ __device__ __forceinline__ void put_chunk(void* out, int64_t row, int D, int c, 
 
 // A thread has a chunk of the keys and values of kHeads heads of a token, whose
 // sequence and page it looks up once and whose loads go together.  Packed row t of
-// sequence b is its cached token context - (cu[b + 1] - t).  Bound by memory: 23k
+// sequence b is its cached token context - (cu[b + 1] - t).  Bound by memory: 46k
 // rows of 8 heads of 128 int8 codes into bf16 (286 MB) take 62 us, 4.6 TB/s; with 2
 // heads 67 us, with 8 65 us, with one 99 us, with 16 codes of one head 67 us (half
 // of each line per store).

@@ -44,8 +44,10 @@ constexpr int kLeastE = -80;  // (2^31 weights of 2^(kSlack + 7 + 80) are inside
 
 // A wave's e, and the largest scale that it allows.
 struct ScaleRoom {
-  float e = 0.0f, cap = -1.0f;
+  int e = 0;
+  float cap = -1.0f;
 };
+__device__ __forceinline__ float uniform_float(float v) { return __int_as_float(uniform_int(__float_as_int(v))); }
 // `vs`: a scale of each lane's (0 for none); those that are not finite are no
 // reason for another e.
 __device__ __forceinline__ bool lacks_room(const ScaleRoom& r, float vs) { return __ballot(vs > r.cap && vs < INFINITY) != 0; }
@@ -56,11 +58,11 @@ __device__ __forceinline__ float make_room(ScaleRoom& r, float vs) {
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
   if (top == 0.0f) return 0.0f;  // (scales of 0 need no e)
-  const int e = clamp_int(ilogbf(top) + 1, kLeastE, kMostE<kBF16>);
-  const float more = static_cast<float>(e) - r.e;
-  r.e = static_cast<float>(e);
-  r.cap = e == kMostE<kBF16> ? INFINITY : ldexpf(1.0f, e + kScaleRoom<kBF16>);
-  return more;
+  const int e = uniform_int(clamp_int(ilogbf(top) + 1, kLeastE, kMostE<kBF16>));
+  const int more = e - r.e;
+  r.e = e;
+  r.cap = uniform_float(e == kMostE<kBF16> ? INFINITY : ldexpf(1.0f, e + kScaleRoom<kBF16>));
+  return static_cast<float>(more);
 }
 
 template <int DT>
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
       for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int e = 0; e < 4; ++e) top = __builtin_elementwise_maximum(top, w[y][e]);
-      top = quarter_max(top) + (room.e - kBias<kBF16>);
+      top = quarter_max(top) + (static_cast<float>(room.e) - kBias<kBF16>);
       if (__builtin_expect(__ballot(top > m[n] + kSlack) != 0, 0)) {
         const float now = fmaxf(m[n], top);
         const float alpha = __builtin_amdgcn_exp2f(m[n] - now);
@@ -573,25 +575,24 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   const int rows = s.Lq * static_cast<int>(a.G.d);
   if (tile * R >= rows) return;
 
-  const int r = tile * R + wave * 32 + (lane & 31);
-  const bool inside = r < rows;
-  const int tok = div_by(inside ? r : rows - 1, a.G);
-  const int head = hk * static_cast<int>(a.G.d) + ((inside ? r : rows - 1) - tok * static_cast<int>(a.G.d));
-  const uint16_t* qrow = a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh;
-  const int limit = last_key(a, s, tok);
+  u32x4 q[DT / 16];
+  int limit;
+  {
+    const int r = tile * R + wave * 32 + (lane & 31);
+    const bool inside = r < rows;
+    const int tok = div_by(inside ? r : rows - 1, a.G);
+    const int head = hk * static_cast<int>(a.G.d) + ((inside ? r : rows - 1) - tok * static_cast<int>(a.G.d));
+    load_query<DT>(q, a.q.p + (s.q0 + tok) * a.q.st + head * a.q.sh, inside, a.D, half);
+    limit = last_key(a, s, tok);
+  }
   const int first_r = tile * R + wave * 32;
   const int full = last_key(a, s, div_by(first_r < rows ? first_r : rows - 1, a.G));  // keys all its rows see
   const int last_r = (tile + 1) * R < rows ? (tile + 1) * R - 1 : rows - 1;
-  const int wave_r = first_r + 31 < rows ? first_r + 31 : rows - 1;
-  const int wave_end = first_r < rows ? last_key(a, s, div_by(wave_r, a.G)) + 1 : 0;
   const int last = last_key(a, s, div_by(last_r, a.G));
   const int end = last < 0 ? 0 : last + 1;
   const int tiles = (end + kKeys - 1) / kKeys;
   const int per = (tiles + a.splits - 1) / a.splits;
   const int t0 = split * per, t1 = t0 + per < tiles ? t0 + per : tiles;
-
-  u32x4 q[DT / 16];
-  load_query<DT>(q, qrow, inside, a.D, half);
 
   CodeColumn<DT> col;
   ScaleRoom room;
@@ -600,50 +601,95 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db) col.o[db] = zero16();
 
-  // This thread's chunk of rows row0 + RPI x of a tile.  Rows past the sequence's
-  // end are its last one again, which the mask drops; chunks past the head are its
+  // This thread's chunk of rows row0 + RPI x of a tile.  Chunks past the head are its
   // first one, which meets zeros of the queries and channels that are not stored.
   // 8 neighbouring lanes have 2 chunks of 4 rows.
   const int ch = (lane & 1) | ((lane >> 3) & (CH / 2 - 1)) << 1;
   const int own_row = ((lane >> 1) & 3) | (lane >> (CH == 8 ? 5 : 4)) << 2;
-  const int wave_row = wave * (64 / CH);  // (of 16 or fewer, of which all are in one page)
+  const int wave_row = wave * (64 / CH);
   const int row0 = wave_row + own_row;
-  auto key_of = [&](int t, int x) {
-    if constexpr (kWhole) return clamp_int(t * kKeys + RPI * x + wave_row, 0, s.Lk - 1);
-    return clamp_int(t * kKeys + RPI * x + row0, 0, s.Lk - 1);
-  };
-  auto page_of = [&](int t, int x) {
-    return a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, x), a.paged.page)];
-  };
   const uint32_t chunk = 16 * ch < a.D ? 16 * ch : 0;
   u32x4 nk[NX], nv[NX];
-  float nks[NX], nvs[NX];
-  auto load = [&](int t, const int (&pages)[NX]) {
+  float nks[NX], nvs[NX];  // (kWhole: the lane's one scale in nks[0])
+
+  // kWhole: the W rows of a wave for each x are in one page.  Lane i < 2 NX makes the
+  // address of the first one's codes, for x = i % NX, of keys or values by i / NX, for
+  // all lanes; lanes from 32 on those of their scale, of row lane % W for x = lane / W
+  // % NX.  (As scalar arithmetic, twenty times as many instructions, it took a fifth
+  // of the time.)
+  constexpr int W = 64 / CH;
+  const int x_of = half ? lane / W % NX : lane % NX;
+  const int values_of = half ? (lane - 32) / (W * NX) : lane / NX % 2;
+  const int my_key = RPI * x_of + wave_row + (half ? lane % W : 0);  // in the tile
+  __shared__ __attribute__((aligned(16))) u32x4 bases[kWhole ? 256 : 1];  // address; strides of pages and tokens
+  if constexpr (kWhole) {
+    const CodeRows& from = values_of ? c.v : c.k;
+    const uint64_t base = half ? reinterpret_cast<uint64_t>(from.scale) + 4 * (hk * from.s_head + lane % W * from.s_token)
+                               : reinterpret_cast<uint64_t>(from.p) + hk * from.head;
+    bases[threadIdx.x] = u32x4{static_cast<uint32_t>(base), static_cast<uint32_t>(base >> 32),
+                               static_cast<uint32_t>(half ? 4 * from.s_page : from.page),
+                               static_cast<uint32_t>(half ? 4 * from.s_token : from.token)};
+  }
+  const uint32_t k_off = own_row * static_cast<uint32_t>(c.k.token) + chunk;
+  const uint32_t v_off = own_row * static_cast<uint32_t>(c.v.token) + chunk;
+  constexpr int NP = kWhole ? 1 : NX;
+  auto key_of = [&](int t, int x) {  // one of the sequence in any case
+    if constexpr (kWhole) return clamp_int(t * kKeys + (my_key & ~(W - 1)), 0, (s.Lk - 1) & ~(W - 1));
+    return clamp_int(t * kKeys + RPI * x + row0, 0, s.Lk - 1);
+  };
+  struct Pages {
+    int p[NP];
+  };
+  auto pages_of = [&](int t) {
+    Pages r;
 #pragma unroll
-    for (int x = 0; x < NX; ++x) {
-      const int key = key_of(t, x);
-      const int at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
-      const int page = clamp_int(kWhole ? uniform_int(pages[x]) : pages[x], 0, a.paged.pages - 1);
-      // (of rows past the end the last one's)
-      int own = own_row;
-      if constexpr (kWhole) own = own < s.Lk - 1 - key ? own : s.Lk - 1 - key;
-      const uint8_t* kp = c.k.p + page * c.k.page + at * c.k.token + hk * c.k.head;
-      const uint8_t* vp = c.v.p + page * c.v.page + at * c.v.token + hk * c.v.head;
-      const float* ks = c.k.scale + page * c.k.s_page + at * c.k.s_token + hk * c.k.s_head;
-      const float* vs = c.v.scale + page * c.v.s_page + at * c.v.s_token + hk * c.v.s_head;
-      const uint32_t ko = (kWhole ? own * static_cast<uint32_t>(c.k.token) : 0u) + chunk;
-      const uint32_t vo = (kWhole ? own * static_cast<uint32_t>(c.v.token) : 0u) + chunk;
-      nk[x] = *reinterpret_cast<const u32x4*>(kp + ko);
-      nv[x] = *reinterpret_cast<const u32x4*>(vp + vo);
-      nks[x] = kWhole ? ks[own * c.k.s_token] : *ks;  // (the same for all of a row's threads)
-      nvs[x] = kWhole ? vs[own * c.v.s_token] : *vs;
+    for (int x = 0; x < NP; ++x) r.p[x] = a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, x), a.paged.page)];
+    return r;
+  };
+  auto load = [&](int t, const Pages& pages) {
+    if constexpr (kWhole) {
+      const int key = key_of(t, 0);
+      const uint32_t at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+      const uint32_t page = clamp_int(pages.p[0], 0, a.paged.pages - 1);
+      const u32x4 base = bases[threadIdx.x];
+      const uint64_t mine = (static_cast<uint64_t>(base[1]) << 32 | base[0]) + static_cast<uint64_t>(page) * base[2] +
+                            static_cast<uint64_t>(at) * base[3];
+      auto from = [&](int i) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine), i);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine >> 32), i);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+      };
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        nk[x] = *(gbl_u32x4*)(from(x) + k_off);
+        nv[x] = *(gbl_u32x4*)(from(NX + x) + v_off);
+      }
+      nks[0] = *(gbl_f32*)(mine);  // (of lanes below 32 the first of the codes)
+    } else {
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        const int key = key_of(t, x);
+        const int at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+        const int page = clamp_int(pages.p[x], 0, a.paged.pages - 1);
+        nk[x] = *reinterpret_cast<const u32x4*>(c.k.p + page * c.k.page + at * c.k.token + hk * c.k.head + chunk);
+        nv[x] = *reinterpret_cast<const u32x4*>(c.v.p + page * c.v.page + at * c.v.token + hk * c.v.head + chunk);
+        nks[x] = c.k.scale[page * c.k.s_page + at * c.k.s_token + hk * c.k.s_head];  // (the same for a row's threads)
+        nvs[x] = c.v.scale[page * c.v.s_page + at * c.v.s_token + hk * c.v.s_head];
+      }
     }
   };
   // (the order of a thread's two chunks takes turns: two lanes' first ones would meet)
   const bool turn = ch & 1;
   const int put0 = (2 * ch + (turn ? 1 : 0)) * kChunk + 16 * row0;
   const int put1 = (2 * ch + (turn ? 0 : 1)) * kChunk + 16 * row0;
-  auto put = [&](int buf) {
+  auto put = [&](int t, int buf) {
+    if (__builtin_expect((t + 1) * kKeys > s.Lk, 0)) {  // rows past the end hold anything
+#pragma unroll
+      for (int x = 0; x < NX; ++x) {
+        if (t * kKeys + RPI * x + row0 >= s.Lk) nv[x] = u32x4{0, 0, 0, 0};
+        if (t * kKeys + (kWhole ? my_key : RPI * x + row0) >= s.Lk) nks[x] = nvs[x] = 0.0f;
+      }
+    }
     lds_u8 *const kt = (lds_u8*)&g_code_tiles<DT>[buf][0][0], *const vt = (lds_u8*)&g_code_tiles<DT>[buf][1][0];
     auto turned = [&](const u32x4& w) { return turn ? u32x4{w[2], w[3], w[0], w[1]} : w; };
 #pragma unroll
@@ -655,9 +701,13 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
       widen16<kBF16, kCode>(turned(nv[x]), lo, hi);
       *(lds_u32x4*)(vt + put0 + 16 * RPI * x) = lo;
       *(lds_u32x4*)(vt + put1 + 16 * RPI * x) = hi;
-      scales[buf][row0 + RPI * x] = nks[x] * a.c;
-      scales[buf][kKeys + row0 + RPI * x] = nvs[x];
+      if constexpr (!kWhole) {
+        scales[buf][row0 + RPI * x] = nks[x] * a.c;
+        scales[buf][kKeys + row0 + RPI * x] = nvs[x];
+      }
     }
+    if constexpr (kWhole)
+      if (half) scales[buf][kKeys * values_of + my_key] = values_of ? nks[0] : nks[0] * a.c;
   };
 
   // where a lane reads: row lane % 32, channels 8 (lane / 32) .. of a product over
@@ -708,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
     };
     if (cut) mask(-INFINITY);
     code_step<kBF16, DT, 2>(
-        col, sc, room.e - kBias<kBF16>, [&](int kt2, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt2 + 8 * g + 4 * half); },
+        col, sc, static_cast<float>(room.e) - kBias<kBF16>, [&](int kt2, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt2 + 8 * g + 4 * half); },
         [&]() {
           if (cut) mask(0.0f);  // (a scale there may be NaN)
         },
@@ -724,33 +774,36 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   // A tile's entries of the block table are loaded before the rows of the tile
   // before it: loads return in order.
   if (t0 < t1) {
-    int p0[NX], p1[NX];
-#pragma unroll
-    for (int x = 0; x < NX; ++x) p0[x] = page_of(t0, x), p1[x] = page_of(t0 + 1, x);
+    Pages p0 = pages_of(t0), p1 = pages_of(t0 + 1);
     load(t0, p0);
-    put(0);
-#pragma unroll
-    for (int x = 0; x < NX; ++x) p0[x] = page_of(t0 + 2, x);
+    put(t0, 0);
+    p0 = pages_of(t0 + 2);
     load(t0 + 1, p1);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       const int buf = (t - t0) & 1;
       use(t, buf, [&]() {
-        put(buf ^ 1);
-#pragma unroll
-        for (int x = 0; x < NX; ++x) p1[x] = p0[x], p0[x] = page_of(t + 3, x);
+        put(t + 1, buf ^ 1);
+        p1 = p0;
+        p0 = pages_of(t + 3);
         load(t + 2, p1);
       });
       __syncthreads();
     }
   }
 
+  int again = threadIdx.x;
+  asm volatile("" : "+v"(again));  // (what stores need is made again: nothing of it is held over the loop)
+  const int r = tile * R + wave * 32 + (again & 31);
+  if (r >= rows) return;
+  const int tok = div_by(r, a.G);
+  const int head = hk * static_cast<int>(a.G.d) + (r - tok * static_cast<int>(a.G.d));
+  const int seen = last_key(a, s, tok) + 1;
   const int k0 = t0 * kKeys;
-  const int k1 = t1 * kKeys < limit + 1 ? t1 * kKeys : limit + 1;
+  const int k1 = t1 * kKeys < seen ? t1 * kKeys : seen;
   const bool none = k1 <= k0;
   const float l = half_sum(col.l);
   const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
-  if (!inside) return;
   if (half == 0 && a.splits > 1) store_part_stats(a, col.m, l, row, none, split);
   const float rl = none ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -857,7 +910,10 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   a.paged.most = static_cast<int>(plan::cached_most(width, page_size));
   a.paged.pages = static_cast<int>(pages);
   a.paged.page = fast_div(static_cast<uint32_t>(page_size));
+  // pages of whole 16s of tokens, and strides whose products with 32 bits are 64
   a.paged.whole = page_size % 16 == 0;
+  for (int64_t x : {k_page / 4, v_page / 4, ks_page, vs_page}) a.paged.whole &= x >= 0 && x < (int64_t{1} << 30);
+  for (int64_t x : {ks_token, vs_token}) a.paged.whole &= x >= 0 && x < (int64_t{1} << 25);
   a.cu_q = cu_q;
   a.B = static_cast<int>(B), a.T = static_cast<int>(T);
   a.H = static_cast<int>(H), a.Hk = static_cast<int>(Hk), a.D = static_cast<int>(D);
