@@ -71,45 +71,63 @@ struct CodeColumn {
   f32x16 o[DT / 32];
 };
 
-// Adds NK x 32 keys with scores s (scaled, -infinity where not seen) to the
-// column's sums; `ahead` is e less kBias.  `scale` gives the scales of the values of
-// keys 32 kt + 8 g + 4 (lane / 32) .. + 3; `drop` clears what belongs to keys that
-// the column does not see, where the tile has any.  `value` gives the operand of
-// value rows 16 ks .. of the tile, channels 32 db ...
-template <bool kBF16, int DT, int NK, class Scale, class Drop, class Value>
-__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, Scale&& scale, Drop&& drop,
-                                          Value&& value) {
+// Adds NK x 32 keys with products s to the column's sums; `ahead` is e less kBias.
+// `key_scale` and `value_scale` give the scales of keys 32 kt + 8 g + 4 (lane / 32) ..
+// + 3, those of keys times c; `hide` sets what belongs to keys that the column does
+// not see, where the tile has any.  `value` gives the operand of value rows 16 ks ..
+// of the tile, channels 32 db ...
+//
+// s ks - m is one instruction, with the m so far: its largest says whether m has to
+// be raised, and only then it is subtracted.
+template <bool kBF16, int DT, int NK, class KeyScale, class ValueScale, class Hide, class Value>
+__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, KeyScale&& key_scale,
+                                          ValueScale&& value_scale, Hide&& hide, Value&& value) {
+  const float m0 = col.m == kLowest ? 0.0f : col.m;  // (kLowest: no key seen)
+#pragma unroll
+  for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 ks = key_scale(kt, g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kt][4 * g + e] = fmaf(s[kt][4 * g + e], ks[e], -m0);
+    }
+  hide(-INFINITY);
   float t = s[0][0];
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);
   t = half_max(t) + ahead;
-  if (__builtin_expect(__ballot(t > col.m + kSlack) != 0, 0)) {
-    const float m = fmaxf(col.m, t);
+  if (__builtin_expect(__ballot(t > (col.m == kLowest ? kLowest : kSlack)) != 0, 0)) {
+    const float m = col.m == kLowest ? fmaxf(kLowest, t) : col.m + fmaxf(0.0f, t);
     const float alpha = __builtin_amdgcn_exp2f(col.m - m);
+    const float more = (m == kLowest ? 0.0f : m) - m0;
     col.m = m;
     col.l *= alpha;
 #pragma unroll
     for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
       for (int i = 0; i < 16; ++i) col.o[db][i] *= alpha;
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[kt][i] -= more;
   }
   float sum = 0.0f;
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const f32x4 vs = scale(kt, g);
+      const f32x4 vs = value_scale(kt, g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[kt][4 * g + e] - col.m);
+        const float p = __builtin_amdgcn_exp2f(s[kt][4 * g + e]);
         sum += p;
         s[kt][4 * g + e] = p * vs[e];
       }
     }
   col.l += sum;
-  drop();
+  hide(0.0f);  // (a scale there may be NaN)
 #pragma unroll
   for (int ks = 0; ks < 2 * NK; ++ks) {
     const u32x4 p = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
@@ -558,10 +576,10 @@ constexpr int kChunk = kKeys * 16 + 64;
 template <int DT>
 __shared__ __attribute__((aligned(1024))) uint8_t g_code_tiles[2][2][DT / 8 * kChunk];  // buffer; keys, values
 
-template <bool kBF16, int DT, int kCode, bool kWhole>
-__global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots) {
-  constexpr int R = 128;
-  constexpr int CH = DT / 16, RPI = 256 / CH, NX = kKeys / RPI;  // chunks of a row of codes, rows at a time
+template <bool kBF16, int DT, int kCode, int NW, bool kWhole>
+__global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int slots) {
+  constexpr int R = 32 * NW;
+  constexpr int CH = DT / 16, RPI = 64 * NW / CH, NX = kKeys / RPI;  // chunks of a row of codes, rows at a time
   const AttnArgs& a = c.a;
   __shared__ __attribute__((aligned(16))) float scales[2][2 * kKeys];  // keys', times c; then values'
   const int lane = threadIdx.x & 63, half = lane >> 5;
@@ -619,9 +637,9 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
   // of the time.)
   constexpr int W = 64 / CH;
   const int x_of = half ? lane / W % NX : lane % NX;
-  const int values_of = half ? (lane - 32) / (W * NX) : lane / NX % 2;
+  const int values_of = (half ? (lane - 32) / (W * NX) : lane / NX) % 2;
   const int my_key = RPI * x_of + wave_row + (half ? lane % W : 0);  // in the tile
-  __shared__ __attribute__((aligned(16))) u32x4 bases[kWhole ? 256 : 1];  // address; strides of pages and tokens
+  __shared__ __attribute__((aligned(16))) u32x4 bases[kWhole ? 64 * NW : 1];  // address; strides of pages and tokens
   if constexpr (kWhole) {
     const CodeRows& from = values_of ? c.v : c.k;
     const uint64_t base = half ? reinterpret_cast<uint64_t>(from.scale) + 4 * (hk * from.s_head + lane % W * from.s_token)
@@ -740,28 +758,19 @@ __global__ __launch_bounds__(256, 2) void code_rows_kernel(CodeArgs c, int slots
         sc[n] = mma32<kBF16>(k, q[d], sc[n]);
       }
     reads_ahead<DT / 8, 8>();
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 ks4 = *(lds_cf32x4*)(sl + 32 * n + 8 * g + 4 * half);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) sc[n][4 * g + e] *= ks4[e];
-      }
     const bool cut = key0 + kKeys - 1 > full;
-    auto mask = [&](float with) {
+    auto hide = [&](float with) {
+      if (!cut) return;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = with;
     };
-    if (cut) mask(-INFINITY);
     code_step<kBF16, DT, 2>(
-        col, sc, static_cast<float>(room.e) - kBias<kBF16>, [&](int kt2, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * kt2 + 8 * g + 4 * half); },
-        [&]() {
-          if (cut) mask(0.0f);  // (a scale there may be NaN)
-        },
+        col, sc, static_cast<float>(room.e) - kBias<kBF16>,
+        [&](int n, int g) { return *(lds_cf32x4*)(sl + 32 * n + 8 * g + 4 * half); },
+        [&](int n, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * n + 8 * g + 4 * half); }, hide,
         [&](int ks, int db) {
           s16x4 v[2];
 #pragma unroll
@@ -829,6 +838,13 @@ void launch_few(const CodeArgs& c, uint32_t grid, int slots, hipStream_t st) {
   else
     code_few_kernel<kBF16, DT, kCode, NQ, false><<<grid, 256, 0, st>>>(c, slots);
 }
+template <bool kBF16, int DT, int kCode, int NW>
+void launch_rows(const CodeArgs& c, uint32_t grid, int slots, hipStream_t st) {
+  if (c.a.paged.whole)
+    code_rows_kernel<kBF16, DT, kCode, NW, true><<<grid, 64 * NW, 0, st>>>(c, slots);
+  else
+    code_rows_kernel<kBF16, DT, kCode, NW, false><<<grid, 64 * NW, 0, st>>>(c, slots);
+}
 template <bool kBF16, int DT, int kCode>
 int launch(const CodeArgs& c, int R, hipStream_t st) {
   const AttnArgs& a = c.a;
@@ -840,10 +856,10 @@ int launch(const CodeArgs& c, int R, hipStream_t st) {
     launch_few<kBF16, DT, kCode, 1>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
   else if (R == 32)
     launch_few<kBF16, DT, kCode, 2>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
-  else if (a.paged.whole)
-    code_rows_kernel<kBF16, DT, kCode, true><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
-  else
-    code_rows_kernel<kBF16, DT, kCode, false><<<static_cast<uint32_t>(grid), 256, 0, st>>>(c, static_cast<int>(slots));
+  else if (R == 128)
+    launch_rows<kBF16, DT, kCode, 4>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
+  else if constexpr (DT == 128)
+    launch_rows<kBF16, DT, kCode, 8>(c, static_cast<uint32_t>(grid), static_cast<int>(slots), st);
   const int rc = check_launch("attention");
   if (rc != GPTQ_OK || a.splits == 1) return rc;
   return launch_join<kBF16>(a, st);
@@ -926,6 +942,6 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   const hipStream_t st = as_hip(stream);
   const bool wide = D > 64;
   if (dtype == GPTQ_BF16)
-    return wide ? launch_code<true, 128>(c, code, p.rows, st) : launch_code<true, 64>(c, code, p.rows, st);
-  return wide ? launch_code<false, 128>(c, code, p.rows, st) : launch_code<false, 64>(c, code, p.rows, st);
+    return wide ? launch_code<true, 128>(c, code, p.rows, st) : launch_code<true, 64>(c, code, p.rows > 128 ? 128 : p.rows, st);
+  return wide ? launch_code<false, 128>(c, code, p.rows, st) : launch_code<false, 64>(c, code, p.rows > 128 ? 128 : p.rows, st);
 }

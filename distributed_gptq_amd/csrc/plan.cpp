@@ -293,10 +293,10 @@ CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_cont
   CodePlan p;
   if (T == 0 || !attention_sizes(B, T, 0, H, Hk, 8)) return p;
   const int64_t rows = ceil_div(T * (H / Hk), B);  // of a sequence and key head, on average
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
+  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 128 ? 128 : 256;
   const int64_t groups = ceil_div(rows, p.rows) * B * Hk;
-  const int64_t want = p.rows < 128 && B > 8 ? 1024 : 512;  // workgroups
-  const int64_t most = ceil_div(std::max<int64_t>(max_context, 1), p.rows == 128 ? 512 : 128);
+  const int64_t want = p.rows < 128 && B > 8 ? 1024 : p.rows == 256 ? 256 : 512;  // workgroups
+  const int64_t most = ceil_div(std::max<int64_t>(max_context, 1), p.rows >= 128 ? 512 : 128);
   p.splits = static_cast<int>(std::min<int64_t>({ceil_div(want, groups), most, 128}));
   return p;
 }
