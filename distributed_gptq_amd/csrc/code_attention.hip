@@ -71,17 +71,16 @@ struct CodeColumn {
   f32x16 o[DT / 32];
 };
 
-// Adds NK x 32 keys with products s to the column's sums; `ahead` is e less kBias.
-// `key_scale` and `value_scale` give the scales of keys 32 kt + 8 g + 4 (lane / 32) ..
-// + 3, those of keys times c; `hide` sets what belongs to keys that the column does
-// not see, where the tile has any.  `value` gives the operand of value rows 16 ks ..
-// of the tile, channels 32 db ...
+// Makes the products s of NK x 32 keys into operands p of weights times scales;
+// `ahead` is e less kBias.  `key_scale` and `value_scale` give the scales of keys 32 kt
+// + 8 g + 4 (lane / 32) .. + 3, those of keys times c; `hide` sets what belongs to keys
+// that the column does not see, where the tile has any.
 //
 // s ks - m is one instruction, with the m so far: its largest says whether m has to
 // be raised, and only then it is subtracted.
-template <bool kBF16, int DT, int NK, class KeyScale, class ValueScale, class Hide, class Value>
-__device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], float ahead, KeyScale&& key_scale,
-                                          ValueScale&& value_scale, Hide&& hide, Value&& value) {
+template <bool kBF16, int DT, int NK, class KeyScale, class ValueScale, class Hide>
+__device__ __forceinline__ void code_weights(CodeColumn<DT>& col, f32x16 (&s)[NK], u32x4 (&p)[2 * NK], float ahead,
+                                             KeyScale&& key_scale, ValueScale&& value_scale, Hide&& hide) {
   const float m0 = col.m == kLowest ? 0.0f : col.m;  // (kLowest: no key seen)
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
@@ -121,19 +120,15 @@ __device__ __forceinline__ void code_step(CodeColumn<DT>& col, f32x16 (&s)[NK], 
       const f32x4 vs = value_scale(kt, g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(s[kt][4 * g + e]);
-        sum += p;
-        s[kt][4 * g + e] = p * vs[e];
+        const float w = __builtin_amdgcn_exp2f(s[kt][4 * g + e]);
+        sum += w;
+        s[kt][4 * g + e] = w * vs[e];
       }
     }
   col.l += sum;
   hide(0.0f);  // (a scale there may be NaN)
 #pragma unroll
-  for (int ks = 0; ks < 2 * NK; ++ks) {
-    const u32x4 p = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
-#pragma unroll
-    for (int db = 0; db < DT / 32; ++db) col.o[db] = mma32<kBF16>(value(ks, db), p, col.o[db]);
-  }
+  for (int ks = 0; ks < 2 * NK; ++ks) p[ks] = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
 }
 
 // 16 codes as two operands of 8 values.
@@ -581,7 +576,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   constexpr int R = 32 * NW;
   constexpr int CH = DT / 16, RPI = 64 * NW / CH, NX = kKeys / RPI;  // chunks of a row of codes, rows at a time
   const AttnArgs& a = c.a;
-  __shared__ __attribute__((aligned(16))) float scales[2][2 * kKeys];  // keys', times c; then values'
+  __shared__ __attribute__((aligned(16))) float scales[4][2 * kKeys + 32];  // of tile t at t % 4: keys', times c; then values'
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int hk = blockIdx.x % a.Hk;
@@ -638,7 +633,8 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   constexpr int W = 64 / CH;
   const int x_of = half ? lane / W % NX : lane % NX;
   const int values_of = (half ? (lane - 32) / (W * NX) : lane / NX) % 2;
-  const int my_key = RPI * x_of + wave_row + (half ? lane % W : 0);  // in the tile
+  // in the tile, or for codes of values in the tile before it
+  const int my_key = RPI * x_of + wave_row + (half ? lane % W : values_of ? -kKeys : 0);
   __shared__ __attribute__((aligned(16))) u32x4 bases[kWhole ? 64 * NW : 1];  // address; strides of pages and tokens
   if constexpr (kWhole) {
     const CodeRows& from = values_of ? c.v : c.k;
@@ -650,10 +646,10 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   }
   const uint32_t k_off = own_row * static_cast<uint32_t>(c.k.token) + chunk;
   const uint32_t v_off = own_row * static_cast<uint32_t>(c.v.token) + chunk;
-  constexpr int NP = kWhole ? 1 : NX;
+  constexpr int NP = kWhole ? 1 : 2 * NX;
   auto key_of = [&](int t, int x) {  // one of the sequence in any case
     if constexpr (kWhole) return clamp_int(t * kKeys + (my_key & ~(W - 1)), 0, (s.Lk - 1) & ~(W - 1));
-    return clamp_int(t * kKeys + RPI * x + row0, 0, s.Lk - 1);
+    return clamp_int((t - x / NX) * kKeys + RPI * (x % NX) + row0, 0, s.Lk - 1);
   };
   struct Pages {
     int p[NP];
@@ -664,6 +660,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     for (int x = 0; x < NP; ++x) r.p[x] = a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, x), a.paged.page)];
     return r;
   };
+  // the keys of tile t and the values of tile t - 1, and the scales of tile t
   auto load = [&](int t, const Pages& pages) {
     if constexpr (kWhole) {
       const int key = key_of(t, 0);
@@ -686,11 +683,16 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     } else {
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
-        const int key = key_of(t, x);
-        const int at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
-        const int page = clamp_int(pages.p[x], 0, a.paged.pages - 1);
+        auto place = [&](int i, int64_t& page, int64_t& at) {
+          const int key = key_of(t, i);
+          at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+          page = clamp_int(pages.p[i], 0, a.paged.pages - 1);
+        };
+        int64_t page, at, v_page, v_at;
+        place(x, page, at);
+        place(NX + x, v_page, v_at);
         nk[x] = *reinterpret_cast<const u32x4*>(c.k.p + page * c.k.page + at * c.k.token + hk * c.k.head + chunk);
-        nv[x] = *reinterpret_cast<const u32x4*>(c.v.p + page * c.v.page + at * c.v.token + hk * c.v.head + chunk);
+        nv[x] = *reinterpret_cast<const u32x4*>(c.v.p + v_page * c.v.page + v_at * c.v.token + hk * c.v.head + chunk);
         nks[x] = c.k.scale[page * c.k.s_page + at * c.k.s_token + hk * c.k.s_head];  // (the same for a row's threads)
         nvs[x] = c.v.scale[page * c.v.s_page + at * c.v.s_token + hk * c.v.s_head];
       }
@@ -700,32 +702,40 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   const bool turn = ch & 1;
   const int put0 = (2 * ch + (turn ? 1 : 0)) * kChunk + 16 * row0;
   const int put1 = (2 * ch + (turn ? 0 : 1)) * kChunk + 16 * row0;
-  auto put = [&](int t, int buf) {
-    if (__builtin_expect((t + 1) * kKeys > s.Lk, 0)) {  // rows past the end hold anything
+  auto put = [&](lds_u8* to, const u32x4& w, int x) {
+    u32x4 lo, hi;
+    widen16<kBF16, kCode>(turn ? u32x4{w[2], w[3], w[0], w[1]} : w, lo, hi);
+    *(lds_u32x4*)(to + put0 + 16 * RPI * x) = lo;
+    *(lds_u32x4*)(to + put1 + 16 * RPI * x) = hi;
+  };
+  // (of lanes without a scale to a place that nothing reads)
+  const int scale_at = kWhole && !half ? 2 * kKeys + lane : kKeys * values_of + my_key;
+  const float scale_by = values_of ? 1.0f : a.c;
+  auto put_scales = [&](int t) {  // those past the end are zeros
+    if constexpr (kWhole) {
+      scales[t & 3][scale_at] = t * kKeys + my_key < s.Lk ? nks[0] * scale_by : 0.0f;
+    } else {
 #pragma unroll
       for (int x = 0; x < NX; ++x) {
-        if (t * kKeys + RPI * x + row0 >= s.Lk) nv[x] = u32x4{0, 0, 0, 0};
-        if (t * kKeys + (kWhole ? my_key : RPI * x + row0) >= s.Lk) nks[x] = nvs[x] = 0.0f;
+        const bool some = t * kKeys + RPI * x + row0 < s.Lk;
+        scales[t & 3][row0 + RPI * x] = some ? nks[x] * a.c : 0.0f;
+        scales[t & 3][kKeys + row0 + RPI * x] = some ? nvs[x] : 0.0f;
       }
     }
-    lds_u8 *const kt = (lds_u8*)&g_code_tiles<DT>[buf][0][0], *const vt = (lds_u8*)&g_code_tiles<DT>[buf][1][0];
-    auto turned = [&](const u32x4& w) { return turn ? u32x4{w[2], w[3], w[0], w[1]} : w; };
+  };
+  auto clear_values = [&](int t) {  // rows past the end hold anything
+    if (__builtin_expect((t + 1) * kKeys > s.Lk, 0)) {
+#pragma unroll
+      for (int x = 0; x < NX; ++x)
+        if (t * kKeys + RPI * x + row0 >= s.Lk) nv[x] = u32x4{0, 0, 0, 0};
+    }
+  };
+  auto put_rows = [&](int t) {  // the keys of tile t, the values of tile t - 1
 #pragma unroll
     for (int x = 0; x < NX; ++x) {
-      u32x4 lo, hi;
-      widen16<kBF16, kCode>(turned(nk[x]), lo, hi);
-      *(lds_u32x4*)(kt + put0 + 16 * RPI * x) = lo;
-      *(lds_u32x4*)(kt + put1 + 16 * RPI * x) = hi;
-      widen16<kBF16, kCode>(turned(nv[x]), lo, hi);
-      *(lds_u32x4*)(vt + put0 + 16 * RPI * x) = lo;
-      *(lds_u32x4*)(vt + put1 + 16 * RPI * x) = hi;
-      if constexpr (!kWhole) {
-        scales[buf][row0 + RPI * x] = nks[x] * a.c;
-        scales[buf][kKeys + row0 + RPI * x] = nvs[x];
-      }
+      put((lds_u8*)&g_code_tiles<DT>[t & 1][0][0], nk[x], x);
+      put((lds_u8*)&g_code_tiles<DT>[t & 1 ^ 1][1][0], nv[x], x);
     }
-    if constexpr (kWhole)
-      if (half) scales[buf][kKeys * values_of + my_key] = values_of ? nks[0] : nks[0] * a.c;
   };
 
   // where a lane reads: row lane % 32, channels 8 (lane / 32) .. of a product over
@@ -733,11 +743,22 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   int krow = half * kChunk + 16 * (lane & 31);
   int vrow = (2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * kChunk + 16 * (4 * half + ((lane & 15) >> 2)) + 8 * (lane & 1);
   asm volatile("" : "+v"(krow), "+v"(vrow));  // (so that the constant parts go into the instructions)
-  auto use = [&](int t, int buf, auto&& meanwhile) {
+  f32x16 sc[2];
+  u32x4 p[4];
+  auto keys_times_queries = [&](int t) {
+    const lds_u8* const kt = (const lds_u8*)&g_code_tiles<DT>[t & 1][0][0] + krow;
+    sc[0] = sc[1] = zero16();
+#pragma unroll
+    for (int d = 0; d < DT / 16; ++d)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const u32x4 k = *(const lds_u32x4*)(kt + 2 * d * kChunk + 512 * n);
+        sc[n] = mma32<kBF16>(k, q[d], sc[n]);
+      }
+  };
+  auto weights = [&](int t) {
     const int key0 = t * kKeys;
-    const lds_u8* const kt = (const lds_u8*)&g_code_tiles<DT>[buf][0][0] + krow;
-    const lds_u8* const vt = (const lds_u8*)&g_code_tiles<DT>[buf][1][0] + vrow;
-    const lds_f32* const sl = (const lds_f32*)&scales[buf][0];
+    const lds_f32* const sl = (const lds_f32*)&scales[t & 3][0];
     const float vs = sl[kKeys + lane];
     if (__builtin_expect(lacks_room(room, vs), 0)) {
       const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
@@ -748,16 +769,6 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
 #pragma unroll
         for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
     }
-    meanwhile();
-    f32x16 sc[2] = {zero16(), zero16()};
-#pragma unroll
-    for (int d = 0; d < DT / 16; ++d)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const u32x4 k = *(const lds_u32x4*)(kt + 2 * d * kChunk + 512 * n);
-        sc[n] = mma32<kBF16>(k, q[d], sc[n]);
-      }
-    reads_ahead<DT / 8, 8>();
     const bool cut = key0 + kKeys - 1 > full;
     auto hide = [&](float with) {
       if (!cut) return;
@@ -765,40 +776,87 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (key0 + 32 * n + acc_row(i, half) > limit) sc[n][i] = with;
+          if (32 * n + acc_row(i, 0) > limit - key0 - 4 * half) sc[n][i] = with;
     };
-    code_step<kBF16, DT, 2>(
-        col, sc, static_cast<float>(room.e) - kBias<kBF16>,
+    code_weights<kBF16, DT, 2>(
+        col, sc, p, static_cast<float>(room.e) - kBias<kBF16>,
         [&](int n, int g) { return *(lds_cf32x4*)(sl + 32 * n + 8 * g + 4 * half); },
-        [&](int n, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * n + 8 * g + 4 * half); }, hide,
-        [&](int ks, int db) {
-          s16x4 v[2];
+        [&](int n, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * n + 8 * g + 4 * half); }, hide);
+  };
+  auto weights_times_values = [&](int t) {
+    const lds_u8* const vt = (const lds_u8*)&g_code_tiles<DT>[t & 1][1][0] + vrow;
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
-            v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + 4 * db * kChunk + 256 * ks + 128 * j));
-          return __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
-        });
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int db = 0; db < DT / 32; ++db) {
+        s16x4 v[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + 4 * db * kChunk + 256 * ks + 128 * j));
+        const u32x4 value = __builtin_bit_cast(u32x4, __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7));
+        col.o[db] = mma32<kBF16>(value, p[ks], col.o[db]);
+      }
   };
 
-  // A tile's entries of the block table are loaded before the rows of the tile
-  // before it: loads return in order.
+  // Phases between barriers: a wave makes a tile's weights (vector instructions), then
+  // multiplies them with the values and the next keys with the queries (matrix
+  // instructions) and stages its part of later tiles meanwhile.  Of 8 waves the second
+  // four, each of which shares a SIMD with one of the first, are a phase behind: one of
+  // both has the matrix unit while the other one has the vector unit.
+  //
+  // Keys of tile t are read in phases 2 t and 2 t + 1 and written in 2 t - 2 and 2 t -
+  // 1, values read in 2 t + 2 and 2 t + 3 and written in 2 t and 2 t + 1 (by the first
+  // four, then by the others), each over what was read last a phase before.  Scales of
+  // tile t, written like its keys, are read until 2 t + 2.
+  //
+  // A tile's entries of the block table are loaded before the rows of the tile before
+  // it: loads return in order.
   if (t0 < t1) {
+    const bool late = NW == 8 && wave >= 4;
     Pages p0 = pages_of(t0), p1 = pages_of(t0 + 1);
+    auto stage = [&](int t) {  // tile t's keys, tile t - 1's values, and the loads of the next ones
+      clear_values(t - 1);
+      put_scales(t);
+      put_rows(t);
+      p0 = p1;
+      p1 = pages_of(t + 2);
+      load(t + 1, p0);
+    };
     load(t0, p0);
-    put(t0, 0);
-    p0 = pages_of(t0 + 2);
-    load(t0 + 1, p1);
+    stage(t0);
+    stage(t0 + 1);
+    __syncthreads();
+    if (late) __syncthreads();
+    keys_times_queries(t0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
-      const int buf = (t - t0) & 1;
-      use(t, buf, [&]() {
-        put(t + 1, buf ^ 1);
-        p1 = p0;
-        p0 = pages_of(t + 3);
-        load(t + 2, p1);
+      weights(t);
+      __syncthreads();
+      clear_values(t + 1);
+      put_scales(t + 2);
+      __builtin_amdgcn_s_setprio(1);
+      weights_times_values(t);
+      keys_times_queries(t + 1);
+      put_rows(t + 2);
+      p0 = p1;
+      p1 = pages_of(t + 4);
+      load(t + 3, p0);
+      // the order: kAhead reads first, so that no product waits for one just issued
+      constexpr int kAhead = 12;
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+      sfor<0, DT / 8 - kAhead / 2>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       });
+      sfor<0, DT / 8>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      });
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead / 2, 0);
+      __builtin_amdgcn_s_setprio(0);
       __syncthreads();
     }
+    if (NW == 8 && !late) __syncthreads();
   }
 
   int again = threadIdx.x;
