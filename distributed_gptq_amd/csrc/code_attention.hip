@@ -660,15 +660,18 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     for (int x = 0; x < NP; ++x) r.p[x] = a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, x), a.paged.page)];
     return r;
   };
+  auto address_of = [&](int t, const Pages& pages) {  // kWhole: the lane's
+    if constexpr (!kWhole) return uint64_t{0};
+    const int key = key_of(t, 0);
+    const uint32_t at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+    const uint32_t page = clamp_int(pages.p[0], 0, a.paged.pages - 1);
+    const u32x4 base = bases[threadIdx.x];
+    return (static_cast<uint64_t>(base[1]) << 32 | base[0]) + static_cast<uint64_t>(page) * base[2] +
+           static_cast<uint64_t>(at) * base[3];
+  };
   // the keys of tile t and the values of tile t - 1, and the scales of tile t
-  auto load = [&](int t, const Pages& pages) {
+  auto load = [&](int t, const Pages& pages, uint64_t mine) {
     if constexpr (kWhole) {
-      const int key = key_of(t, 0);
-      const uint32_t at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
-      const uint32_t page = clamp_int(pages.p[0], 0, a.paged.pages - 1);
-      const u32x4 base = bases[threadIdx.x];
-      const uint64_t mine = (static_cast<uint64_t>(base[1]) << 32 | base[0]) + static_cast<uint64_t>(page) * base[2] +
-                            static_cast<uint64_t>(at) * base[3];
       auto from = [&](int i) {
         const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine), i);
         const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(mine >> 32), i);
@@ -756,10 +759,17 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
         sc[n] = mma32<kBF16>(k, q[d], sc[n]);
       }
   };
+  f32x4 ks[8];  // the scales of a tile's keys, and of values one a lane
+  float vs;
+  auto read_scales = [&](int t) {
+    const lds_f32* const sl = (const lds_f32*)&scales[t & 3][0];
+    vs = sl[kKeys + lane];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ks[i] = *(lds_cf32x4*)(sl + 8 * i + 4 * half);
+  };
   auto weights = [&](int t) {
     const int key0 = t * kKeys;
     const lds_f32* const sl = (const lds_f32*)&scales[t & 3][0];
-    const float vs = sl[kKeys + lane];
     if (__builtin_expect(lacks_room(room, vs), 0)) {
       const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
       col.m += more;
@@ -780,7 +790,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     };
     code_weights<kBF16, DT, 2>(
         col, sc, p, static_cast<float>(room.e) - kBias<kBF16>,
-        [&](int n, int g) { return *(lds_cf32x4*)(sl + 32 * n + 8 * g + 4 * half); },
+        [&](int n, int g) { return ks[4 * n + g]; },
         [&](int n, int g) { return *(lds_cf32x4*)(sl + kKeys + 32 * n + 8 * g + 4 * half); }, hide);
   };
   auto weights_times_values = [&](int t) {
@@ -820,39 +830,51 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
       put_rows(t);
       p0 = p1;
       p1 = pages_of(t + 2);
-      load(t + 1, p0);
+      load(t + 1, p0, address_of(t + 1, p0));
     };
-    load(t0, p0);
+    load(t0, p0, address_of(t0, p0));
     stage(t0);
     stage(t0 + 1);
     __syncthreads();
     if (late) __syncthreads();
     keys_times_queries(t0);
+    read_scales(t0);
     __syncthreads();
     for (int t = t0; t < t1; ++t) {
       weights(t);
+      p0 = p1;
+      p1 = pages_of(t + 4);
+      uint64_t next = address_of(t + 3, p0);
+      asm volatile("" : "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]), "+v"(col.l), "+v"(next));  // (all in this phase)
       __syncthreads();
       clear_values(t + 1);
       put_scales(t + 2);
       __builtin_amdgcn_s_setprio(1);
-      weights_times_values(t);
-      keys_times_queries(t + 1);
-      put_rows(t + 2);
-      p0 = p1;
-      p1 = pages_of(t + 4);
-      load(t + 3, p0);
-      // the order: kAhead reads first, so that no product waits for one just issued
+      // reads ahead of the products, so that none waits for one just issued; the writes,
+      // which pass no read, between both products
       constexpr int kAhead = 12;
+      weights_times_values(t);
       __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
       sfor<0, DT / 8 - kAhead / 2>([](auto) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
       });
-      sfor<0, DT / 8>([](auto) {
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead / 2, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      put_rows(t + 2);
+      load(t + 3, p0, next);
+      __builtin_amdgcn_sched_barrier(0);
+      keys_times_queries(t + 1);
+      read_scales(t + 1);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead / 2, 0);
+      sfor<0, DT / 8 - kAhead / 2>([](auto) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
       });
-      __builtin_amdgcn_sched_group_barrier(0x008, kAhead / 2, 0);
+      sfor<0, kAhead / 2>([](auto) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      });
       __builtin_amdgcn_s_setprio(0);
       __syncthreads();
     }
