@@ -782,11 +782,13 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     const bool cut = key0 + kKeys - 1 > full;
     auto hide = [&](float with) {
       if (!cut) return;
+      int last_seen = limit - key0 - 4 * half;
+      asm volatile("" : "+v"(last_seen));  // (so that the comparisons stay behind the branch)
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * n + acc_row(i, 0) > limit - key0 - 4 * half) sc[n][i] = with;
+          if (32 * n + acc_row(i, 0) > last_seen) sc[n][i] = with;
     };
     code_weights<kBF16, DT, 2>(
         col, sc, p, static_cast<float>(room.e) - kBias<kBF16>,
