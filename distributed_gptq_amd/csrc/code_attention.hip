@@ -993,7 +993,7 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   for (int64_t x : {k_token, v_token})  // (16 tokens' offsets are 32 bits)
     GPTQ_REQUIRE(x < (int64_t{1} << 27), GPTQ_ERR_SHAPE, "%s: tokens of codes have to be less than 2^27 apart (got %lld)", fn,
                  static_cast<long long>(x));
-  const plan::CodePlan p = plan::code_plan(B, T, H, Hk, max_context);
+  const plan::CodePlan p = plan::code_plan(B, T, H, Hk, D, max_context);
   const size_t need = plan::code_workspace(B, T, H, Hk, D, max_context);
   GPTQ_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), GPTQ_ERR_WORKSPACE,
                "%s: workspace of %zu bytes, needs %zu", fn, workspace_bytes, need);
@@ -1024,6 +1024,6 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   const hipStream_t st = as_hip(stream);
   const bool wide = D > 64;
   if (dtype == GPTQ_BF16)
-    return wide ? launch_code<true, 128>(c, code, p.rows, st) : launch_code<true, 64>(c, code, p.rows > 128 ? 128 : p.rows, st);
-  return wide ? launch_code<false, 128>(c, code, p.rows, st) : launch_code<false, 64>(c, code, p.rows > 128 ? 128 : p.rows, st);
+    return wide ? launch_code<true, 128>(c, code, p.rows, st) : launch_code<true, 64>(c, code, p.rows, st);
+  return wide ? launch_code<false, 128>(c, code, p.rows, st) : launch_code<false, 64>(c, code, p.rows, st);
 }

@@ -108,12 +108,12 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context);
 size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context);
-// The same over a cache of codes: rows of a workgroup (16, 32 or 128) and parts.
+// The same over a cache of codes: rows of a workgroup (16, 32, 128 or 256) and parts.
 struct CodePlan {
   int rows = 16;
   int splits = 1;
 };
-CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t max_context);
+CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context);
 size_t code_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context);
 // The gradient: workgroups of the first kernel, into how many parts the query
 // rows of each 64 keys are cut, and the workspace.
