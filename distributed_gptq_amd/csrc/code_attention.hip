@@ -297,39 +297,93 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
   const int from = 16 * (row >> 3) + 4 * quarter + ((row >> 1) & 3);
   const int get = from * DT + (code_slot<DT>(from) << 4) + ((row & 1) << 3);
 
-  // The block table's entries of a tile: of its halves, or of the lane's two rows.
-  // They are loaded a tile before the rows are, and before the rows of the tile
-  // between: loads return in order, so that a wait for an entry does not wait for
-  // rows.
+  // kWhole: a lane of quarter i has of half i % 2 of a tile the keys (i < 2) or the
+  // values, and makes the address of their codes, for all lanes, and of its row's
+  // scale.  What it needs, base and strides of pages and tokens, is in LDS where the
+  // registers do not suffice.
+  constexpr bool kBasesHeld = NQ > 1;
+  __shared__ __attribute__((aligned(16))) u32x4 bases[kWhole && !kBasesHeld ? 512 : 1];
+  u32x4 base0, base1;
+  if constexpr (kWhole) {
+    const CodeRows& from = quarter >= 2 ? c.v : c.k;
+    const uint64_t codes = reinterpret_cast<uint64_t>(from.p) + hk * from.head;
+    const uint64_t first = reinterpret_cast<uint64_t>(from.scale) + 4 * (hk * from.s_head + row * from.s_token);
+    base0 = u32x4{static_cast<uint32_t>(codes), static_cast<uint32_t>(codes >> 32), static_cast<uint32_t>(from.page),
+                  static_cast<uint32_t>(from.token)};
+    base1 = u32x4{static_cast<uint32_t>(first), static_cast<uint32_t>(first >> 32), static_cast<uint32_t>(4 * from.s_page),
+                  static_cast<uint32_t>(4 * from.s_token)};
+    if constexpr (!kBasesHeld) bases[threadIdx.x] = base0, bases[256 + threadIdx.x] = base1;
+  }
+  auto base_of = [&](int i) {
+    if constexpr (kBasesHeld) return i ? base1 : base0;
+    return bases[256 * i + threadIdx.x];
+  };
+
+  // The block table's entries of a tile: of the lane's half, or of its two rows.  They
+  // are loaded a tile before the rows are, and before the rows of the tile between:
+  // loads return in order, so that a wait for an entry does not wait for rows.
+  constexpr int NP = kWhole ? 1 : 2;
+  struct Pages {
+    int p[NP];
+  };
   auto key_of = [&](int t, int n) {  // a half's first key, or the lane's: one of the sequence in any case
-    if constexpr (kWhole) return clamp_int(t * kFew + 16 * n, 0, (s.Lk - 1) & ~15);
+    if constexpr (kWhole) return clamp_int(t * kFew + 16 * (quarter & 1), 0, (s.Lk - 1) & ~15);
     return clamp_int(t * kFew + 16 * n + row, 0, s.Lk - 1);
   };
-  auto page_of = [&](int t, int n) {
-    return a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, n), a.paged.page)];
+  auto pages_of = [&](int t) {
+    Pages r;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) r.p[n] = a.paged.table[s.b * a.paged.table_stride + div_by(key_of(t, n), a.paged.page)];
+    return r;
   };
   // A tile's rows.  Every lane loads in any case, of tiles past the last one the
   // same few bytes: with loads under a branch the compiler waits for all of them
   // where it could wait for the older ones.
-  auto load = [&](u32x4 (&k)[2][NX], u32x4 (&v)[2][NX], float& scale, int t, const int (&pages)[2]) {
+  auto load = [&](u32x4 (&k)[2][NX], u32x4 (&v)[2][NX], float& scale, int t, const Pages& pages) {
     const bool some = t < t1;
     const uint32_t keep = some ? ~0u : 0u;
     const uint64_t none = reinterpret_cast<uint64_t>(&g_no_codes[0]);
-    int page[2], at[2];
-    uint64_t kp[2], vp[2];
+    uint64_t kp[2], vp[2], sp;
+    uint32_t krow = 0, vrow = 0;
+    if constexpr (kWhole) {
+      const int key = key_of(t, 0);
+      const uint32_t at = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+      const uint32_t page = clamp_int(pages.p[0], 0, a.paged.pages - 1);
+      auto address = [&](int i) {
+        const u32x4 x = base_of(i);
+        const uint64_t to = (static_cast<uint64_t>(x[1]) << 32 | x[0]) + static_cast<uint64_t>(page) * x[2] +
+                            static_cast<uint64_t>(at) * x[3];
+        return some ? to : none;
+      };
+      const uint64_t codes = address(0);
+      sp = address(1);
+      auto from = [&](int i) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(codes), 16 * i);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(codes >> 32), 16 * i);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+      };
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int key = key_of(t, n);
-      at[n] = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
-      page[n] = clamp_int(kWhole ? uniform_int(pages[n]) : pages[n], 0, a.paged.pages - 1);
-      kp[n] = reinterpret_cast<uint64_t>(c.k.p) + page[n] * c.k.page + at[n] * c.k.token + hk * c.k.head;
-      vp[n] = reinterpret_cast<uint64_t>(c.v.p) + page[n] * c.v.page + at[n] * c.v.token + hk * c.v.head;
-      kp[n] = some ? kp[n] : none;
-      vp[n] = some ? vp[n] : none;
-      if constexpr (kWhole) kp[n] = uniform_u64(kp[n]), vp[n] = uniform_u64(vp[n]);
+      for (int n = 0; n < 2; ++n) kp[n] = from(n), vp[n] = from(2 + n);
+      krow = row * static_cast<uint32_t>(c.k.token), vrow = row * static_cast<uint32_t>(c.v.token);
+    } else {
+      int page[2], at[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = key_of(t, n);
+        at[n] = key - div_by(key, a.paged.page) * static_cast<int>(a.paged.page.d);
+        page[n] = clamp_int(pages.p[n], 0, a.paged.pages - 1);
+        kp[n] = reinterpret_cast<uint64_t>(c.k.p) + page[n] * c.k.page + at[n] * c.k.token + hk * c.k.head;
+        vp[n] = reinterpret_cast<uint64_t>(c.v.p) + page[n] * c.v.page + at[n] * c.v.token + hk * c.v.head;
+        kp[n] = some ? kp[n] : none;
+        vp[n] = some ? vp[n] : none;
+      }
+      // quarters 0 and 1: the keys' scales of the two halves, 2 and 3: the values'
+      const int pg = quarter & 1 ? page[1] : page[0], to = quarter & 1 ? at[1] : at[0];
+      const bool values = quarter >= 2;
+      const int64_t i = pg * (values ? c.v.s_page : c.k.s_page) + to * (values ? c.v.s_token : c.k.s_token) +
+                        hk * (values ? c.v.s_head : c.k.s_head);
+      sp = some ? reinterpret_cast<uint64_t>(values ? c.v.scale : c.k.scale) + 4 * i : none;
     }
-    const uint32_t krow = kWhole ? row * static_cast<uint32_t>(c.k.token) : 0u;
-    const uint32_t vrow = kWhole ? row * static_cast<uint32_t>(c.v.token) : 0u;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -338,20 +392,13 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int x = 0; x < NX; ++x) v[n][x] = *(gbl_u32x4*)(vp[n] + ((vrow + chunk[x]) & keep));
-    // quarters 0 and 1: the keys' scales of the two halves, 2 and 3: the values'
-    const int pg = quarter & 1 ? page[1] : page[0];
-    const int to = (quarter & 1 ? at[1] : at[0]) + (kWhole ? row : 0);
-    const bool values = quarter >= 2;
-    const int64_t i = pg * (values ? c.v.s_page : c.k.s_page) + to * (values ? c.v.s_token : c.k.s_token) +
-                      hk * (values ? c.v.s_head : c.k.s_head);
-    const uint64_t sp = reinterpret_cast<uint64_t>(values ? c.v.scale : c.k.scale) + 4 * i;
-    scale = *(gbl_f32*)(some ? sp : none);
+    scale = *(gbl_f32*)sp;
   };
   // Uses a tile's rows, and has the next one's loaded into their registers as soon
   // as these are free: the loads are in flight for the larger part of a tile's time.
   u32x4 k[2][NX], v[2][NX];
   float scale;
-  auto use = [&](int t, const int (&next)[2]) {
+  auto use = [&](int t, const Pages& next) {
     const int key0 = t * kFew;
     if (key0 + kFew > s.Lk) {  // rows past the end hold anything
 #pragma unroll
@@ -484,11 +531,11 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
   };
   const int first = t0 + wave;
   if (first < t1) {
-    int p0[2] = {page_of(first, 0), page_of(first, 1)}, p1[2] = {page_of(first + 4, 0), page_of(first + 4, 1)};
+    Pages p0 = pages_of(first), p1 = pages_of(first + 4);
     load(k, v, scale, first, p0);
     for (int t = first; t < t1; t += 4) {
-      p0[0] = p1[0], p0[1] = p1[1];
-      p1[0] = page_of(t + 8, 0), p1[1] = page_of(t + 8, 1);
+      p0 = p1;
+      p1 = pages_of(t + 8);
       use(t, p0);
     }
   }
