@@ -37,7 +37,7 @@ struct NormArgs {
   int interleaved;
   // a thread's work: `per` heads of one kind of a token
   int per, gq, gk;
-  FastDiv groups;
+  FastDiv groups, tokens;
   // the gradient
   HeadRows grad_q, grad_k;
   void *dq, *dk;                     // (T, heads, D)
@@ -136,9 +136,8 @@ __device__ __forceinline__ void load_weights(const void* w, int type, const Unit
 }
 
 // 1 / sqrt(mean of squares + eps) of a row (the hardware's, to a unit of the last
-// place).  Squares of values past 2^64 leave
-// fp32: the row's sum is made again of values 2^-80 as large, beside whose
-// squares eps is nothing.
+// place).  Squares of values past 2^64 leave fp32: the row's sum is made again of
+// values 2^-80 as large, beside whose squares eps is nothing.
 template <int N>
 __device__ __forceinline__ float rms_inverse(const float (&x)[N], const float (&y)[N], const NormArgs& a, int lanes) {
   float ss = 0.0f;
@@ -161,10 +160,10 @@ __device__ __forceinline__ float rms_inverse(const float (&x)[N], const float (&
 // value that is not finite reads back as NaN: its scale is one.
 template <int N, int kType, int kStore>
 __device__ __forceinline__ void store_cached(const CacheRows& r, int64_t page, int64_t at, int h, const Unit<N>& unit,
-                                             const float (&x)[N], const float (&y)[N], int lanes, int u, bool kept) {
+                                             const float (&x)[N], const float (&y)[N], int lanes, int u) {
   const int64_t o = page * r.page + at * r.token + h * r.head;
   if constexpr (kStore == 0) {
-    if (!kept || !unit.some) return;
+    if (!unit.some) return;
     store_pairs<N, kType>(r.p, o + unit.first, x);
     store_pairs<N, kType>(r.p, o + unit.second, y);
   } else {
@@ -177,7 +176,7 @@ __device__ __forceinline__ void store_cached(const CacheRows& r, int64_t page, i
     const bool finite = most < INFINITY;
     const bool some = finite && most > kLeast;
     const float inv = some ? top / most : 0.0f;
-    if (!kept || !unit.some) return;
+    if (!unit.some) return;
     uint8_t* to = static_cast<uint8_t*>(r.p) + o;
     typedef uint32_t words __attribute__((ext_vector_type(N / 4)));
     words w0, w1;
@@ -199,26 +198,31 @@ __device__ __forceinline__ void store_cached(const CacheRows& r, int64_t page, i
 // is read and written once, and 16 waves of a CU (128 registers) hide the loads
 // better than fewer with the next heads' loads ahead.  16384 tokens of 32 + 8 heads
 // of 128 bf16 values (336 MB): 66 us, 5.1 TB/s, 71 us with two heads at once, 83 us
-// with a head per thread.
+// with a head per thread.  2048 tokens of 40 + 40 + 40 heads of 128 fp16 values into
+// e4m3 (106 MB): 33 us, 3.2 TB/s, the tokens of a head in neighbouring rows so that
+// their scales and codes fill lines (38 us by tokens).  One token: 4.4 us, the launch.
 template <int N, int kType, int kStore>
 __global__ __launch_bounds__(256, 4) void norm_rotary_kernel(NormArgs a, int lanes) {
   const int rows = 256 / lanes;
   const int u = threadIdx.x & (lanes - 1);
   const int64_t id = static_cast<int64_t>(blockIdx.x) * rows + threadIdx.x / lanes;
   if (id >= static_cast<int64_t>(a.T) * a.groups.d) return;
-  const int t = div_by(static_cast<int>(id), a.groups);
+  // a token's groups lie next to each other, but in a cache a head's tokens do
+  int t = div_by(static_cast<int>(id), a.groups);
   int g = static_cast<int>(id) - t * static_cast<int>(a.groups.d);
+  if (a.slots) {
+    g = div_by(static_cast<int>(id), a.tokens);
+    t = static_cast<int>(id) - g * a.T;
+  }
   const int kind = g < a.gq ? 0 : g < a.gq + a.gk ? 1 : 2;
   g -= kind == 0 ? 0 : kind == 1 ? a.gq : a.gq + a.gk;
   const int heads = kind == 0 ? a.H : a.Hk;
   const int h0 = g * a.per, h1 = h0 + a.per < heads ? h0 + a.per : heads;
   const HeadRows from = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
   int64_t page = 0, at = t;
-  bool kept = true;
   if (kind != 0 && a.slots) {
     const int slot = a.slots[t];
-    kept = slot >= 0 && slot < a.capacity;
-    if (!kept) return;
+    if (slot < 0 || slot >= a.capacity) return;
     page = div_by(slot, a.page);
     at = slot - page * static_cast<int64_t>(a.page.d);
   }
@@ -251,7 +255,7 @@ __global__ __launch_bounds__(256, 4) void norm_rotary_kernel(NormArgs a, int lan
         store_pairs<N, kType>(to, o + unit.second, y);
       }
     } else {
-      store_cached<N, kType, kStore>(kind == 1 ? a.kc : a.vc, page, at, h, unit, x, y, lanes, u, kept);
+      store_cached<N, kType, kStore>(kind == 1 ? a.kc : a.vc, page, at, h, unit, x, y, lanes, u);
     }
   }
 }
@@ -384,6 +388,7 @@ int launch(NormArgs a, const char* fn, hipStream_t st) {
   a.gq = (a.H + a.per - 1) / a.per;
   a.gk = (a.Hk + a.per - 1) / a.per;
   a.groups = fast_div(static_cast<uint32_t>(a.gq + (a.v.p ? 2 : 1) * a.gk));
+  a.tokens = fast_div(static_cast<uint32_t>(a.T));
   const int64_t items = static_cast<int64_t>(a.T) * a.groups.d;
   GPTQ_REQUIRE(items < (int64_t{1} << 31), GPTQ_ERR_SHAPE, "%s: too many tokens", fn);
   norm_rotary_kernel<N, kType, kStore><<<static_cast<uint32_t>(cdiv(items, 256 / lanes)), 256, 0, st>>>(a, lanes);
