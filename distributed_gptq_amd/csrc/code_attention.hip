@@ -1070,7 +1070,9 @@ extern "C" int gptq_code_attention(const void* q, int dtype, int64_t q_token, in
   a.paged.most = static_cast<int>(plan::cached_most(width, page_size));
   a.paged.pages = static_cast<int>(pages);
   a.paged.page = fast_div(static_cast<uint32_t>(page_size));
-  // pages of whole 16s of tokens, and strides whose products with 32 bits are 64
+  // Pages of whole 16s of tokens, and strides whose products with 32 bits are 64:
+  // addresses by lanes.  Pages of 16 / 24 tokens (us): 512 tokens over 16896 152 / 162,
+  // one over 131072 55.3 / 56.8.
   a.paged.whole = page_size % 16 == 0;
   for (int64_t x : {k_page / 4, v_page / 4, ks_page, vs_page}) a.paged.whole &= x >= 0 && x < (int64_t{1} << 30);
   for (int64_t x : {ks_token, vs_token}) a.paged.whole &= x >= 0 && x < (int64_t{1} << 25);
