@@ -293,14 +293,18 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
 // but leave more of them empty (us, heads 32 over 8 of 128, 128 rows / 256 rows: 256
 // new tokens for each of 4 sequences over 4096 91.3 / 87.8, 80 for each 61.4 / 51.0,
 // 64 for each of 4 over 2048 37.6 / 38.6, 40 of one over 8192 30.5 / 34.2, 32 for
-// each of 16 over 2048 43.5 / 49.9).  Of few rows, 512 workgroups or twice that of
-// many sequences (us with the join, 512 / 1024 wanted: 24 sequences of 1 to 8192
-// tokens 51.6 / 43.5, 8 of 2048 14.9 / 16.0, one of 131072 55.4 / 57.2).
+// each of 16 over 2048 43.5 / 49.9).  Of 33 to 64 rows, two tiles of 32 / one of 128:
+// 16 new tokens for each of 8 sequences over 4096 32.7 / 34.6, of one over 8192 23.4 /
+// 25.3, for each of 32 over 2048 65.8 / 57.7.
+//
+// Of few rows, 512 workgroups or twice that of many sequences (us with the join, 512 /
+// 1024 wanted: 24 sequences of 1 to 8192 tokens 51.8 / 43.3, 8 of 2048 15.0 / 19.2,
+// one of 131072 55.8 / 60.6).
 CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context) {
   CodePlan p;
   if (T == 0 || !attention_sizes(B, T, 0, H, Hk, D)) return p;
   const int64_t rows = ceil_div(T * (H / Hk), B);  // of a sequence and key head, on average
-  p.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 256 || D <= 64 ? 128 : 256;
+  p.rows = rows <= 16 ? 16 : rows <= (B <= 8 ? 64 : 32) ? 32 : rows <= 256 || D <= 64 ? 128 : 256;
   const int64_t groups = ceil_div(rows, p.rows) * B * Hk;
   const int64_t want = p.rows < 128 && B > 8 ? 1024 : p.rows == 256 ? 256 : 512;  // workgroups
   const int64_t most = ceil_div(std::max<int64_t>(max_context, 1), p.rows >= 128 ? 512 : 128);

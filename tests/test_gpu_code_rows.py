@@ -144,3 +144,30 @@ def test_pages_far_apart(new, bits):
         q = (torch.randn(n, H, D, generator=g, device="cuda") * 2).to(dtype)
         got = A().paged_attention(q, kc, vc, table[b:b + 1], ints([c]), offsets([n]), **s)
         check(got, attended(q, *rows))
+
+
+@pytest.mark.parametrize("code", [1, 2])
+@pytest.mark.parametrize("used,T", [(2, 40), (0, 7), (300, 700), (40, 41), (90, 130)])
+def test_rows_behind_the_last_sequence_are_zeros(used, T, code):
+    """A padded batch: whatever the output held."""
+    from distributed_gptq_amd import _lib
+    H, Hk, D, page, pages = 4, 2, 128, 16, 40
+    g = gen(T)
+    q = torch.randn(T, H, D, generator=g, device="cuda").half()
+    q[used:] = math.nan
+    kc, vc = (torch.randint(-5, 6, (pages, page, Hk, D), generator=g, device="cuda").to(torch.int8) for _ in "kv")
+    if code == 2:
+        kc, vc = (x.float().to(torch.float8_e4m3fn).view(torch.int8) for x in (kc, vc))
+    ks, vs = (torch.full((pages, page, Hk), 0.01, device="cuda") for _ in "kv")
+    table = torch.randperm(pages, generator=g, device="cuda").int()[None]
+    cu, ctx = ints([0, used]), ints([600])
+    for longest in (1, 640):
+        out = torch.full((T, H, D), math.nan, dtype=torch.float16, device="cuda")
+        n = _lib.lib().gptq_code_attention_workspace_size(1, T, H, Hk, D, longest)
+        ws = torch.full((max(n, 1),), 0xFF, dtype=torch.uint8, device="cuda")
+        _lib.call("gptq_code_attention", ptr(q), 1, *strides(q), code, ptr(kc), *kc.stride()[:3], ptr(vc), *vc.stride()[:3],
+                  ptr(ks), *ks.stride(), ptr(vs), *vs.stride(), ptr(table), pages, pages, page, pages, ptr(ctx), ptr(cu), 1, T,
+                  H, Hk, D, 0.1, longest, ptr(out), ptr(ws), n, torch.cuda.current_stream().cuda_stream)
+        assert bool((out[used:] == 0).all()) and bool(torch.isfinite(out[:used]).all())
+        if used:
+            assert bool((out[:used] != 0).any(-1).all())
