@@ -799,7 +799,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
 #pragma unroll
     for (int x = 0; x < NX; ++x) {
       put((lds_u8*)&g_code_tiles<DT>[t & 1][0][0], nk[x], x);
-      put((lds_u8*)&g_code_tiles<DT>[t & 1 ^ 1][1][0], nv[x], x);
+      put((lds_u8*)&g_code_tiles<DT>[(t & 1) ^ 1][1][0], nv[x], x);
     }
   };
 

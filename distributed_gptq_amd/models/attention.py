@@ -203,7 +203,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     ``k_scale`` and ``v_scale``: those of a cache of codes (``rotary_append``),
     whose rows are code times scale; q is fp16 or bf16.  A row whose scale is NaN
-    reaches the queries that see it only."""
+    reaches the queries that see it only.  A value's code that is NaN, which
+    ``rotary_append`` never writes, may reach those before it too."""
     if _needs_grad(q, k_cache, v_cache):
         raise RuntimeError("paged_attention records no gradient: call it under torch.no_grad()")
     if max_context is None:
@@ -376,11 +377,10 @@ class QuantizedAttention(nn.Module):
 
     ``forward`` runs whole packed sequences, for prompts, calibration and
     training; ``step`` runs new tokens over a ``PagedKVCache``, a quantised one
-    too.  Both raise
-    ValueError where the host knows that a position is past the table: one
-    sequence longer than it, a step whose longest context is.  Sequences by
-    ``cu_seqlens`` and given positions are not looked at; positions past the
-    table are turned by its last angles."""
+    too.  Both raise ValueError where the host knows that a position is past the
+    table: one sequence longer than it, a step whose longest context is.
+    Sequences by ``cu_seqlens`` and given positions are not looked at; positions
+    past the table are turned by its last angles."""
 
     def __init__(self, qkv: nn.Module, o: nn.Module, heads: int, kv_heads: int, head_dim: int,
                  table: Optional[torch.Tensor] = None, interleaved: bool = False, scale: Optional[float] = None,
