@@ -256,11 +256,8 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     for (int x = 0; x < 2 * NX; ++x) {
       const int d = 64 * (x / 2) + 16 * quarter + 8 * (x % 2);
       q[n][x] = inside && d < a.D ? *reinterpret_cast<const u32x4*>(qrow + d) : u32x4{0, 0, 0, 0};
-      if constexpr (!kHeld)
-        if (wave == x % 4) queries[2 * NX * n + x][lane] = q[n][x];  // (the waves' are the same)
     }
   }
-  if constexpr (!kHeld) __syncthreads();
   auto query = [&](int n, int x) {
     if constexpr (kHeld) return q[n][x];
     return queries[2 * NX * n + x][lane];
@@ -537,14 +534,23 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     wave_sync();
   };
   const int first = t0 + wave;
+  Pages p0, p1;
   if (first < t1) {
-    Pages p0 = pages_of(first), p1 = pages_of(first + 4);
+    p0 = pages_of(first), p1 = pages_of(first + 4);
     load(k, v, scale, first, p0);
-    for (int t = first; t < t1; t += 4) {
-      p0 = p1;
-      p1 = pages_of(t + 8);
-      use(t, p0);
-    }
+  }
+  if constexpr (!kHeld) {  // (while the first rows are on their way)
+#pragma unroll
+    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+      for (int x = 0; x < 2 * NX; ++x)
+        if (wave == x % 4) queries[2 * NX * n + x][lane] = q[n][x];  // (the waves' are the same)
+    __syncthreads();
+  }
+  for (int t = first; t < t1; t += 4) {
+    p0 = p1;
+    p1 = pages_of(t + 8);
+    use(t, p0);
   }
   // a column's sums of this wave as a weighted mean, and the log2 of its weights
   float lse[NQ];
