@@ -29,7 +29,7 @@ struct CodeArgs {
 };
 
 // fp16 weights are kept 2^7 times larger than 2^(s - m), which is at most
-// 2^kSlack: above their smallest and below their largest value (attention.hip).
+// 2^kSlack (of many rows their sums of 32 are): above their smallest and below their largest value (attention.hip).
 constexpr float kSlack = 8.0f;
 template <bool kBF16>
 constexpr float kBias = kBF16 ? 0.0f : 7.0f;
@@ -76,8 +76,10 @@ struct CodeColumn {
 // + 8 g + 4 (lane / 32) .. + 3, those of keys times c; `hide` sets what belongs to keys
 // that the column does not see, where the tile has any.
 //
-// s ks - m is one instruction, with the m so far: its largest says whether m has to
-// be raised, and only then it is subtracted.
+// s ks - m is one instruction, with the m so far, and the sum of the weights that it
+// gives is made in any case: where that is small enough for each of them, m stays.
+// Otherwise, and where no key was seen before, the largest score is looked for and m
+// raised to it.
 template <bool kBF16, int DT, int NK, class KeyScale, class ValueScale, class Hide>
 __device__ __forceinline__ void code_weights(CodeColumn<DT>& col, f32x16 (&s)[NK], u32x4 (&p)[2 * NK], float ahead,
                                              KeyScale&& key_scale, ValueScale&& value_scale, Hide&& hide) {
@@ -90,14 +92,27 @@ __device__ __forceinline__ void code_weights(CodeColumn<DT>& col, f32x16 (&s)[NK
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[kt][4 * g + e] = fmaf(s[kt][4 * g + e], ks[e], -m0);
     }
-  hide(-INFINITY);
-  float t = s[0][0];
+  hide(s, -INFINITY);
+  f32x16 w[NK];
+  float sum;
+  auto weigh = [&]() {
+    sum = 0.0f;
 #pragma unroll
-  for (int kt = 0; kt < NK; ++kt)
+    for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);
-  t = half_max(t) + ahead;
-  if (__builtin_expect(__ballot(t > (col.m == kLowest ? kLowest : kSlack)) != 0, 0)) {
+      for (int i = 0; i < 16; ++i) {
+        w[kt][i] = __builtin_amdgcn_exp2f(s[kt][i]);
+        sum += w[kt][i];
+      }
+  };
+  weigh();
+  if (__builtin_expect(__ballot(col.m == kLowest || sum > __builtin_amdgcn_exp2f(kSlack - ahead)) != 0, 0)) {
+    float t = s[0][0];
+#pragma unroll
+    for (int kt = 0; kt < NK; ++kt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t = __builtin_elementwise_maximum(t, s[kt][i]);
+    t = half_max(t) + ahead;
     const float m = col.m == kLowest ? fmaxf(kLowest, t) : col.m + fmaxf(0.0f, t);
     const float alpha = __builtin_amdgcn_exp2f(col.m - m);
     const float more = (m == kLowest ? 0.0f : m) - m0;
@@ -111,24 +126,20 @@ __device__ __forceinline__ void code_weights(CodeColumn<DT>& col, f32x16 (&s)[NK
     for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[kt][i] -= more;
+    weigh();
   }
-  float sum = 0.0f;
+  col.l += sum;
 #pragma unroll
   for (int kt = 0; kt < NK; ++kt)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const f32x4 vs = value_scale(kt, g);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float w = __builtin_amdgcn_exp2f(s[kt][4 * g + e]);
-        sum += w;
-        s[kt][4 * g + e] = w * vs[e];
-      }
+      for (int e = 0; e < 4; ++e) w[kt][4 * g + e] *= vs[e];
     }
-  col.l += sum;
-  hide(0.0f);  // (a scale there may be NaN)
+  hide(w, 0.0f);  // (a scale there may be NaN)
 #pragma unroll
-  for (int ks = 0; ks < 2 * NK; ++ks) p[ks] = operand_of<kBF16>(s[ks / 2], 8 * (ks % 2));
+  for (int ks = 0; ks < 2 * NK; ++ks) p[ks] = operand_of<kBF16>(w[ks / 2], 8 * (ks % 2));
 }
 
 // 16 codes as two operands of 8 values.
@@ -630,10 +641,11 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 // Bound by issue: of a tile of 32 queries and 64 keys the products hold the matrix
 // unit for 1024 cycles and, for about half of these, the vector unit's port; the
 // weights take it for 1200 (32 exponentials a lane are 512 of them).  Measured, 512
-// new tokens over 16896, heads 32 over 8 of 128, bf16 over e4m3 (140 GFLOP): 146 us
-// and 8 us for the join, 909 TFLOP/s; 177 us with 128 rows and all waves in step,
-// 161 us with 256 rows in step.  Cycles of a tile: 1980 for its
-// weights, 1700 for its products and staging, 450 at both barriers.
+// new tokens over 16896, heads 32 over 8 of 128, bf16 over e4m3 (140 GFLOP): 144 us
+// and 8 us for the join, 915 TFLOP/s; with the join 177 us with 128 rows and all waves
+// in step, 161 us with 256 rows in step, 154.6 us with the largest score looked for in
+// every tile.  Cycles of a tile: 1900 for its weights, 1700 for its products and
+// staging, 450 at both barriers.
 constexpr int kKeys = 64;
 constexpr int kChunk = kKeys * 16 + 64;
 template <int DT>
@@ -848,7 +860,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
         for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
     }
     const bool cut = key0 + kKeys - 1 > full;
-    auto hide = [&](float with) {
+    auto hide = [&](f32x16 (&x)[2], float with) {
       if (!cut) return;
       int last_seen = limit - key0 - 4 * half;
       asm volatile("" : "+v"(last_seen));  // (so that the comparisons stay behind the branch)
@@ -856,7 +868,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (32 * n + acc_row(i, 0) > last_seen) sc[n][i] = with;
+          if (32 * n + acc_row(i, 0) > last_seen) x[n][i] = with;
     };
     code_weights<kBF16, DT, 2>(
         col, sc, p, static_cast<float>(room.e) - kBias<kBF16>,
