@@ -644,8 +644,8 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 // new tokens over 16896, heads 32 over 8 of 128, bf16 over e4m3 (140 GFLOP): 144 us
 // and 8 us for the join, 915 TFLOP/s; with the join 177 us with 128 rows and all waves
 // in step, 161 us with 256 rows in step, 154.6 us with the largest score looked for in
-// every tile.  Cycles of a tile: 1900 for its weights, 1700 for its products and
-// staging, 450 at both barriers.
+// every tile.  Cycles of a tile (of the last of these): 1980 for its weights, 1700 for
+// its products and staging, 450 at both barriers.
 constexpr int kKeys = 64;
 constexpr int kChunk = kKeys * 16 + 64;
 template <int DT>
