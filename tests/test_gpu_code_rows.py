@@ -9,7 +9,7 @@ import torch
 from attention_check import check
 from code_check import attended
 from test_gpu_attention_guards import FAR, Room, ints, ptr, strides
-from test_gpu_code_cache import A, CODES, TYPES, case, expect, gen
+from test_gpu_code_cache import A, CODES, TYPES, case, expect, gen, random_rows
 from test_gpu_paged_attention import offsets
 
 pytestmark = pytest.mark.gpu
@@ -171,3 +171,60 @@ def test_rows_behind_the_last_sequence_are_zeros(used, T, code):
         assert bool((out[used:] == 0).all()) and bool(torch.isfinite(out[:used]).all())
         if used:
             assert bool((out[:used] != 0).any(-1).all())
+
+
+# ------------------------------------------------- more than 2^31 elements --
+
+def test_norms_past_32_bits():
+    """The rows of a long call are those of short ones, bit for bit, with gradients."""
+    T, H, D = 66000, 256, 128
+    g = gen(1)
+    q = torch.empty(T, H, D, dtype=torch.bfloat16, device="cuda").uniform_(-2, 2, generator=g)
+    k = torch.randn(T, 1, D, generator=g, device="cuda").bfloat16()
+    w, w2 = (torch.rand(D, generator=g, device="cuda") + 0.5 for _ in "qk")
+    table, pos = A().rotary_table(D, 100), torch.arange(T, device="cuda", dtype=torch.int32) % 100
+    qo, ko = A().norm_rotary(q, k, w, w2, table, pos)
+    dq, dk, *_ = torch.ops.gptq.norm_rotary_backward(q.flip(0), k, q, k, w, w2, table, pos, False, 1e-6, False)
+    for rows in (slice(0, 3), slice(65530, 65542), slice(T - 3, T)):
+        one = [x[rows].contiguous() for x in (q, k)]
+        want = A().norm_rotary(*one, w, w2, table, pos[rows])
+        assert torch.equal(qo[rows], want[0]) and torch.equal(ko[rows], want[1])
+        grad = q.flip(0)[rows].contiguous()
+        back = torch.ops.gptq.norm_rotary_backward(grad, one[1], *one, w, w2, table, pos[rows], False, 1e-6, False)
+        assert torch.equal(dq[rows], back[0]) and torch.equal(dk[rows], back[1])
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_rows_past_32_bits(code):
+    T, Hk, D, page, pages = 1_100_000, 16, 128, 16, 64
+    g = gen(2)
+    kc, vc = (torch.randint(-100, 100, (pages, page, Hk, D), generator=g, device="cuda").to(torch.int8) for _ in "kv")
+    if code != torch.int8:
+        kc, vc = (x.float().to(code) for x in (kc, vc))
+    ks, vs = (torch.rand(pages, page, Hk, generator=g, device="cuda") for _ in "kv")
+    width = T // page + 1
+    table = torch.randint(0, pages, (1, width), generator=g, device="cuda", dtype=torch.int32)
+    k, v = A().cached_rows(kc, vc, table, ints([T]), ints([0, T]), T, k_scale=ks, v_scale=vs)
+    for rows in (torch.arange(5), torch.arange(2 ** 20 - 5, 2 ** 20 + 5), torch.arange(T - 5, T)):
+        place = (table[0].long().cpu()[rows // page], rows % page)
+        rows = rows.cuda()
+        for got, c, s in ((k, kc, ks), (v, vc, vs)):
+            place = tuple(x.cuda() for x in place)
+            assert torch.equal(got[rows], (c.float()[place] * s[place][..., None]).bfloat16())
+
+
+@pytest.mark.parametrize("code", CODES)
+def test_attention_past_32_bits(code):
+    """One token for each of very many sequences."""
+    B, H, Hk, D, page, pages = 140_000, 128, 16, 128, 16, 64
+    g = gen(3)
+    rows = [random_rows(g, pages * page, Hk, D, code) for _ in "kv"]
+    (kc, ks), (vc, vs) = ((c.view(pages, page, Hk, D), s.view(pages, page, Hk)) for c, s in rows)
+    table = torch.randint(0, pages, (B, 2), generator=g, device="cuda", dtype=torch.int32)
+    ctx = torch.randint(1, 33, (B,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.empty(B, H, D, dtype=torch.float16, device="cuda").uniform_(-2, 2, generator=g)
+    out = A().paged_attention(q, kc, vc, table, ctx, max_context=32, k_scale=ks, v_scale=vs)
+    for b in (0, 1, 131071, 131072, B - 1):
+        j = torch.arange(int(ctx[b]), device="cuda")
+        place = (table[b].long()[j // page], j % page)
+        check(out[b:b + 1], attended(q[b:b + 1], kc[place], ks[place], vc[place], vs[place]))
