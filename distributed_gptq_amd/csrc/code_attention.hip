@@ -153,12 +153,14 @@ __device__ __forceinline__ void widen16(const u32x4& w, u32x4& lo, u32x4& hi) {
 }
 
 // A part's statistics of a row, whose sums are divided already: a weight of 1 at
-// the maximum m + log2 l.  Of a sum that is NaN the weight is NaN.
+// the maximum m + log2 l.  Of a sum that is NaN (m may be too) the weight is NaN, at a
+// maximum that is a number: the join passes over one that is not, and takes a row
+// without any for one that sees no key.
 __device__ __forceinline__ void store_part_stats(const AttnArgs& a, float m, float l, int64_t row, bool none, int split) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.H;
   float* mm = a.part + a.splits * rows * a.D;
   const bool number = l == l;
-  mm[split * rows + row] = none ? -INFINITY : number ? m + log2f(l) : m;
+  mm[split * rows + row] = none ? -INFINITY : number ? m + log2f(l) : kLowest;
   mm[(a.splits + split) * rows + row] = none ? 0.0f : number ? 1.0f : l;
 }
 

@@ -1,0 +1,77 @@
+"""Attention over codes of rows whose sums are not finite: against 64 bits, and the
+same with contexts in one part and in many."""
+import math
+
+import pytest
+import torch
+
+from attention_check import check
+from code_check import attended
+from test_gpu_attention_guards import ints
+from test_gpu_code_cache import case, empty_cache, expect, gen
+from test_gpu_paged_attention import offsets
+
+pytestmark = pytest.mark.gpu
+CODES = [torch.int8, torch.float8_e4m3fn]
+TYPES = [torch.bfloat16, torch.float16]
+PAGE = 16
+
+
+def A():
+    from distributed_gptq_amd.models import attention
+    return attention
+
+
+def places(table, b, n):
+    j = torch.arange(n, device="cuda")
+    return table[b].long()[j // PAGE], j % PAGE
+
+
+# ------------------------------------------------------- sums that are no numbers --
+# (one part, 2, up to 8 and more: for few rows a part has at least 128 keys, for
+# many 512)
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,context", [(1, 100), (1, 200), (1, 900), (1, 5000), (12, 200), (12, 5000), (100, 600), (100, 3000),
+                                         (100, 9000)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_queries_that_are_not_finite(new, context, bad, dtype, code):
+    """One head of one token: its output is NaN, whatever the number of parts,
+    and no other one changes."""
+    q, kc, vc, table, s, rows = case((new,), (context,), PAGE, 4, 2, 128, dtype, code)
+    want = expect(q, rows, (new,))
+    q = q.clone()
+    t, h = new // 2, 3
+    q[t, h, 17] = bad
+    for longest in (None, 1, 16 * context):
+        got = A().paged_attention(q, kc, vc, table, ints([context]), offsets([new]), max_context=longest, **s)
+        assert bool(got[t, h].isnan().all())
+        got[t, h] = 0
+        y, b = (x.clone() for x in want)
+        y[t, h], b[t, h] = 0, 0
+        check(got, (y, b))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,context", [(1, 1), (1, 40), (5, 100), (20, 90), (70, 70), (140, 500)])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+def test_a_scale_that_is_nan_in_a_short_sequence(which, new, context, dtype, code):
+    """All keys in one part of many: NaN for the rows that see the key, the same
+    rows whatever max_context says."""
+    q, kc, vc, table, s, rows = case((new, 3), (context, 9), PAGE, 4, 2, 64, dtype, code)
+    y, b = expect(q, rows, (new, 3))
+    cu, ctx = offsets([new, 3]), ints([context, 9])
+    for key in {0, context // 2, context - 1}:
+        x = s[which].clone()
+        x[table[0].long()[key // PAGE], key % PAGE, 1] = math.nan
+        sees = torch.arange(context - new, context, device="cuda") >= key
+        sees = torch.cat([sees, torch.zeros(3, dtype=torch.bool, device="cuda")])
+        for longest in (1, 300, 1000, 100000):
+            got = A().paged_attention(q, kc, vc, table, ctx, cu, max_context=longest, **{**s, which: x})
+            assert bool(got[sees][:, 2:].isnan().all())
+            got[sees, 2:] = 0
+            yy, bb = y.clone(), b.clone()
+            yy[sees, 2:], bb[sees, 2:] = 0, 0
+            check(got, (yy, bb))
