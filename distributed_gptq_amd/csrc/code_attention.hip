@@ -153,15 +153,21 @@ __device__ __forceinline__ void widen16(const u32x4& w, u32x4& lo, u32x4& hi) {
 }
 
 // A part's statistics of a row, whose sums are divided already: a weight of 1 at
-// the maximum m + log2 l.  Of a sum that is NaN (m may be too) the weight is NaN, at a
-// maximum that is a number: the join passes over one that is not, and takes a row
-// without any for one that sees no key.
+// the maximum m + log2 l.  Of a sum l that is 0 (all its scores -infinity) or NaN (m may
+// be too) that is the weight, at the lowest maximum: the join adds the first to other
+// parts without a trace and makes NaN of a row that has no others, and it passes over a
+// maximum that is no number, and takes a row without any for one that sees no key.
 __device__ __forceinline__ void store_part_stats(const AttnArgs& a, float m, float l, int64_t row, bool none, int split) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.H;
   float* mm = a.part + a.splits * rows * a.D;
-  const bool number = l == l;
-  mm[split * rows + row] = none ? -INFINITY : number ? m + log2f(l) : kLowest;
-  mm[(a.splits + split) * rows + row] = none ? 0.0f : number ? 1.0f : l;
+  const bool some = l > 0.0f;
+  mm[split * rows + row] = none ? -INFINITY : some ? m + log2f(l) : kLowest;
+  mm[(a.splits + split) * rows + row] = none ? 0.0f : some ? 1.0f : l;
+}
+// What a row's sums of values are divided by, as a factor; a part whose weights are all
+// 0 leaves zeros.
+__device__ __forceinline__ float inverse_sum(const AttnArgs& a, float l, bool none) {
+  return none || (l == 0.0f && a.splits > 1) ? 0.0f : 1.0f / l;
 }
 
 // -------------------------------------------------------------- few rows ----
@@ -613,7 +619,7 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
   constexpr int N = DT * R / 256;  // channels of a thread
   const int d0 = (threadIdx.x / R) * N;
   if (threadIdx.x < R && a.splits > 1) store_part_stats(a, top, sum, out_row, none, split);
-  const float inv = none ? 0.0f : 1.0f / sum;
+  const float inv = inverse_sum(a, sum, none);
 #pragma unroll
   for (int d = 0; d < N; d += 4) {
     if (d0 + d >= a.D) break;
@@ -978,7 +984,7 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
   const float l = half_sum(col.l);
   const int64_t row = static_cast<int64_t>(s.q0 + tok) * a.H + head;
   if (half == 0 && a.splits > 1) store_part_stats(a, col.m, l, row, none, split);
-  const float rl = none ? 0.0f : 1.0f / l;
+  const float rl = inverse_sum(a, l, none);
 #pragma unroll
   for (int db = 0; db < DT / 32; ++db)
 #pragma unroll

@@ -75,3 +75,29 @@ def test_a_scale_that_is_nan_in_a_short_sequence(which, new, context, dtype, cod
             yy, bb = y.clone(), b.clone()
             yy[sees, 2:], bb[sees, 2:] = 0, 0
             check(got, (yy, bb))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new,context,past", [(1, 300, 128), (1, 300, 200), (1, 5000, 1500), (12, 300, 128), (100, 1300, 600),
+                                              (100, 5000, 2600)])
+def test_scores_of_minus_infinity(new, context, past, dtype, code):
+    """The first keys' scores are below fp32's range: their weights are 0, in parts
+    that have no other keys too.  Where all are, there is no mean: NaN."""
+    q, kc, vc, table, s, rows = case((new,), (context,), PAGE, 4, 2, 64, dtype, code)
+    q = q.clone()
+    q[:, :, 0] = -60000.0
+    k, ks, v, vs = rows[0]
+    k, ks = k.view(torch.int8).clone(), ks.clone()
+    k[:, :, 0] = 0
+    k[:past] = 0
+    k[:past, :, 0] = 0x70            # 112, or e4m3's 128
+    ks[:past] = 2.0 ** 120           # -60000 * 112 * 2^120 / 8 is past -2^128
+    at = places(table, 0, context)
+    kc.view(torch.int8)[at], s["k_scale"][at] = k, ks
+    want = attended(q, k[past:].view(code), ks[past:], v[past:], vs[past:])
+    for longest in (None, 1):
+        check(A().paged_attention(q, kc, vc, table, ints([context]), offsets([new]), max_context=longest, **s), want)
+    for longest in (None, 1):
+        got = A().paged_attention(q, kc, vc, table, ints([past]), offsets([new]), max_context=longest, **s)
+        assert bool(got.isnan().all())
