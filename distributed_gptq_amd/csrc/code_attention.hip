@@ -51,18 +51,20 @@ __device__ __forceinline__ float uniform_float(float v) { return __int_as_float(
 // `vs`: a scale of each lane's (0 for none); those that are not finite are no
 // reason for another e.
 __device__ __forceinline__ bool lacks_room(const ScaleRoom& r, float vs) { return __ballot(vs > r.cap && vs < INFINITY) != 0; }
-// Raises e, by how much it returns.
+// Raises e, by how much it returns.  That is up to 200: the sums are made so much
+// smaller by ldexpf, since no factor of fp32 is (2^-149 is the last), while a sum of
+// weights, 2^-e and more, stays one.
 template <bool kBF16>
-__device__ __forceinline__ float make_room(ScaleRoom& r, float vs) {
+__device__ __forceinline__ int make_room(ScaleRoom& r, float vs) {
   float top = vs > 0.0f && vs < INFINITY ? vs : 0.0f;
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor(top, s));
-  if (top == 0.0f) return 0.0f;  // (scales of 0 need no e)
+  if (top == 0.0f) return 0;  // (scales of 0 need no e)
   const int e = uniform_int(clamp_int(ilogbf(top) + 1, kLeastE, kMostE<kBF16>));
   const int more = e - r.e;
   r.e = e;
   r.cap = uniform_float(e == kMostE<kBF16> ? INFINITY : ldexpf(1.0f, e + kScaleRoom<kBF16>));
-  return static_cast<float>(more);
+  return more;
 }
 
 template <int DT>
@@ -439,15 +441,15 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
     sc_lds[lane] = quarter >= 2 ? scale : scale * a.c;
     const float vs = quarter >= 2 ? scale : 0.0f;
     if (__builtin_expect(lacks_room(room, vs), 0)) {
-      const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
+      const int more = make_room<kBF16>(room, vs);
 #pragma unroll
       for (int n = 0; n < NQ; ++n) {
-        m[n] += more;
-        l[n] *= less;
+        m[n] += static_cast<float>(more);
+        l[n] = __builtin_amdgcn_ldexpf(l[n], -more);
 #pragma unroll
         for (int x = 0; x < NB; ++x)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[n][x][e] *= less;
+          for (int e = 0; e < 4; ++e) o[n][x][e] = __builtin_amdgcn_ldexpf(o[n][x][e], -more);
       }
     }
 
@@ -859,13 +861,13 @@ __global__ __launch_bounds__(64 * NW, 2) void code_rows_kernel(CodeArgs c, int s
     const int key0 = t * kKeys;
     const lds_f32* const sl = (const lds_f32*)&scales[t & 3][0];
     if (__builtin_expect(lacks_room(room, vs), 0)) {
-      const float more = make_room<kBF16>(room, vs), less = __builtin_amdgcn_exp2f(-more);
-      col.m += more;
-      col.l *= less;
+      const int more = make_room<kBF16>(room, vs);
+      col.m += static_cast<float>(more);
+      col.l = __builtin_amdgcn_ldexpf(col.l, -more);
 #pragma unroll
       for (int db = 0; db < DT / 32; ++db)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) col.o[db][i] *= less;
+        for (int i = 0; i < 16; ++i) col.o[db][i] = __builtin_amdgcn_ldexpf(col.o[db][i], -more);
     }
     const bool cut = key0 + kKeys - 1 > full;
     auto hide = [&](f32x16 (&x)[2], float with) {

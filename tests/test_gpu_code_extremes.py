@@ -1,5 +1,6 @@
-"""Attention over codes of rows whose sums are not finite: against 64 bits, and the
-same with contexts in one part and in many."""
+"""Attention over codes of rows whose sums are not finite, or whose scales rise by
+more powers of two than one fp32 factor spans: against 64 bits, and the same with
+contexts in one part and in many."""
 import math
 
 import pytest
@@ -101,3 +102,23 @@ def test_scores_of_minus_infinity(new, context, past, dtype, code):
     for longest in (None, 1):
         got = A().paged_attention(q, kc, vc, table, ints([past]), offsets([new]), max_context=longest, **s)
         assert bool(got.isnan().all())
+
+
+# -------------------------------------------------------------- scales that rise --
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype,low,high", [(torch.bfloat16, -90, 90), (torch.bfloat16, -100, 110), (torch.bfloat16, -60, 70),
+                                            (torch.bfloat16, -119, 20), (torch.float16, -90, 3)])
+@pytest.mark.parametrize("new", [1, 5, 20, 140])
+def test_scales_that_rise_along_the_keys(new, dtype, low, high, code):
+    """Values of 2^low, then of 2^high, under equal scores and under ordinary ones:
+    the weights of the first ones stay in the sum that divides."""
+    q, kc, vc, table, s, rows = case((new,), (2048,), PAGE, 4, 2, 64, dtype, code)
+    k, ks, v, vs = rows[0]
+    vs = vs / vs.amax()
+    vs = torch.cat([vs[:1000] * 2.0 ** low, vs[1000:] * 2.0 ** high])
+    s["v_scale"][places(table, 0, 2048)] = vs
+    for queries in (torch.zeros_like(q), q):
+        want = attended(queries, k, ks, v, vs)
+        for longest in (None, 1):
+            check(A().paged_attention(queries, kc, vc, table, ints([2048]), offsets([new]), max_context=longest, **s), want)
