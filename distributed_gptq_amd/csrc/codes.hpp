@@ -10,9 +10,12 @@ namespace {
 template <int kCode>
 constexpr float kTop = kCode == GPTQ_CODE_I8 ? 127.0f : 448.0f;
 
-// Rows whose largest value is not above this have code and scale 0: the
-// reciprocal that codes are made with stays far inside fp32.
+// Rows whose largest value is not above this have code and scale 0.
 constexpr float kLeast = 0x1p-120f;
+
+// Rows whose largest value is below this are made kRaise as large, which is exact,
+// before they are divided by it: 448 over values up to 1.75 2^-120 is past fp32.
+constexpr float kSmall = 0x1p-64f, kRaise = 0x1p64f;
 
 // The largest scale whose product with the last code is a number of fp32 (the
 // largest value over top may round past it).

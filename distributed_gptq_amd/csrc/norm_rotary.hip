@@ -175,15 +175,19 @@ __device__ __forceinline__ void store_cached(const CacheRows& r, int64_t page, i
     constexpr float top = kTop<kStore>;
     const bool finite = most < INFINITY;
     const bool some = finite && most > kLeast;
-    const float inv = some ? top / most : 0.0f;
+    const float raise = most < kSmall ? kRaise : 1.0f;
+    const float inv = some ? top / (most * raise) : 0.0f;
     if (!unit.some) return;
     uint8_t* to = static_cast<uint8_t*>(r.p) + o;
     typedef uint32_t words __attribute__((ext_vector_type(N / 4)));
     words w0, w1;
 #pragma unroll
     for (int e = 0; e < N; e += 4) {
-      w0[e / 4] = finite ? encode4<kStore>(x[e], x[e + 1], x[e + 2], x[e + 3], inv) : 0u;
-      w1[e / 4] = finite ? encode4<kStore>(y[e], y[e + 1], y[e + 2], y[e + 3], inv) : 0u;
+      auto code = [&](const float (&z)[N]) {
+        return encode4<kStore>(z[e] * raise, z[e + 1] * raise, z[e + 2] * raise, z[e + 3] * raise, inv);
+      };
+      w0[e / 4] = finite ? code(x) : 0u;
+      w1[e / 4] = finite ? code(y) : 0u;
     }
     *reinterpret_cast<words*>(to + unit.first) = w0;
     *reinterpret_cast<words*>(to + unit.second) = w1;

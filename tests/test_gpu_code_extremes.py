@@ -1,6 +1,6 @@
 """Attention over codes of rows whose sums are not finite, or whose scales rise by
 more powers of two than one fp32 factor spans: against 64 bits, and the same with
-contexts in one part and in many."""
+contexts in one part and in many.  And the smallest rows that are quantised."""
 import math
 
 import pytest
@@ -122,3 +122,45 @@ def test_scales_that_rise_along_the_keys(new, dtype, low, high, code):
         want = attended(queries, k, ks, v, vs)
         for longest in (None, 1):
             check(A().paged_attention(queries, kc, vc, table, ints([2048]), offsets([new]), max_context=longest, **s), want)
+
+
+# ----------------------------------------------------------- the smallest rows --
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_above_the_smallest_that_are_quantised(dtype, code):
+    """Rows whose largest value is a little above 2^-120, beside zeros and values
+    below fp32's normal range: the codes of the same rows 2^64 as large, and finite
+    rows read back; up to 2^-120 zeros."""
+    m, D, n = A(), 32, 40
+    g = gen(11)
+    x = torch.randn(n, 1, D, generator=g, device="cuda").clamp(-1, 1)
+    x[:, 0, 3:9] = 0.0
+    x[:, 0, 9] *= 2.0 ** -15
+    top = 2.0 ** torch.linspace(0, 4, n, device="cuda").double()
+    x[:, 0, 11] = 1.0
+    small = (x.double() * top[:, None, None] * 2.0 ** -120).to(dtype)
+    small[0] = small[0].sign() * 2.0 ** -120       # not above the border
+    big = (small.double() * 2.0 ** 64).to(dtype)
+    assert torch.equal(small.double() * 2.0 ** 64, big.double())
+
+    def write(y):
+        (kc, ks), (vc, vs) = (empty_cache(1, n, 1, D, code) for _ in "kv")
+        m.rotary_append(y, y, y, None, None, kc, vc, torch.arange(n, device="cuda"), k_scale=ks, v_scale=vs)
+        table, cu = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), ints([0, n])
+        back = m.cached_rows(kc, vc, table, ints([n]), cu, n, torch.float32, k_scale=ks, v_scale=vs)
+        assert torch.equal(kc.view(torch.int8), vc.view(torch.int8)) and torch.equal(ks, vs) and torch.equal(*back)
+        return kc[0], ks[0], back[0]
+    got, want = write(small), write(big)
+    assert bool((got[0][0].float() == 0).all()) and float(got[1][0]) == 0.0   # (e4m3 has a -0 too)
+    assert torch.equal(got[0][1:].view(torch.int8), want[0][1:].view(torch.int8))
+    # (scales and products end at 2^-149; 2^-21 of the largest for the code's product)
+    assert bool(((got[1][1:].double() * 2.0 ** 64 - want[1][1:].double()).abs() <= 2.0 ** -85).all())
+    err = (got[2][1:].double() - small[1:].double()).abs()
+    most = small[1:].double().abs().amax(-1, keepdim=True)
+    if code == torch.int8:   # half a step, and what the scale's end leaves of the largest code
+        bound = most / 254 * (1 + 2.0 ** -18) + 127 * 2.0 ** -149 + 2.0 ** -21 * most
+    else:
+        bound = torch.maximum(2.0 ** -4 * small[1:].double().abs(), most / 448 * 2.0 ** -10) * (1 + 2.0 ** -18)
+        bound = bound + 449 * 2.0 ** -149 + 2.0 ** -21 * most
+    assert bool((err <= bound).all())
