@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256, 4) void norm_rotary_kernel(NormArgs a, int lan
     if (weight) {
       const float r = rms_inverse<N>(x, y, a, lanes);
 #pragma unroll
-      for (int e = 0; e < N; ++e) x[e] *= r * wx[e], y[e] *= r * wy[e];
+      for (int e = 0; e < N; ++e) x[e] = x[e] * r * wx[e], y[e] = y[e] * r * wy[e];  // (r w may leave fp32 where x r w does not)
     }
     if (turns) turn<N>(x, y, c, s, a.interleaved);
     if (kind == 0 || !a.slots) {
