@@ -5,11 +5,16 @@
 // The 16-bit types hold every code exactly, so both products run on their MFMA
 // with the codes as they are, and the scales, one a key, go into the scores and
 // into the weights.  The weights times scales are rounded to the queries' type;
-// their unrounded sum divides.
+// their unrounded sum divides.  Of few rows what that leaves is multiplied too (a
+// decode step waits for the cache's bytes); of many rows it is not, as over a cache of
+// 16-bit values: each weight is off by no more than the output's own rounding, and the
+// second product takes a quarter more time (512 tokens over 16896, bf16: 193 us, error
+// against 64 bits 0.0016; without it 152 us, 0.0023; the output's rounding 0.0016).
 //
 // Both sums are kept 2^-e as large, with e a wave's own that follows the scales: it
 // is added to m, and leaves the quotient.  The sums of values of any size then stay
-// inside fp32, and fp16 weights inside their 16 bits.
+// inside fp32, and fp16 weights inside their 16 bits; what is lost below is small beside
+// the largest scale so far.
 #include "attn_join.hpp"
 #include "attn_tile.hpp"
 #include "codes.hpp"
@@ -188,7 +193,7 @@ __device__ __forceinline__ float inverse_sum(const AttnArgs& a, float l, bool no
 // over 8 of 128, e4m3, 277 MB) 51 us and 4 for the join, 5.4 TB/s; 48 sequences of
 // 200 to 1939 tokens over 40 heads (int8) 99.5 us, 5.5 TB/s.  24 sequences of 1 to
 // 8192 (int8, 163 MB) 43 us, 3.8 TB/s: their parts differ, and the longest end last.
-// One over 8192 takes 13.4 us, of which three dependent loads (lengths, block table,
+// One over 8192 takes 12.8 us, of which three dependent loads (lengths, block table,
 // rows), two joins and two launches are the larger part.
 constexpr int kFew = 32;
 
@@ -654,8 +659,8 @@ __global__ __launch_bounds__(256, NQ == 1 ? 3 : 2) void code_few_kernel(CodeArgs
 // new tokens over 16896, heads 32 over 8 of 128, bf16 over e4m3 (140 GFLOP): 144 us
 // and 8 us for the join, 915 TFLOP/s; with the join 177 us with 128 rows and all waves
 // in step, 161 us with 256 rows in step, 154.6 us with the largest score looked for in
-// every tile.  Cycles of a tile (of the last of these): 1980 for its weights, 1700 for
-// its products and staging, 450 at both barriers.
+// every tile.  Cycles of a tile: 1880 for its weights, 1720 for its products and
+// staging, 420 at both barriers.
 constexpr int kKeys = 64;
 constexpr int kChunk = kKeys * 16 + 64;
 template <int DT>

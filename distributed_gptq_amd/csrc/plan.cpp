@@ -294,12 +294,26 @@ size_t paged_workspace(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, i
 // new tokens for each of 4 sequences over 4096 91.3 / 87.8, 80 for each 61.4 / 51.0,
 // 64 for each of 4 over 2048 37.6 / 38.6, 40 of one over 8192 30.5 / 34.2, 32 for
 // each of 16 over 2048 43.5 / 49.9).  Of 33 to 64 rows, two tiles of 32 / one of 128:
-// 16 new tokens for each of 8 sequences over 4096 32.7 / 34.6, of one over 8192 23.4 /
-// 25.3, for each of 32 over 2048 65.8 / 57.7.
+// 16 new tokens for each of 8 sequences over 4096 31.7 / 34.9, of one over 8192 23.4 /
+// 25.3, for each of 32 over 2048 65.8 / 57.7.  Past 8 sequences neither side wins
+// throughout (16 over 4096 for each of 9 / 12 / 16 / 24 / 32: 47.5 55.1 58.9 90.7 96.2 /
+// 47.6 56.4 53.1 101 93.3; 9 over 2048: 35.3 39.2 38.5 52.1 56.2 / 30.0 31.2 32.9 59.2
+// 50.9), nor below with 40 key heads (48 over 2048 for each of 1 / 2 / 4 / 8: 27.5 30.5
+// 42.3 64.3 / 24.9 31.4 47.4 82.4).
 //
-// Of few rows, 512 workgroups or twice that of many sequences (us with the join, 512 /
-// 1024 wanted: 24 sequences of 1 to 8192 tokens 51.8 / 43.3, 8 of 2048 15.0 / 19.2,
-// one of 131072 55.8 / 60.6).
+// Of few rows, 512 workgroups or, above 8 sequences, twice that, which evens out
+// lengths that differ and costs equal ones up to a fifth: the lengths are on the GPU.
+// One token each, us with the join, 512 / 1024 wanted:
+//   sequences                        8     9     12    16    24    32    48
+//   up to 8192, 8 key heads  512   22.4  27.9  31.4  41.2  60.0  76.9  101
+//                           1024   25.7  26.9  31.2  36.9  51.0  64.1  87.0
+//   2048 each                512   15.6  18.4  20.2  23.9  28.4  37.5  46.4
+//                           1024   18.8  21.8  23.4  24.9  29.0  34.9  49.6
+//   8192 each                512         41.3  51.4  70.7  92.7
+//                           1024         43.3  51.6  61.1  86.3
+// 40 key heads, 2 / 4 / 8 / 16 sequences up to 8192: 35.7 52.1 86.8 156 / 33.2 52.0 80.5
+// 143, of 2048 each 18.4 25.6 42.9 73.3 / 21.6 28.4 42.1 69.1; one sequence of 131072
+// over 8 key heads 55.8 / 60.6.
 CodePlan code_plan(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t max_context) {
   CodePlan p;
   if (T == 0 || !attention_sizes(B, T, 0, H, Hk, D)) return p;

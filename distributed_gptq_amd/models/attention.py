@@ -204,7 +204,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``k_scale`` and ``v_scale``: those of a cache of codes (``rotary_append``),
     whose rows are code times scale; q is fp16 or bf16.  A row whose scale is NaN
     reaches the queries that see it only.  A value's code that is NaN, which
-    ``rotary_append`` never writes, may reach those before it too."""
+    ``rotary_append`` never writes, may reach those before it too.  One kernel, by
+    the average number of new tokens, takes all sequences: a long chunk beside many
+    single tokens is faster as a call for each kind."""
     if _needs_grad(q, k_cache, v_cache):
         raise RuntimeError("paged_attention records no gradient: call it under torch.no_grad()")
     if max_context is None:

@@ -541,7 +541,9 @@ int gptq_cached_rows(int code, const void* k_cache, int64_t k_page,
  * the codes as they are and of the queries; a weight times its value's scale is
  * rounded to the queries' type (for few rows to twice its bits) relative to the
  * largest scale so far.  Codes are numbers (not e4m3's NaN); a row that is not
- * finite has a scale that is NaN, which reaches only the queries that see it.
+ * finite has a scale that is NaN, which reaches only the queries that see it.  A
+ * query that is not finite gives NaN; scores below fp32's range have weights of 0,
+ * and NaN where all of a query's are.
  * Tokens of codes are less than 2^27 bytes apart. */
 size_t gptq_code_attention_workspace_size(int64_t B, int64_t T, int64_t H,
                                           int64_t Hk, int64_t D,
